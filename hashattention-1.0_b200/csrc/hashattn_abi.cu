@@ -11,6 +11,7 @@
 #include "common.cuh"
 #include "hash_decode.cuh"
 #include "hash_prefill_tc.cuh"
+#include "host.cuh"
 #include "lsh.cuh"
 #include "score_select.cuh"
 #include "select_attend.cuh"
@@ -31,18 +32,6 @@ bool g_options_ready = [] {
     return true;
 }();
 inline int option(int key) { return g_options[key].load(std::memory_order_relaxed); }
-
-int check_shape(const ha_shape_t* s) {
-    if (s == nullptr) return HA_ERR_BAD_ARG;
-    if (s->gqa_group != kGroup || s->head_dim != kHeadDim || s->page_size != kPage)
-        return HA_ERR_UNSUPPORTED_DIM;
-    if (s->batch < 1 || s->num_kv_heads < 1 || s->max_pages < 1 || s->num_pages < 1 ||
-        s->sel_stride < 1)
-        return HA_ERR_BAD_ARG;
-    if (s->batch > 65535 || s->num_kv_heads * kGroup > 65535 || s->max_pages > 65535)
-        return HA_ERR_UNSUPPORTED_DIM;
-    return HA_OK;
-}
 
 int check_budget(const ha_budget_t* b) {
     if (b == nullptr) return HA_ERR_BAD_ARG;
@@ -222,32 +211,6 @@ Workspace carve(const ha_shape_t* s, const ha_budget_t* b, void* base) {
     for (int cp = 4; cp <= kMaxChunkPages && (cp == 4 || s->max_pages > cp / 2); cp *= 2)
         w.bytes = std::max(w.bytes, carve_cut(s, b, geometry_of(s, cp), base).bytes);
     return w;
-}
-
-// Every kernel is launched with programmatic stream serialization (it may start while its
-// predecessor drains and synchronises itself with griddepcontrol.wait); cluster_x > 1 adds a
-// thread-block cluster along x.
-template <typename... KArgs, typename... Args>
-cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, cudaStream_t stream, int cluster_x,
-                   Args&&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = 0;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.numAttrs = 1;
-    if (cluster_x > 1) {
-        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-        attr[cfg.numAttrs].val.clusterDim.x = cluster_x;
-        attr[cfg.numAttrs].val.clusterDim.y = 1;
-        attr[cfg.numAttrs].val.clusterDim.z = 1;
-        ++cfg.numAttrs;
-    }
-    cfg.attrs = attr;
-    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
 // Kernels that keep more than a few KB of shared memory per CTA ask for a carve-out that holds a full SM's worth
@@ -731,30 +694,6 @@ int ha_hash_decode(const ha_shape_t* shape, const ha_hash_weights_t* weights,
                             q_codes, preact_dbg, nullptr, status, stream);
 }
 
-// cuTensorMapEncodeTiled, looked up once through the runtime (the library does not link against libcuda).
-static bool encode_key_map(CUtensorMap* map, const void* k_pages, uint64_t rows) {
-    typedef CUresult (*encode_fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static std::atomic<encode_fn> cached{nullptr};
-    encode_fn fn = cached.load();
-    if (fn == nullptr) {
-        void* sym = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess || sym == nullptr)
-            return false;
-        fn = reinterpret_cast<encode_fn>(sym);
-        cached.store(fn);
-    }
-    const cuuint64_t dims[2] = {(cuuint64_t)kHeadDim, rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)kHeadDim * sizeof(__nv_bfloat16)};
-    const cuuint32_t box[2] = {64, (cuuint32_t)kTcTile}, elem[2] = {1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(k_pages), dims, strides, box, elem,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 int ha_hash_prefill(const ha_shape_t* shape, const ha_hash_weights_t* weights,
                     const void* k_pages, uint32_t* hash_pages,
                     const int32_t* page_table, const int32_t* seq_lens,
@@ -807,7 +746,7 @@ int ha_hash_prefill(const ha_shape_t* shape, const ha_hash_weights_t* weights,
         // the key cache as a 2-d tensor [rows = pages x kv heads x page size][128] for the kernel's TMA loads: boxes of
         // 64 elements x 128 rows, 128-byte swizzle
         CUtensorMap k_map;
-        if (!encode_key_map(&k_map, k_pages, (uint64_t)shape->num_pages * shape->num_kv_heads * kPage)) return HA_ERR_LAUNCH;
+        if (!encode_row_map(&k_map, k_pages, (uint64_t)shape->num_pages * shape->num_kv_heads * kPage, kTcTile)) return HA_ERR_LAUNCH;
         // one CTA per SM; the kernel cuts the (head, tile) pairs into that many ranges of equal cost
         const int Hq = shape->num_kv_heads * kGroup;
         const long long tiles = (long long)Hq * shape->batch * shape->max_pages * (kPage / kTcTile);
