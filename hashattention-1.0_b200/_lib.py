@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_size_t, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libhashattn.so")
@@ -31,6 +31,7 @@ HA_EVAL_DEPTH = 1
 HA_OPT_CLUSTER_GATHER = 0
 HA_OPT_CLUSTER_SELECT = 1
 HA_OPT_PLAN_HANDOVER = 2
+HA_MAX_TREE_NODES = 128
 
 
 class HaShape(ctypes.Structure):
@@ -50,8 +51,13 @@ class HaHashWeights(ctypes.Structure):
                 ("num_layers", c_int32), ("lsh_state", c_void_p)]
 
 
+class HaTree(ctypes.Structure):
+    _fields_ = [("max_nodes", c_int32), ("tree_lens", c_void_p), ("tree_mask", c_void_p)]
+
+
 _P = c_void_p
-_S, _B, _W = POINTER(HaShape), POINTER(HaBudget), POINTER(HaHashWeights)
+_S, _B, _W, _T = POINTER(HaShape), POINTER(HaBudget), POINTER(HaHashWeights), POINTER(HaTree)
+_I64 = POINTER(c_int64)
 
 # name -> (restype, argtypes); one entry per function declared in include/hashattn.h
 PROTOTYPES = {
@@ -78,6 +84,13 @@ PROTOTYPES = {
     "ha_rope_split": (c_int, [_P, _P, c_int32, c_int32, c_int32, c_float, _P, _P, _P, _P]),
     "ha_decode_step_host": (c_int, [_S, _B, _W, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
                                     _P, _P, _P, c_float, _P, c_size_t, _P, _P, c_int]),
+    "ha_tree_workspace_bytes": (c_size_t, [c_int32]),
+    "ha_tree_mask": (c_int, [_P, _P, c_int32, c_int32, _P, _P, _P]),
+    "ha_tree_attention": (c_int, [_S, _T, _P, _I64, _P, _P, _P, _P, c_float, _P, _P, _P, c_size_t, _P, _P]),
+    "ha_attention_mass": (c_int, [_S, _T, _P, _I64, _P, _P, _P, _P, _P, c_float, _P, _P, _P]),
+    "ha_tree_accept": (c_int, [_P, _P, _P, _P, _P, c_int32, c_int32, _P, _P, _P, _P, _P, _P]),
+    "ha_tree_commit": (c_int, [_S, _T, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "ha_cache_evict": (c_int, [_S, c_int32, c_int32, c_int32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
 }
 
 _lib = None

@@ -1,0 +1,413 @@
+// Dense attention of a few query rows per kv-head over the paged cache (a decode step's token, or a small drafted tree), and
+// the merge of partial results.
+//
+//   o_i = sum_j e^{c q_i.k_j - lse_i} v_j,   lse_i = log sum_j e^{c q_i.k_j},   j over the tokens that row i sees
+//
+// in one pass over K and V with a running maximum and sum per row. A CTA takes a range of token tiles (DenseCut) of 64 tokens:
+// 32 KB of K and V, copied by TMA in the 128-byte swizzle into a ring of stages. Four warps take 16 tokens of a tile each and
+// keep a maximum, a sum and 16 (or 32) x 128 sums of their own; they meet at the end of a unit only.
+//
+// The products run on the warps' matrix instructions (m16n8k16, bf16 with fp32 sums): with 4 to 32 query rows, of which a tcgen05
+// tile of 128 would be mostly padding, the bytes of K and V bound the kernel and not the products. The weights e^{s - m} are
+// handed to the second product as two bf16 (hi + lo, 16 bits of mantissa), so that their rounding does not show beside
+// the one of the bf16 output. The maximum a row's weights refer to moves only when a score passes it by more than 2^8: the
+// sums are fp32 and do not mind, and rescaling 16 x 128 of them at every new maximum would.
+//
+// Tokens that a row does not see are taken out by selection, not by a weight of zero: an infinity or NaN in the K or V of a
+// token that only other branches of the tree see stays with those.
+#pragma once
+
+#include "dense_common.cuh"
+
+namespace ha {
+
+struct TreeAttentionParams {
+    DenseSeqs seqs;
+    const __nv_bfloat16* q;  // [B][T][Hq][128], strides in elements
+    long long q_batch, q_node, q_head;
+    __nv_bfloat16* out;      // [B][T][Hq][128]
+    float* lse;              // [B][T][Hq] or null
+    float2* part_ml;         // [2 * CTAs][rows] maximum (in powers of two) and sum of each partial result
+    float* part_acc;         // [2 * CTAs][rows][128]
+    float scale_log2;        // c * log2(e)
+};
+
+constexpr int kRowsTile = 64;            // tokens per tile
+constexpr int kRowsWarps = 4;            // consumer warps, 16 tokens each
+constexpr int kRowsThreads = (kRowsWarps + 1) * 32;
+constexpr uint32_t kRowsHalf = kRowsTile * 128;      // 64 rows x 64 elements
+constexpr uint32_t kRowsStage = 4 * kRowsHalf;       // K and V of a tile: 32 KB
+constexpr float kRescaleAt = 8.0f;       // a row's weights may grow to 2^8 before its sums are rescaled
+
+template <int MT>  // 16-row tiles of query rows
+struct RowsLayout {
+    static constexpr int kRows = 16 * MT;
+    static constexpr int kStages = MT == 1 ? 5 : 4;
+    static constexpr int kAccPitch = kHeadDim + 4;
+    static constexpr uint32_t kOffAcc = kStages * kRowsStage;                               // [4 warps][kRows][kAccPitch] floats
+    static constexpr uint32_t kOffMl = kOffAcc + kRowsWarps * kRows * kAccPitch * 4;        // [4 warps][kRows] float2
+    static constexpr uint32_t kOffBar = kOffMl + kRowsWarps * kRows * 8;
+    static constexpr uint32_t kOffAbort = kOffBar + 2 * kStages * 8;
+    static constexpr uint32_t kSmemBytes = kOffAbort + 16 + 1024;  // + slack to align the base to 1024 B
+    static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 16-byte chunk `chunk` (0..15) of row `row` of a tile of kRowsTile rows: two halves of 64 elements, 128-byte swizzle
+__device__ __forceinline__ uint32_t rows_at(uint32_t row, uint32_t chunk) {
+    return (chunk >> 3) * kRowsHalf + row * 128u + (((chunk & 7u) ^ (row & 7u)) << 4);
+}
+__device__ __forceinline__ bool any_nonfinite(uint4 w) {
+    auto bad = [](uint32_t x) { return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u; };
+    return bad(w.x) || bad(w.y) || bad(w.z) || bad(w.w);
+}
+
+// The output row and log-sum-exp of (sequence, node, query head): 4 dimensions per lane.
+__device__ __forceinline__ void store_row(const TreeAttentionParams& p, int b, int node, int qh, int lane, float4 acc, float M, float L) {
+    const size_t row = ((size_t)b * p.seqs.T + node) * ((size_t)p.seqs.Hkv * kGroup) + qh;
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // a row that sees nothing: zeros
+    uint2 w;
+    w.x = tc_pack_bf16(acc.x * inv, acc.y * inv);
+    w.y = tc_pack_bf16(acc.z * inv, acc.w * inv);
+    reinterpret_cast<uint2*>(p.out + row * kHeadDim)[lane] = w;
+    if (lane == 0 && p.lse != nullptr) p.lse[row] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+}
+
+template <int MT>
+__global__ void __launch_bounds__(kRowsThreads, 1)
+tree_attention_rows_kernel(const TreeAttentionParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+    using L = RowsLayout<MT>;
+    using Cursor = DenseCursor<kRowsTile, L::kRows>;
+    extern __shared__ unsigned char rows_smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(rows_smem_raw) + 1023) & ~(uintptr_t)1023);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t sbase = tc_smem_u32(smem), bars = sbase + L::kOffBar;
+    volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::kOffAbort);
+    auto full = [&](uint32_t s) { return bars + 8u * s; };
+    auto empty = [&](uint32_t s) { return bars + 8u * (L::kStages + s); };
+    if (tid == 0) {
+        for (uint32_t s = 0; s < (uint32_t)L::kStages; ++s) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full(s)));
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(empty(s)), "r"(kRowsWarps));
+        }
+        *s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
+    }
+    __syncthreads();
+    pdl_wait();
+    pdl_launch_dependents();
+
+    Cursor cur(p.seqs, lane, blockIdx.x == 0 && warp == 0);
+    DenseSegment seg;
+    uint32_t it = 0;  // tiles so far: stage it % kStages, phase it / kStages
+    if (warp == kRowsWarps) {
+        // ---- the loading warp: lane l holds the l-th page of a window of 32; one lane copies -------------------------
+        bool ok = true;
+        while (ok && cur.next(seg)) {
+            int base = -64, page_l = 0;
+            for (int t = seg.tile0; t < seg.tile1 && ok; ++t, ++it) {
+                const int pi = t / (kPage / kRowsTile);
+                if (pi - base >= 32) {
+                    base = pi;
+                    page_l = (base + lane) * kPage < seg.S ? dense_page(p.seqs, seg.b, base + lane) : 0;
+                }
+                const int page = __shfl_sync(0xffffffffu, page_l, pi - base);
+                if (lane == 0) {
+                    const uint32_t s = it % L::kStages, dst = sbase + s * kRowsStage;
+                    ok = tc_wait(empty(s), ((it / L::kStages) & 1) ^ 1, s_abort, p.seqs.status);
+                    if (ok) {
+                        const int y = (int)(((size_t)page * p.seqs.Hkv + seg.kvh) * kPage) + (t % (kPage / kRowsTile)) * kRowsTile;
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full(s)), "r"(kRowsStage) : "memory");
+                        tc_tma_load(dst, &k_map, 0, y, full(s));
+                        tc_tma_load(dst + kRowsHalf, &k_map, 64, y, full(s));
+                        tc_tma_load(dst + 2 * kRowsHalf, &v_map, 0, y, full(s));
+                        tc_tma_load(dst + 3 * kRowsHalf, &v_map, 64, y, full(s));
+                    }
+                }
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (!ok) break;  // (tile `it` was not issued)
+            }
+        }
+        // no copy is left in flight when the CTA ends (they have all landed unless the CTA gave up early)
+        if (lane == 0)
+            for (uint32_t j = it > (uint32_t)L::kStages ? it - L::kStages : 0; j < it; ++j)
+                for (int spin = 0; spin < (1 << 22) && !tc_test(full(j % L::kStages), (j / L::kStages) & 1); ++spin) {}
+        return;
+    }
+
+    // ---- consumer warps ----------------------------------------------------------------------------------------------
+    // A warp that gives up (another one's time-out included) goes on through the segments without waiting, so that
+    // the barriers below are reached by all four.
+    bool ok = true;
+    float* s_acc = reinterpret_cast<float*>(smem + L::kOffAcc);
+    float2* s_ml = reinterpret_cast<float2*>(smem + L::kOffMl);
+    const uint32_t k_row = (uint32_t)(warp * 16 + ((lane >> 4) << 3) + (lane & 7)), k_chunk = (uint32_t)((lane >> 3) & 1);
+    const uint32_t v_row = (uint32_t)(warp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7)), v_chunk = (uint32_t)(lane >> 4);
+    while (cur.next(seg)) {
+        const int P = seg.S - seg.n, row0 = seg.group * L::kRows;
+        uint32_t qa[MT][8][4];  // the query rows as the A operand: rows lane / 4 and + 8, elements 2 (lane % 4) and + 8
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = row0 + mt * 16 + h * 8 + (lane >> 2);
+                const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + seg.b * p.q_batch + (r >> 2) * p.q_node +
+                                                                        (seg.kvh * kGroup + (r & 3)) * p.q_head) + (lane & 3);
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks) {
+                    qa[mt][ks][h] = r < seg.n * kGroup ? __ldg(src + ks * 8) : 0u;
+                    qa[mt][ks][h + 2] = r < seg.n * kGroup ? __ldg(src + ks * 8 + 4) : 0u;
+                }
+            }
+        float o[MT][16][4] = {};
+        float m[MT][2], l[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) m[mt][h] = -INFINITY, l[mt][h] = 0.0f;
+
+        for (int t = seg.tile0; t < seg.tile1; ++t, ++it) {
+            const uint32_t s = it % L::kStages, kb = sbase + s * kRowsStage, vb = kb + 2 * kRowsHalf;
+            if (ok) ok = __all_sync(0xffffffffu, tc_wait(full(s), (it / L::kStages) & 1, s_abort, p.seqs.status)) != 0;
+            if (!ok) continue;
+            const int tok0 = t * kRowsTile + warp * 16;
+            float c[MT][2][4] = {};
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) {
+                uint32_t kf[4];
+                ldmatrix4(kb + rows_at(k_row, 2 * ks + k_chunk), kf);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    mma16816(c[mt][0], qa[mt][ks], kf[0], kf[1]);
+                    mma16816(c[mt][1], qa[mt][ks], kf[2], kf[3]);
+                }
+            }
+            uint32_t vkeep[2] = {0xffffffffu, 0xffffffffu}, bad = 0;  // V values to use; tokens of the tree with an infinity or NaN in V
+            if (tok0 + 16 > P) {
+                // tokens of the tree or behind the sequence's end
+                bool nonfinite = false;
+                const int vt = lane >> 1;
+                if (tok0 + vt >= P && tok0 + vt < seg.S) {
+#pragma unroll
+                    for (int ch = 0; ch < 8; ++ch)
+                        nonfinite |= any_nonfinite(*reinterpret_cast<const uint4*>(smem + (vb - sbase) + rows_at(warp * 16 + vt, (lane & 1) * 8 + ch)));
+                }
+                const uint32_t votes = __ballot_sync(0xffffffffu, nonfinite);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) bad |= ((votes >> (2 * i)) & 3u) != 0 ? 1u << i : 0u;
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int tk = nt * 8 + (lane & 3) * 2 + e;
+                        if (tok0 + tk >= seg.S || ((bad >> tk) & 1u)) vkeep[nt] &= e ? 0x0000ffffu : 0xffff0000u;
+                    }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int node = (row0 + mt * 16 + h * 8 + (lane >> 2)) >> 2;
+                        const uint4 words = node < seg.n ? dense_mask(p.seqs, seg.b, node) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int j = tok0 + nt * 8 + (lane & 3) * 2 + e;
+                                if (j >= seg.S || (j >= P && !dense_bit(words, j - P))) c[mt][nt][2 * h + e] = -INFINITY;
+                            }
+                    }
+            }
+            uint32_t ph[MT][4], pl[MT][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                bool grow = false;
+                float alpha[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float x = fmaxf(fmaxf(c[mt][0][2 * h], c[mt][0][2 * h + 1]), fmaxf(c[mt][1][2 * h], c[mt][1][2 * h + 1]));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2)) * p.scale_log2;
+                    alpha[h] = 1.0f;
+                    if (x > m[mt][h] + kRescaleAt) {  // (from -inf: any score at all)
+                        alpha[h] = exp2_approx(m[mt][h] - x);
+                        m[mt][h] = x;
+                        grow = true;
+                    }
+                }
+                if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                    for (int dt = 0; dt < 16; ++dt) {
+                        o[mt][dt][0] *= alpha[0]; o[mt][dt][1] *= alpha[0];
+                        o[mt][dt][2] *= alpha[1]; o[mt][dt][3] *= alpha[1];
+                    }
+                    l[mt][0] *= alpha[0];
+                    l[mt][1] *= alpha[1];
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float ref = m[mt][h] == -INFINITY ? 0.0f : m[mt][h];
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt) {
+                        const float p0 = exp2_approx(fmaf(c[mt][nt][2 * h], p.scale_log2, -ref));
+                        const float p1 = exp2_approx(fmaf(c[mt][nt][2 * h + 1], p.scale_log2, -ref));
+                        l[mt][h] += p0 + p1;
+                        const uint32_t hi = tc_pack_bf16(p0, p1);
+                        ph[mt][2 * nt + h] = hi;
+                        pl[mt][2 * nt + h] = tc_pack_bf16(p0 - bf16_lo(hi), p1 - bf16_hi(hi));
+                        c[mt][nt][2 * h] = p0;
+                        c[mt][nt][2 * h + 1] = p1;
+                    }
+                }
+            }
+#pragma unroll
+            for (int dt = 0; dt < 16; dt += 2) {
+                uint32_t vf[4];
+                ldmatrix4_trans(vb + rows_at(v_row, dt + v_chunk), vf);
+                vf[0] &= vkeep[0]; vf[1] &= vkeep[1]; vf[2] &= vkeep[0]; vf[3] &= vkeep[1];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    mma16816(o[mt][dt], ph[mt], vf[0], vf[1]);
+                    mma16816(o[mt][dt + 1], ph[mt], vf[2], vf[3]);
+                    mma16816(o[mt][dt], pl[mt], vf[0], vf[1]);
+                    mma16816(o[mt][dt + 1], pl[mt], vf[2], vf[3]);
+                }
+            }
+            if (bad != 0) {
+                // V rows with an infinity or NaN, one by one, for the rows that see them
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        for (int w = 0; w < 4; ++w) {
+                            const int tk = nt * 8 + 2 * w + e;
+                            if (((bad >> tk) & 1u) == 0) continue;
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const float pv = __shfl_sync(0xffffffffu, c[mt][nt][2 * h + e], (lane & ~3) | w);
+                                    const int node = (row0 + mt * 16 + h * 8 + (lane >> 2)) >> 2;
+                                    if (node >= seg.n || !dense_bit(dense_mask(p.seqs, seg.b, node), tok0 + tk - P)) continue;
+#pragma unroll
+                                    for (int dt = 0; dt < 16; ++dt) {
+                                        const uint32_t w2 = *reinterpret_cast<const uint32_t*>(smem + (vb - sbase) + rows_at(warp * 16 + tk, dt) + (lane & 3) * 4);
+                                        o[mt][dt][2 * h] = fmaf(pv, bf16_lo(w2), o[mt][dt][2 * h]);
+                                        o[mt][dt][2 * h + 1] = fmaf(pv, bf16_hi(w2), o[mt][dt][2 * h + 1]);
+                                    }
+                                }
+                            __syncwarp();
+                        }
+            }
+            __syncwarp();
+            if (lane == 0) tc_arrive(empty(s));
+        }
+
+        // ---- the four warps' results: one row at a time per warp ------------------------------------------------------
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = mt * 16 + h * 8 + (lane >> 2);
+                float sum = l[mt][h];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                if ((lane & 3) == 0) s_ml[warp * L::kRows + r] = make_float2(m[mt][h], sum);
+                float* dst = s_acc + (size_t)(warp * L::kRows + r) * L::kAccPitch + (lane & 3) * 2;
+#pragma unroll
+                for (int dt = 0; dt < 16; ++dt) *reinterpret_cast<float2*>(dst + dt * 8) = make_float2(o[mt][dt][2 * h], o[mt][dt][2 * h + 1]);
+            }
+        asm volatile("bar.sync 1, %0;" ::"n"(kRowsWarps * 32) : "memory");
+        const int rows = min(L::kRows, seg.n * kGroup - row0);
+        for (int r = warp; r < rows; r += kRowsWarps) {
+            float2 ml[kRowsWarps];
+            float M = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kRowsWarps; ++w) {
+                ml[w] = s_ml[w * L::kRows + r];
+                M = fmaxf(M, ml[w].x);
+            }
+            const float ref = M == -INFINITY ? 0.0f : M;
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kRowsWarps; ++w) {
+                const float f = exp2_approx(ml[w].x - ref);
+                const float4 a = *reinterpret_cast<const float4*>(s_acc + (size_t)(w * L::kRows + r) * L::kAccPitch + lane * 4);
+                sum = fmaf(ml[w].y, f, sum);
+                acc.x = fmaf(a.x, f, acc.x); acc.y = fmaf(a.y, f, acc.y);
+                acc.z = fmaf(a.z, f, acc.z); acc.w = fmaf(a.w, f, acc.w);
+            }
+            if (seg.whole()) {
+                if (ok) store_row(p, seg.b, (row0 + r) >> 2, seg.kvh * kGroup + ((row0 + r) & 3), lane, acc, M, sum);
+            } else {
+                const size_t at = (size_t)(2 * blockIdx.x + seg.slot) * L::kRows + r;
+                if (lane == 0) p.part_ml[at] = make_float2(M, sum);
+                reinterpret_cast<float4*>(p.part_acc + at * kHeadDim)[lane] = acc;
+            }
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(kRowsWarps * 32) : "memory");
+    }
+}
+
+// The partial results of the units that several CTAs share, a warp per query row; grid (Hkv * groups of T, B, rows / 4).
+constexpr int kTreeMergeWarps = 4;
+template <int kTile, int kRows>
+__global__ void __launch_bounds__(kTreeMergeWarps * 32) tree_merge_kernel(const TreeAttentionParams p, int ctas) {
+    using Cut = DenseCut<kTile, kRows>;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31, r = blockIdx.z * kTreeMergeWarps + (threadIdx.x >> 5), b = blockIdx.y;
+    const int max_groups = Cut::groups(p.seqs.T);
+    const int kvh = blockIdx.x / max_groups, group = blockIdx.x - kvh * max_groups;
+    int S, n;
+    dense_seq(p.seqs, b, false, S, n);
+    const int row = group * kRows + r;
+    if (row >= n * kGroup) return;
+    long long quota, before;
+    Cut::count(p.seqs, ctas, lane, b, quota, before);
+    const int tiles = (S + kTile - 1) / kTile;
+    const long long start = before + (long long)(kvh * Cut::groups(n) + group) * tiles;
+    const int c0 = (int)(start / quota), c1 = (int)((start + tiles - 1) / quota);
+    if (c0 == c1) return;  // one CTA had the whole unit
+    auto at = [&](int c) { return (size_t)(2 * c + (c == c0 && c0 * quota != start ? 1 : 0)) * kRows + r; };
+
+    float M = -INFINITY;
+    for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, __ldcg(&p.part_ml[at(c)]).x);
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, i));
+    const float ref = M == -INFINITY ? 0.0f : M;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float sum = 0.0f;
+    for (int cb = c0; cb <= c1; cb += 32) {
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        if (cb + lane <= c1) ml = __ldcg(&p.part_ml[at(cb + lane)]);
+        const float f = cb + lane <= c1 ? exp2_approx(ml.x - ref) : 0.0f;
+        float part = ml.y * f;  // (the sums of 32 partials in an order that is always the same)
+#pragma unroll
+        for (int i = 16; i > 0; i >>= 1) part += __shfl_xor_sync(0xffffffffu, part, i);
+        sum += part;
+        const int count = min(32, c1 - cb + 1);
+#pragma unroll 4
+        for (int i = 0; i < count; ++i) {
+            const float w = __shfl_sync(0xffffffffu, f, i);
+            const float4 a = __ldcg(reinterpret_cast<const float4*>(p.part_acc + at(cb + i) * kHeadDim) + lane);
+            acc.x = fmaf(a.x, w, acc.x); acc.y = fmaf(a.y, w, acc.y);
+            acc.z = fmaf(a.z, w, acc.z); acc.w = fmaf(a.w, w, acc.w);
+        }
+    }
+    store_row(p, b, row >> 2, kvh * kGroup + (row & 3), lane, acc, M, sum);
+}
+
+}  // namespace ha

@@ -322,6 +322,82 @@ int ha_decode_step_host(const ha_shape_t* shape, const ha_budget_t* budget,
 int ha_rope_split(const void* qkv, const int64_t* positions, int32_t batch, int32_t num_q_heads,
                   int32_t num_kv_heads, float rope_theta, void* q, void* k_new, void* v_new, void* stream);
 
+/* ---- dense attention over the paged cache, and what goes with it ------------------------------------------------------
+ * (No counterpart in the reference, whose decode attends the selected tokens only.) Uses: the dense step beside the sparse
+ * one; verification of a tree of drafted tokens, for instance tokens drafted by the sparse step, with full attention over the
+ * same cache; the attention weight that each cached token has received, and eviction by it.
+ *
+ * A sequence's last n tokens are its drafted tree: seq_lens[b] counts them, their K / V rows (and codes) lie in the cache
+ * at the tokens P = seq_lens[b] - n, P + 1, ... (ha_hash_decode on rows, or the caller, has put them there). Node i is the
+ * token P + i; a parent comes before its children. One new token per sequence is a tree of one node.
+ * Sequences with n == 0 are left out: nothing of theirs is read or written. Lengths out of range (n < 0 or > max_nodes,
+ * seq_len < n or beyond max_pages * page_size) are reported as HA_ERR_BAD_SEQ_LEN and left out too.
+ * sel_stride of the shape is not used by these entry points (any value >= 1). ha_tree_mask and ha_tree_accept, which have no
+ * context to report to, take status == NULL too.                                                                       */
+#define HA_MAX_TREE_NODES 128
+typedef struct ha_tree {
+    int32_t max_nodes;          /* T: columns of the tree arrays, 1 .. HA_MAX_TREE_NODES                          */
+    const int32_t* tree_lens;   /* [batch] drafted tokens n of each sequence, or NULL: max_nodes                  */
+    const uint32_t* tree_mask;  /* [batch][max_nodes][4] bit j of node i: node i sees node j (j >= n: ignored); every node
+                                 * sees the whole prefix. NULL: a chain, node i sees the nodes 0 .. i              */
+} ha_tree_t;
+
+/* Workspace of ha_tree_attention for trees of up to max_nodes nodes (0 if out of range); it needs no initialisation and keeps
+ * nothing between calls. Host-only arithmetic. One workspace per concurrently running call.                             */
+size_t ha_tree_workspace_bytes(int32_t max_nodes);
+
+/* Mask words of trees given by their parents [batch][max_nodes] (-1: a root): each node sees its ancestors and itself. Rows
+ * behind a tree's own are zero. A parent that does not come before its child is reported (HA_ERR_BAD_ARG in the status
+ * word) and taken as -1.                                                                                            */
+int ha_tree_mask(const int32_t* parents, const int32_t* tree_lens, int32_t batch, int32_t max_nodes,
+                 uint32_t* tree_mask, int32_t* status, void* stream);
+
+/* out[b][i][h] = softmax(sm_scale * q[b][i][h] . K) V over the prefix and the nodes that node i sees, fp32 sums, bf16 output;
+ * lse (optional) [batch][max_nodes][num_q_heads] f32: the natural log of the sum of e^(scaled scores). Rows of nodes behind
+ * a tree's own are left as they were. A row that sees nothing (or only scores of -inf) gives zeros and an lse of -inf.
+ * q [batch][max_nodes][num_q_heads][128] bf16 with strides q_strides[3] = {batch, node, head} in elements (HOST array;
+ * multiples of 8, the 128 elements of a row contiguous), or contiguous if NULL: a view of a fused projection will do.
+ * out is contiguous. sm_scale > 0.                                                                                  */
+int ha_tree_attention(const ha_shape_t* shape, const ha_tree_t* tree, const void* q, const int64_t* q_strides,
+                      const void* k_pages, const void* v_pages, const int32_t* page_table, const int32_t* seq_lens,
+                      float sm_scale, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                      int32_t* status, void* stream);
+
+/* mass[b][j][t] += sum over the counted nodes i and the query heads h of kv-head j of the weight e^(score - lse[b][i][h])
+ * that cached token t has in row (i, h); mass [batch][num_kv_heads][max_pages * page_size] f32. rows (optional) [batch][4]:
+ * the nodes whose weights count, one bit each (an accepted path); NULL: all of the tree. q, q_strides, sm_scale, the tree
+ * and lse as ha_tree_attention took and left them. Rows with an lse of -inf count for nothing.                      */
+int ha_attention_mass(const ha_shape_t* shape, const ha_tree_t* tree, const void* q, const int64_t* q_strides,
+                      const float* lse, const uint32_t* rows, const void* k_pages, const int32_t* page_table,
+                      const int32_t* seq_lens, float sm_scale, float* mass, int32_t* status, void* stream);
+
+/* Greedy acceptance: from node 0 (the token that is certain) on, the lowest child whose drafted token is the target token of
+ * its parent (target[b][i]: the token the model puts behind node i). draft, target [batch][max_nodes] int64, parents as
+ * ha_tree_mask takes them. accepted [batch][4] <- the path's nodes, one bit each; count[b] <- their number; next_token[b] <-
+ * the target of the path's last node (untouched where n == 0); new_lens[b] <- seq_lens[b] - n + count[b].               */
+int ha_tree_accept(const int64_t* draft, const int32_t* parents, const int64_t* target, const int32_t* tree_lens,
+                   const int32_t* seq_lens, int32_t batch, int32_t max_nodes, uint32_t* accepted, int32_t* count,
+                   int64_t* next_token, int32_t* new_lens, int32_t* status, void* stream);
+
+/* Moves the rows of the accepted nodes (any set of nodes) of one layer's cache to the front of the drafts, in order, in
+ * place: K, V, the code words (hash_pages, optional) and the received weights (mass, optional; zero behind the accepted ones).
+ * seq_lens are those before the commit and are not changed (the layers of a model share them): afterwards the sequence's
+ * length is new_lens of ha_tree_accept.                                                                              */
+int ha_tree_commit(const ha_shape_t* shape, const ha_tree_t* tree, const uint32_t* accepted, void* k_pages, void* v_pages,
+                   uint32_t* hash_pages, const int32_t* page_table, const int32_t* seq_lens, float* mass,
+                   int32_t* status, void* stream);
+
+/* Cuts every sequence longer than keep_tokens to that many tokens, per kv-head: the first init_budget, the last
+ * recent_budget and, of those in between, the ones with the largest mass (ties: the lowest token; negative values and NaN
+ * count as 0), in their order. K, V and code rows (hash_pages, optional) move in place. kept [batch][num_kv_heads]
+ * [keep_tokens] <- the former token numbers (entries behind a shorter sequence's end are left as they were); mass_out
+ * (optional, not mass) <- the kept tokens' mass, zeros behind; lens_out (not seq_lens) <- the new lengths. Rotary positions are
+ * in the keys already: later tokens keep counting from the former length.                                            */
+int ha_cache_evict(const ha_shape_t* shape, int32_t keep_tokens, int32_t init_budget, int32_t recent_budget,
+                   const float* mass, void* k_pages, void* v_pages, uint32_t* hash_pages, const int32_t* page_table,
+                   const int32_t* seq_lens, int32_t* kept, float* mass_out, int32_t* lens_out,
+                   int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
