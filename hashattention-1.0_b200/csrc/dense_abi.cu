@@ -6,6 +6,7 @@
 
 #include "cache_moves.cuh"
 #include "host.cuh"
+#include "tree_attention_tc.cuh"
 
 namespace ha {
 namespace {
@@ -54,31 +55,31 @@ int q_strides_of(const ha_shape_t* s, const ha_tree_t* t, const int64_t* strides
     return (batch | node | head) % 8 == 0 && batch >= 0 && node >= 0 && head >= 0 ? HA_OK : HA_ERR_BAD_ARG;
 }
 
-int rows_of(int max_nodes) { return max_nodes * kGroup <= 16 ? 16 : 32; }
+// Query rows per CTA of the attention of trees of up to max_nodes nodes: a kernel each.
+int rows_of(int max_nodes) { return max_nodes * kGroup <= 16 ? 16 : (max_nodes * kGroup <= 128 ? 128 : 256); }
 
 size_t tree_workspace(int max_nodes) {
     return (size_t)2 * kDenseMaxCtas * rows_of(max_nodes) * (sizeof(float2) + kHeadDim * sizeof(float));
 }
 
-template <int MT>
-int launch_tree_rows(const ha_shape_t* shape, const TreeAttentionParams& p, const void* k_pages, const void* v_pages, cudaStream_t st) {
-    using L = RowsLayout<MT>;
+// The attention kernel and the merge behind it.
+template <int kTile, int kRows>
+int launch_tree(void (*kernel)(TreeAttentionParams, CUtensorMap, CUtensorMap), int threads, size_t smem_bytes, const ha_shape_t* shape,
+                const TreeAttentionParams& p, cudaStream_t st) {
     int sms = 0;
     if (sm_count(sms) != HA_OK) return HA_ERR_LAUNCH;
     CUtensorMap k_map, v_map;
     const uint64_t rows = (uint64_t)shape->num_pages * shape->num_kv_heads * kPage;
-    if (!encode_row_map(&k_map, k_pages, rows, kRowsTile) || !encode_row_map(&v_map, v_pages, rows, kRowsTile)) return HA_ERR_LAUNCH;
+    if (!encode_row_map(&k_map, p.k_pages, rows, kTile) || !encode_row_map(&v_map, p.v_pages, rows, kTile)) return HA_ERR_LAUNCH;
     // (a per-device function attribute: set at every call, so that a process driving several GPUs is served)
-    if (cudaFuncSetAttribute(tree_attention_rows_kernel<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kSmemBytes) != cudaSuccess)
-        return HA_ERR_LAUNCH;
-    const int groups = DenseCut<kRowsTile, L::kRows>::groups(p.seqs.T);
-    const long long tiles = (long long)shape->batch * shape->num_kv_heads * groups * shape->max_pages * (kPage / kRowsTile);
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes) != cudaSuccess) return HA_ERR_LAUNCH;
+    const int groups = DenseCut<kTile, kRows>::groups(p.seqs.T);
+    const long long tiles = (long long)shape->batch * shape->num_kv_heads * groups * shape->max_pages * (kPage / kTile);
     const int ctas = (int)std::min<long long>(tiles, std::min(sms, kDenseMaxCtas));
-    if (launch_smem(tree_attention_rows_kernel<MT>, dim3(ctas), dim3(kRowsThreads), L::kSmemBytes, st, 1, p, k_map, v_map) != cudaSuccess)
-        return HA_ERR_LAUNCH;
-    const int rows_max = std::min(L::kRows, p.seqs.T * kGroup);
+    if (launch_smem(kernel, dim3(ctas), dim3(threads), smem_bytes, st, 1, p, k_map, v_map) != cudaSuccess) return HA_ERR_LAUNCH;
+    const int rows_max = std::min(kRows, p.seqs.T * kGroup);
     const dim3 grid(shape->num_kv_heads * groups, shape->batch, (rows_max + kTreeMergeWarps - 1) / kTreeMergeWarps);
-    return launch(tree_merge_kernel<kRowsTile, L::kRows>, grid, dim3(kTreeMergeWarps * 32), st, 1, p, ctas) == cudaSuccess ? HA_OK : HA_ERR_LAUNCH;
+    return launch(tree_merge_kernel<kTile, kRows>, grid, dim3(kTreeMergeWarps * 32), st, 1, p, ctas) == cudaSuccess ? HA_OK : HA_ERR_LAUNCH;
 }
 
 }  // namespace
@@ -146,7 +147,11 @@ int ha_tree_attention(const ha_shape_t* shape, const ha_tree_t* tree, const void
     p.part_ml = reinterpret_cast<float2*>(p.part_acc + (size_t)2 * kDenseMaxCtas * rows * kHeadDim);
     p.scale_log2 = sm_scale * 1.4426950408889634f;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return rows == 16 ? launch_tree_rows<1>(shape, p, k_pages, v_pages, st) : launch_tree_rows<2>(shape, p, k_pages, v_pages, st);
+    p.k_pages = static_cast<const __nv_bfloat16*>(k_pages);
+    p.v_pages = static_cast<const __nv_bfloat16*>(v_pages);
+    if (rows == 16) return launch_tree<kRowsTile, 16>(tree_attention_rows_kernel<1>, kRowsThreads, RowsLayout<1>::kSmemBytes, shape, p, st);
+    if (rows == 128) return launch_tree<kTaTile, 128>(tree_attention_tc_kernel<false>, kTaThreads, TaLayout<false>::kSmemBytes, shape, p, st);
+    return launch_tree<kTaTile, 256>(tree_attention_tc_kernel<true>, kTaThreads, TaLayout<true>::kSmemBytes, shape, p, st);
 }
 
 int ha_attention_mass(const ha_shape_t* shape, const ha_tree_t* tree, const void* q, const int64_t* q_strides, const float* lse, const uint32_t* rows,

@@ -29,6 +29,8 @@ struct TreeAttentionParams {
     float* lse;              // [B][T][Hq] or null
     float2* part_ml;         // [2 * CTAs][rows] maximum (in powers of two) and sum of each partial result
     float* part_acc;         // [2 * CTAs][rows][128]
+    const __nv_bfloat16* k_pages;  // [num_pages][Hkv][256][128]: single rows only, the tiles come by tensor map
+    const __nv_bfloat16* v_pages;
     float scale_log2;        // c * log2(e)
 };
 

@@ -1,0 +1,528 @@
+// Dense attention of many query rows per kv-head over the paged cache, on the 5th-generation tensor cores (tcgen05): drafted
+// trees of more than a few nodes.
+//
+// The mathematics of tree_attention.cuh with the rows of a kv-head (4 per node) on the 128 lanes of tensor memory. Per tile of
+// 128 tokens S = Q K^T (128 x 128 sums), P = e^{S - m} by two threads per row, O += P V with P handed over in tensor memory as two bf16
+// (hi + lo) in the columns S was read from. A CTA works on two such chains ("streams") at a time, so that one's softmax runs
+// under the other's products:
+//   * up to 128 rows (kWide == false): both streams have the same rows and take every second tile; their results are joined
+//     at the end of the unit, each group of softmax warps reading a quarter of the columns of both.
+//   * up to 256 rows (kWide): stream w has rows 128 w .. 128 w + 127, and a tile of K and V serves both.
+//
+// Roles of the warps: 0 issues the products, 4 - 19 are the softmax warps (eight per stream: a thread has
+// 64 of a row's 128 columns, and the two halves of a row agree on its maximum, as bf16, through shared memory), 2 loads: K and
+// V tiles by TMA (two boxes of 64 elements x 128 tokens, 128-byte swizzle) into a ring of 32 KB slots, K and V of a tile in turn. Streams that take different tiles have a ring of three slots each, so that a barrier is waited for
+// in every phase by the one who uses it; those that share tiles share a ring of five.
+//
+// A stream's S takes the place of its last P: its product Q K^T is issued behind P V of the tile before, in the tensor core's
+// order, so S complete means O complete too, and the softmax warps may rescale O (which they do only when a row's maximum has
+// grown by more than 2^8) without another barrier.
+//
+// The V rows behind a sequence's end, and V rows of drafts with an infinity or NaN in them, are zeroed in shared memory before
+// the product sees them; the latter are added at the end to the rows that see them, by scalar arithmetic.
+#pragma once
+
+#include "tree_attention.cuh"
+
+namespace ha {
+
+constexpr int kTaTile = 128;                       // tokens per tile
+constexpr uint32_t kTaSlot = 2 * 128 * 128;        // K or V of a tile: 32 KB
+constexpr uint32_t kTaHalf = 128 * 128;            // 64 elements of 128 rows
+constexpr int kTaLoadWarp = 2;
+constexpr int kTaSoftWarp0 = 4;                    // (a warp group of its own for the others; warps 1 and 3 do nothing)
+constexpr int kTaSoftWarps = 16;
+constexpr int kTaThreads = (kTaSoftWarp0 + kTaSoftWarps) * 32;
+
+template <bool kWide>
+struct TaLayout {
+    static constexpr int kRows = kWide ? 256 : 128;
+    static constexpr int kRings = kWide ? 1 : 2;
+    static constexpr int kSlots = kWide ? 5 : 3;           // per ring
+    static constexpr uint32_t kOffQ = 0;                   // 128 rows x 128 each, K-major, 128-byte swizzle
+    static constexpr uint32_t kOffRing = (kWide ? 2 : 1) * kTaSlot;
+    static constexpr uint32_t kOffMl = kOffQ;              // [2][2][128] float2, once the unit's products are complete
+    static constexpr int kBarFull = 0;                     // [rings][slots] the loader's arrival and the bytes of two copies
+    static constexpr int kBarEmpty = kBarFull + kRings * kSlots;  // [rings][slots] commit: the products have read the slot
+    static constexpr int kBarS = kBarEmpty + kRings * kSlots;     // [2] commit: S complete (and every product in front)
+    static constexpr int kBarP = kBarS + 2;                // [2] 8 warps: P is written
+    static constexpr int kBarO = kBarP + 2;                // [2] commit: the unit's last product is complete
+    static constexpr int kBarQ = kBarO + 2;                // 16 warps: the unit's queries are in place, the last unit's results read
+    static constexpr int kBarFinal = kBarQ + 1;            // commit: every product of the CTA is complete
+    static constexpr int kBars = kBarFinal + 1;
+    static constexpr uint32_t kOffMax = kOffRing + kRings * kSlots * kTaSlot;  // [2 streams][2 halves][128] bf16: maxima of half rows
+    static constexpr uint32_t kOffBar = kOffMax + 2 * 2 * 128 * 2;
+    static constexpr uint32_t kOffTmem = kOffBar + kBars * 8;     // tmem base, abort flag
+    static constexpr uint32_t kOffBad = (kOffTmem + 8 + 15) / 16 * 16;  // [4] nodes with an infinity or NaN in V
+    static constexpr uint32_t kSmemBytes = kOffBad + 16 + 1024;   // + slack to align the base to 1024 B
+    static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
+};
+
+// V as the B operand of O (128 x 128) += P (128 x 16) V (16 x 128): the 128 output columns run along the 128-byte rows
+// ("MN-major"), so blocks of 64 columns are kTaHalf apart and groups of 8 tokens 1024 bytes.
+__device__ __forceinline__ uint32_t ta_v_desc_lo(uint32_t saddr) { return ((saddr >> 4) & 0x3FFFu) | ((kTaHalf >> 4) << 16); }
+__device__ __forceinline__ uint32_t ta_pv_idesc() { return tc_idesc(128) | (1u << 16); }
+
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+        :: "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+           "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+        : "memory");
+}
+
+// 32 tokens from token `base` on that a row with mask `m` (bits below n only) sees, one bit each.
+__device__ __forceinline__ uint32_t visible32(const uint4& m, int base, int P, int S) {
+    uint32_t vis;
+    const int at = base - P;  // the first token's node, negative in the prefix
+    if (at <= -32) vis = 0xffffffffu;
+    else {
+        auto word = [&](int w) { return w < 0 ? 0xffffffffu : (w == 0 ? m.x : (w == 1 ? m.y : (w == 2 ? m.z : (w == 3 ? m.w : 0u)))); };
+        const int w = at >> 5;  // (rounds down)
+        vis = __funnelshift_r(word(w), word(w + 1), at & 31);
+    }
+    const int left = S - base;
+    return left >= 32 ? vis : (left <= 0 ? 0u : vis & ((1u << left) - 1u));
+}
+
+template <bool kWide>
+__global__ void __launch_bounds__(kTaThreads, 1)
+tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+    using L = TaLayout<kWide>;
+    using Cursor = DenseCursor<kTaTile, L::kRows>;
+    extern __shared__ unsigned char ta_smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ta_smem_raw) + 1023) & ~(uintptr_t)1023);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t sbase = tc_smem_u32(smem), bars = sbase + L::kOffBar;
+    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + L::kOffTmem);
+    volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::kOffTmem + 4);
+    uint32_t* s_bad = reinterpret_cast<uint32_t*>(smem + L::kOffBad);
+    float2* s_ml = reinterpret_cast<float2*>(smem + L::kOffMl);
+    auto bar = [&](int i) { return bars + 8u * (uint32_t)i; };
+    if (tid == 0) {
+        auto init = [&](int first, int n, uint32_t count) {
+            for (int i = first; i < first + n; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar(i)), "r"(count));
+        };
+        init(L::kBarFull, L::kRings * L::kSlots, 1);
+        init(L::kBarEmpty, L::kRings * L::kSlots, 1);
+        init(L::kBarS, 2, 1);
+        init(L::kBarP, 2, 8);
+        init(L::kBarO, 2, 1);
+        init(L::kBarQ, 1, kTaSoftWarps);
+        init(L::kBarFinal, 1, 1);
+        *s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem_u32(s_tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *s_tmem;
+    pdl_wait();
+    pdl_launch_dependents();
+
+    // every lane waits for itself; the warp then agrees, so that warp-wide instructions are never executed by a part of it
+    auto wait = [&](int b, uint32_t parity) {
+        const bool ok = tc_wait(bar(b), parity, s_abort, p.seqs.status);
+        return __all_sync(0xffffffffu, ok) != 0;
+    };
+    // tiles of the segment that stream w takes
+    auto stream_tiles = [&](const DenseSegment& s, int w) { return kWide ? s.tile1 - s.tile0 : (s.tile1 - s.tile0 + 1 - w) / 2; };
+
+    // Registers: 640 threads start with 96 each. The four warps that issue and load keep 56, the 16 softmax warps
+    // go up to 104: 128 x 56 + 512 x 104 <= 640 x 96.
+    static_assert((kTaSoftWarp0 * 32) * 56 + (kTaSoftWarps * 32) * 104 <= kTaThreads * 96, "registers of one CTA");
+    if (warp < kTaSoftWarp0) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+
+    DenseSegment seg;
+    bool ok = true;
+
+    if (warp == 0) {
+        // ---- the issuer: P V of a stream's tile and Q K^T of its next one back to back, the streams in turn ----------------
+        Cursor cur(p.seqs, lane, false);
+        const uint32_t t_0 = __shfl_sync(0xffffffffu, tmem, 0);
+        uint32_t use[2] = {0, 0}, tiles[2] = {0, 0}, segs = 0;  // ring slots and tiles so far
+        auto wait_mma = [&](int b, uint32_t parity) {
+            const bool done = wait(b, parity);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            return done;
+        };
+        auto ring_at = [&](int w) { return (uint32_t)((kWide ? 0 : w * L::kSlots)) + use[kWide ? 0 : w] % L::kSlots; };
+        auto ring_parity = [&](int w) { return (use[kWide ? 0 : w] / L::kSlots) & 1; };
+        // S = Q K^T of stream w with the tile at the front of its ring; streams that share the tile release it together
+        auto qk = [&](int w) {
+            const uint32_t at = ring_at(w);
+            if (!(kWide && w == 1) && !wait_mma(L::kBarFull + (int)at, ring_parity(w))) return false;
+            const uint32_t q_lo = tc_desc_lo(sbase + L::kOffQ + (kWide ? (uint32_t)w * kTaSlot : 0u));
+            const uint32_t k_lo = tc_desc_lo(sbase + L::kOffRing + at * kTaSlot);
+#pragma unroll
+            for (uint32_t ks = 0; ks < 8; ++ks)
+                tc_mma_ss(t_0 + 128u * (uint32_t)w, tc_desc(q_lo + tc_koff(ks, kTaHalf)), tc_desc(k_lo + tc_koff(ks, kTaHalf)), tc_idesc(128), ks == 0 ? 0u : 1u);
+            tc_commit(bar(L::kBarS + w));
+            if (!kWide || w == 1) tc_commit(bar(L::kBarEmpty + (int)at));
+            return true;
+        };
+        auto pv = [&](int w, bool first) {
+            if (!wait_mma(L::kBarP + w, tiles[w] & 1)) return false;
+            ++tiles[w];
+            const uint32_t at = ring_at(w);
+            if (!(kWide && w == 1) && !wait_mma(L::kBarFull + (int)at, ring_parity(w))) return false;
+            const uint32_t v_lo = ta_v_desc_lo(sbase + L::kOffRing + at * kTaSlot), t_s = t_0 + 128u * (uint32_t)w, t_o = t_s + 256u;
+#pragma unroll
+            for (uint32_t ks = 0; ks < 8; ++ks) {
+                const uint64_t vd = tc_desc(v_lo + ks * (2048u >> 4));
+                tc_mma_ts(t_o, t_s + 16 * ks, vd, ta_pv_idesc(), first && ks == 0 ? 0u : 1u);
+                tc_mma_ts(t_o, t_s + 16 * ks + 8, vd, ta_pv_idesc(), 1u);
+            }
+            if (!kWide || w == 1) tc_commit(bar(L::kBarEmpty + (int)at));
+            return true;
+        };
+        while (ok && cur.next(seg)) {
+            if (!(ok = wait_mma(L::kBarQ, segs & 1))) break;
+            ++segs;
+            const int count0 = stream_tiles(seg, 0), count1 = stream_tiles(seg, 1);  // count1 = count0 or one less
+            // `use` of a ring: the K tile of the stream's next product, then its V tile. Streams that share a ring: K of tile i is
+            // used by both, then V of tile i - 1 ... so the place in the ring is set by hand.
+            if constexpr (kWide) {
+                const uint32_t base = use[0];
+                ok = qk(0) && qk(1);
+                for (int i = 0; i < count0 && ok; ++i) {
+                    for (int w = 0; w < 2 && ok; ++w) {
+                        use[0] = base + 2 * i + 1;
+                        if (!(ok = pv(w, i == 0))) break;
+                        use[0] = base + 2 * i + 2;
+                        if (i + 1 < count0) ok = qk(w);
+                    }
+                }
+                use[0] = base + 2 * count0;
+            } else {
+                ok = qk(0);
+                ++use[0];
+                if (ok && count1 > 0) {
+                    ok = qk(1);
+                    ++use[1];
+                }
+                for (int i = 0; i < count0 && ok; ++i) {
+                    for (int w = 0; w < 2 && ok; ++w) {
+                        const int count = w == 0 ? count0 : count1;
+                        if (i >= count) break;
+                        if (!(ok = pv(w, i == 0))) break;
+                        ++use[w];
+                        if (i + 1 < count) {
+                            ok = qk(w);
+                            ++use[w];
+                        }
+                    }
+                }
+            }
+            // (for a unit without a tile for a stream too: its softmax warps then never run ahead of the issuer)
+            if (ok) {
+                tc_commit(bar(L::kBarO));
+                tc_commit(bar(L::kBarO + 1));
+            }
+        }
+        // the tensor core has finished everything issued above (after a time-out: one more bounded wait)
+        tc_commit(bar(L::kBarFinal));
+        for (int spin = 0; spin < (1 << 22) && __all_sync(0xffffffffu, tc_test(bar(L::kBarFinal), 0)) == 0; ++spin) {}
+    } else if (warp >= kTaSoftWarp0) {
+        // ---- softmax warps -----------------------------------------------------------------------------------------------
+        // A warp that gives up goes on through the units without waiting, so that the barriers among these warps are
+        // reached by all of them.
+        Cursor cur(p.seqs, lane, false);
+        const int group = (warp - kTaSoftWarp0) >> 2, w = group >> 1, half = group & 1;  // stream, half of the columns
+        const int quarter = warp & 3, r = quarter * 32 + lane, ring = kWide ? 0 : w;      // quarter of the rows = tensor-memory lanes
+        const int t_all = tid - kTaSoftWarp0 * 32, t_stream = t_all & 255;
+        const uint32_t t_lane = tmem + ((uint32_t)quarter << 21), t_s = t_lane + 128u * (uint32_t)w + 64u * (uint32_t)half;
+        const uint32_t t_o = t_lane + 256u + 128u * (uint32_t)w + 64u * (uint32_t)half;
+        __nv_bfloat16* s_max = reinterpret_cast<__nv_bfloat16*>(smem + L::kOffMax) + (size_t)w * 256;
+        const unsigned char* ring_mem = smem + L::kOffRing + (size_t)(ring * L::kSlots) * kTaSlot;
+        uint32_t use = 0, tiles = 0, seg_o = 0;
+        const f32x2 scale2 = pack2(p.scale_log2, p.scale_log2);
+        while (cur.next(seg)) {
+            const int P = seg.S - seg.n, row0 = seg.group * L::kRows + (kWide ? 128 * w : 0);
+            const int rows_left = seg.n * kGroup - row0;  // may be <= 0 for the second half of a wide unit
+            const bool idle = quarter * 32 >= rows_left;
+            const int node = (row0 + r) >> 2;
+            const bool mine = r < rows_left;
+            uint4 mask = make_uint4(0, 0, 0, 0);
+            if (mine && seg.tile1 * kTaTile > P) {
+                mask = dense_mask(p.seqs, seg.b, node);
+                const uint4 f = first_nodes(seg.n);
+                mask.x &= f.x; mask.y &= f.y; mask.z &= f.z; mask.w &= f.w;
+            }
+            // queries: row-major pieces of 16 bytes, rows behind the last one zero
+            {
+                constexpr int kThreads = kWide ? 256 : 512;
+                const int t = kWide ? t_stream : t_all;
+                unsigned char* dst = smem + L::kOffQ + (kWide ? (size_t)w * kTaSlot : 0);
+                uint4 v[128 * 16 / kThreads];
+#pragma unroll
+                for (int k = 0; k < 128 * 16 / kThreads; ++k) {
+                    const int i = t + k * kThreads, qr = i >> 4, c = i & 15;
+                    v[k] = make_uint4(0, 0, 0, 0);
+                    if (qr < rows_left)
+                        v[k] = __ldg(reinterpret_cast<const uint4*>(p.q + seg.b * p.q_batch + (long long)((row0 + qr) >> 2) * p.q_node +
+                                                                    (seg.kvh * kGroup + (qr & 3)) * p.q_head) + c);
+                }
+#pragma unroll
+                for (int k = 0; k < 128 * 16 / kThreads; ++k) {
+                    const int i = t + k * kThreads, qr = i >> 4, c = i & 15;
+                    *reinterpret_cast<uint4*>(dst + (c >> 3) * kTaHalf + tc_swizzled(qr, c & 7)) = v[k];
+                }
+                if (warp == kTaSoftWarp0 && lane < kMaskWords) s_bad[lane] = 0;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) tc_arrive(bar(L::kBarQ));
+            }
+            const int count = stream_tiles(seg, w);
+            float m = -INFINITY, l = 0.0f;
+            for (int i = 0; i < count; ++i, ++tiles, use += 2) {
+                if (ok) ok = wait(L::kBarS + w, tiles & 1);
+                const int tok0 = (seg.tile0 + (kWide ? i : 2 * i + w)) * kTaTile;
+                const bool masked = tok0 + kTaTile > P;
+                if (masked) {
+                    // the tile has drafts or lies beyond the end: V rows are looked at by the threads that share the tile
+                    const uint32_t v_use = use + 1, slot = v_use % L::kSlots;
+                    if (ok) ok = wait(L::kBarFull + ring * L::kSlots + (int)slot, (v_use / L::kSlots) & 1);
+                    const int t = kWide ? t_all : t_stream;  // the first 128 of them: a token each
+                    unsigned char* row = const_cast<unsigned char*>(ring_mem) + slot * kTaSlot + (uint32_t)t * 128u;
+                    const int j = tok0 + t;
+                    if (ok && t < kTaTile && j >= P) {
+                        bool drop = j >= seg.S;
+                        if (!drop) {
+#pragma unroll
+                            for (int c = 0; c < 16; ++c)  // (in any order: the swizzle permutes pieces inside a row)
+                                drop |= any_nonfinite(*reinterpret_cast<const uint4*>(row + (c >> 3) * kTaHalf + (c & 7) * 16));
+                            if (drop) atomicOr(&s_bad[(j - P) >> 5], 1u << ((j - P) & 31));
+                        }
+                        if (drop)
+                            for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(row + (c >> 3) * kTaHalf + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    if (kWide) asm volatile("bar.sync 1, 512;" ::: "memory");
+                    else asm volatile("bar.sync %0, 256;" ::"r"(10 + w) : "memory");
+                }
+                if (idle) {
+                    __syncwarp();
+                    if (ok && lane == 0) tc_arrive(bar(L::kBarP + w));
+                    continue;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                uint32_t s[4][16];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) tc_ld16_issue(t_s + 16 * q, s[q]);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) tc_ld16_wait(s[q]);
+                if (masked) {
+#pragma unroll
+                    for (int q = 0; q < 4; q += 2) {
+                        const uint32_t vis = visible32(mask, tok0 + 64 * half + 16 * q, P, seg.S);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            if (((vis >> k) & 1u) == 0) s[q + (k >> 4)][k & 15] = 0xff800000u;  // -inf
+                    }
+                }
+                float x0 = -INFINITY, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int k = 0; k < 16; k += 4) {
+                        x0 = fmaxf(x0, __uint_as_float(s[q][k]));
+                        x1 = fmaxf(x1, __uint_as_float(s[q][k + 1]));
+                        x2 = fmaxf(x2, __uint_as_float(s[q][k + 2]));
+                        x3 = fmaxf(x3, __uint_as_float(s[q][k + 3]));
+                    }
+                // the maximum of the row, as both halves know it (a reference for the exponents: its rounding does not matter)
+                const __nv_bfloat16 mine_max = __float2bfloat16_rn(fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * p.scale_log2);
+                s_max[half * 128 + r] = mine_max;
+                asm volatile("bar.sync %0, 64;" ::"r"(2 + 4 * w + quarter) : "memory");
+                const float x = fmaxf(__bfloat162float(mine_max), __bfloat162float(s_max[(half ^ 1) * 128 + r]));
+                if (!ok) continue;
+                const bool grow = x > m + kRescaleAt;  // (from -inf: any score at all)
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float alpha = grow ? exp2_approx(m - x) : 1.0f;
+                    m = grow ? x : m;
+                    l *= alpha;
+                    if (i > 0) {
+                    // O is complete: S of this tile was issued behind the product that wrote it
+#pragma unroll 1
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t o[16];
+                        tc_ld16_issue(t_o + 16 * q, o);
+                        tc_ld16_wait(o);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+                        tc_st16(t_o + 16 * q, o);
+                    }
+                    }
+                }
+                const float ref = m == -INFINITY ? 0.0f : m;
+                const f32x2 nref2 = pack2(-ref, -ref);
+                f32x2 la = pack2(0.0f, 0.0f), lb = pack2(0.0f, 0.0f);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t out[16];  // one k-step of the A operand: words 0 .. 7 the hi halves, 8 .. 15 the lo halves
+#pragma unroll
+                    for (int pr = 0; pr < 8; ++pr) {
+                        float t0, t1;
+                        unpack2(fma2(pack2(__uint_as_float(s[q][2 * pr]), __uint_as_float(s[q][2 * pr + 1])), scale2, nref2), t0, t1);
+                        const float e0 = exp2_approx(t0), e1 = exp2_approx(t1);
+                        if (pr & 1) lb = add2(lb, pack2(e0, e1));
+                        else la = add2(la, pack2(e0, e1));
+                        const uint32_t hi = tc_pack_bf16(e0, e1);
+                        float l0, l1;  // e - hi, exact: the multiply-add takes the bf16 halves of hi as they are
+                        asm("{\n\t.reg .b16 h0, h1;\n\tmov.b32 {h0, h1}, %2;\n\t"
+                            "fma.rn.f32.bf16 %0, h0, %3, %4;\n\tfma.rn.f32.bf16 %1, h1, %3, %5;\n\t}"
+                            : "=f"(l0), "=f"(l1) : "r"(hi), "h"((unsigned short)0xBF80), "f"(e0), "f"(e1));
+                        out[pr] = hi;
+                        out[pr + 8] = tc_pack_bf16(l0, l1);
+                    }
+                    tc_st16(t_s + 16 * q, out);
+                }
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) tc_arrive(bar(L::kBarP + w));
+                float a0, a1, b0, b1;
+                unpack2(la, a0, a1);
+                unpack2(lb, b0, b1);
+                l += (a0 + a1) + (b0 + b1);
+            }
+            // ---- the unit's result -------------------------------------------------------------------------------------
+            if (ok) ok = wait(L::kBarO + w, seg_o & 1);
+            ++seg_o;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            // sums of the halves, and of the streams that share the rows
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            asm volatile("bar.sync 1, 512;" ::: "memory");  // (all products have read the queries, whose place this is)
+            s_ml[(2 * w + half) * 128 + r] = make_float2(m, l);
+            asm volatile("bar.sync 1, 512;" ::: "memory");
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            float M = m, sum, f0 = 1.0f, f1 = 0.0f;
+            if constexpr (kWide) {
+                sum = l + s_ml[(2 * w + (half ^ 1)) * 128 + r].y;
+            } else {
+                const float2 a = s_ml[r], b = s_ml[256 + r];
+                M = fmaxf(a.x, b.x);
+                const float ref = M == -INFINITY ? 0.0f : M;
+                f0 = exp2_approx(a.x - ref);
+                f1 = exp2_approx(b.x - ref);
+                sum = (a.y + s_ml[128 + r].y) * f0 + (b.y + s_ml[384 + r].y) * f1;
+            }
+            if (ok && !idle) {
+                const bool second = !kWide && stream_tiles(seg, 1) > 0;  // (otherwise that stream's columns hold something else)
+                const size_t out_row = ((size_t)seg.b * p.seqs.T + node) * ((size_t)p.seqs.Hkv * kGroup) + seg.kvh * kGroup + (r & 3);
+                const size_t part = (size_t)(2 * blockIdx.x + seg.slot) * L::kRows + (kWide ? 128 * w : 0) + r;
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const uint32_t bad = s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3];
+                const int q0 = kWide ? 4 * half : 2 * group, q1 = q0 + (kWide ? 4 : 2);
+#pragma unroll 1
+                for (int q = q0; q < q1; ++q) {
+                    uint32_t o0[16], o1[16];
+                    tc_ld16_issue(t_lane + 256u + (kWide ? 128u * (uint32_t)w : 0u) + 16 * q, o0);
+                    if (second) tc_ld16_issue(t_lane + 384u + 16 * q, o1);
+                    tc_ld16_wait(o0);
+                    if (second) tc_ld16_wait(o1);
+                    if (!mine) continue;
+                    float acc[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        acc[k] = __uint_as_float(o0[k]) * f0;
+                        if (second) acc[k] = fmaf(__uint_as_float(o1[k]), f1, acc[k]);
+                    }
+                    if (bad != 0) {
+                        const __nv_bfloat16* qr = p.q + seg.b * p.q_batch + (long long)node * p.q_node + (seg.kvh * kGroup + (r & 3)) * p.q_head;
+                        for (int t = 0; t < seg.n; ++t) {
+                            if (((s_bad[t >> 5] >> (t & 31)) & 1u) == 0 || !dense_bit(mask, t)) continue;
+                            const int j = P + t;
+                            const size_t at = (((size_t)dense_page(p.seqs, seg.b, j / kPage) * p.seqs.Hkv + seg.kvh) * kPage + j % kPage) * kHeadDim;
+                            float dot = 0.0f;
+                            for (int d = 0; d < kHeadDim; ++d) dot = fmaf(__bfloat162float(qr[d]), __bfloat162float(p.k_pages[at + d]), dot);
+                            const float e = exp2_approx(fmaf(dot, p.scale_log2, M == -INFINITY ? 0.0f : -M));
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) acc[k] = fmaf(e, __bfloat162float(p.v_pages[at + 16 * q + k]), acc[k]);
+                        }
+                    }
+                    if (seg.whole()) {
+                        uint32_t words[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) words[k] = tc_pack_bf16(acc[2 * k] * inv, acc[2 * k + 1] * inv);
+                        uint4* dst = reinterpret_cast<uint4*>(p.out + out_row * kHeadDim + 16 * q);
+                        dst[0] = make_uint4(words[0], words[1], words[2], words[3]);
+                        dst[1] = make_uint4(words[4], words[5], words[6], words[7]);
+                    } else {
+                        float4* dst = reinterpret_cast<float4*>(p.part_acc + part * kHeadDim + 16 * q);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) dst[k] = make_float4(acc[4 * k], acc[4 * k + 1], acc[4 * k + 2], acc[4 * k + 3]);
+                    }
+                }
+                if (mine && (kWide ? half : group) == 0) {
+                    if (!seg.whole()) p.part_ml[part] = make_float2(M, sum);
+                    else if (p.lse != nullptr) p.lse[out_row] = sum == 0.0f ? -INFINITY : (M + log2f(sum)) * 0.6931471805599453f;
+                }
+            }
+            // the queries and O make room for the next unit: every product of this one is complete, and what was read of the other
+            // stream's is read before its next product (the queries' barrier)
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            asm volatile("bar.sync 1, 512;" ::: "memory");
+        }
+    } else if (warp == kTaLoadWarp) {
+        // ---- the loading warp: lane l holds the l-th page of a window of 32; one lane copies -----------------------------
+        Cursor cur(p.seqs, lane, blockIdx.x == 0);
+        uint32_t use[2] = {0, 0};
+        auto copy = [&](int ring, const CUtensorMap* map, int y) {
+            const uint32_t slot = use[ring] % L::kSlots, at = (uint32_t)(ring * L::kSlots) + slot, dst = sbase + L::kOffRing + at * kTaSlot;
+            if (!tc_wait(bar(L::kBarEmpty + (int)at), ((use[ring] / L::kSlots) & 1) ^ 1, s_abort, p.seqs.status)) return false;
+            const uint32_t full = bar(L::kBarFull + (int)at);
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full), "r"(kTaSlot) : "memory");
+            tc_tma_load(dst, map, 0, y, full);
+            tc_tma_load(dst + kTaHalf, map, 64, y, full);
+            ++use[ring];
+            return true;
+        };
+        if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
+        }
+        while (ok && cur.next(seg)) {
+            int base = -64, page_l = 0;
+            for (int t = seg.tile0; t < seg.tile1 && ok; ++t) {
+                const int pi = t / (kPage / kTaTile);
+                if (pi - base >= 32) {
+                    base = pi;
+                    page_l = (base + lane) * kPage < seg.S ? dense_page(p.seqs, seg.b, base + lane) : 0;
+                }
+                const int page = __shfl_sync(0xffffffffu, page_l, pi - base);
+                if (lane == 0) {
+                    const int y = (int)(((size_t)page * p.seqs.Hkv + seg.kvh) * kPage) + (t % (kPage / kTaTile)) * kTaTile;
+                    const int ring = kWide ? 0 : (t - seg.tile0) & 1;
+                    ok = copy(ring, &k_map, y) && copy(ring, &v_map, y);
+                }
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+            }
+        }
+        // no copy is left in flight when the CTA ends (they have all landed unless the CTA gave up early)
+        if (lane == 0)
+            for (int ring = 0; ring < L::kRings; ++ring)
+                for (uint32_t j = use[ring] > (uint32_t)L::kSlots ? use[ring] - L::kSlots : 0; j < use[ring]; ++j)
+                    for (int spin = 0; spin < (1 << 22) && !tc_test(bar(L::kBarFull + ring * L::kSlots + (int)(j % L::kSlots)), (j / L::kSlots) & 1); ++spin) {}
+        __syncwarp();
+    }
+
+    // ---- release tensor memory -----------------------------------------------------------------------------------------
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 0) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+}  // namespace ha
