@@ -90,7 +90,8 @@ PROTOTYPES = {
     "ha_attention_mass": (c_int, [_S, _T, _P, _I64, _P, _P, _P, _P, _P, c_float, _P, _P, _P]),
     "ha_tree_accept": (c_int, [_P, _P, _P, _P, _P, c_int32, c_int32, _P, _P, _P, _P, _P, _P]),
     "ha_tree_commit": (c_int, [_S, _T, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
-    "ha_cache_evict": (c_int, [_S, c_int32, c_int32, c_int32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "ha_cache_evict": (c_int, [_S, c_int32, c_int32, c_int32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_size_t, _P, _P]),
+    "ha_evict_workspace_bytes": (c_size_t, [_S]),
 }
 
 _lib = None

@@ -181,7 +181,12 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const TreeC
     float m = 0.0f;
     float* mass = p.mass != nullptr ? p.mass + ((size_t)b * d.Hkv + kvh) * ((size_t)d.max_pages * kPage) + P : nullptr;
     if (mass != nullptr && tid < count) m = __ldcg(mass + s_src[tid]);
-    __syncthreads();
+    // (the barrier takes a predicate formed from what was loaded, so that no load is still on its way behind it)
+    uint32_t arrived = __float_as_uint(m);
+#pragma unroll
+    for (int k = 0; k < kCommitPieces; ++k)
+        if (tid + k * kCommitThreads < moved * per_row) arrived ^= v[k].x;
+    __syncthreads_or(arrived == 0x5bd1e995u);
 #pragma unroll
     for (int k = 0; k < kCommitPieces; ++k) {
         const int i = tid + k * kCommitThreads;
@@ -192,10 +197,11 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const TreeC
 
 // ---- eviction: which tokens stay -------------------------------------------------------------------------------------------
 // Per (sequence, kv-head): the sink, the recent tokens and the H candidates of the largest accumulated weight, ties by the
-// lowest index, in their order. A cluster of 8 CTAs holds a row of weights in its shared memory (as unsigned keys that order
-// as the weights do: weights that are not above zero, NaN included, are all 0), finds the H-th largest key by three
-// histograms of 11, 10 and 10 bits that it adds up through distributed shared memory, and writes the list and the
-// weights of the kept tokens. A warp owns a contiguous part, so that positions follow from counts of the parts in front.
+// lowest index, in their order. The weights order as unsigned keys: their bits, or 0 where they are not above zero (NaN included).
+// kCtas CTAs (a cluster, or one of them for short rows) hold a row of weights in shared memory, find the H-th largest key by
+// three histograms of 11, 10 and 10 bits that they add up through distributed shared memory, and write the list and the weights
+// of the kept tokens. A warp owns a contiguous part, so that positions follow from counts of the parts in front.
+// What bounds it are the eight cluster barriers (about a microsecond each) and, for long rows, one trip of the weights.
 struct EvictParams {
     const float* mass;       // [B][Hkv][pitch]
     float* mass_out;         // [B][Hkv][pitch] or null
@@ -207,15 +213,20 @@ struct EvictParams {
     uint4* v_pages;
     uint4* hash_pages;       // or null
     int32_t* status;
+    uint32_t* ticket;        // [1] next piece of the move (cleared by the selection)
+    uint32_t* read;          // [B][Hkv][read_words] one bit per 64 kept rows: they have been read (cleared by the selection)
     int B, Hkv, max_pages, num_pages;
     int keep, sink, recent;
-    int share_max;           // keys of a CTA that its shared memory holds
+    int share_max;           // weights of a CTA that its shared memory holds
+    int read_words;
 };
 constexpr int kEvictCtas = 8;
 constexpr int kEvictThreads = 512;
 constexpr int kEvictWarps = kEvictThreads / 32;
 constexpr int kEvictBins = 2048;
-constexpr int kEvictShareCap = 40960;  // 160 KB of keys; longer rows are read again by each step
+constexpr int kEvictShareCap = 40960;  // 160 KB of weights; longer rows are read again by each step
+// Rows of up to this many tokens take one CTA: no cluster barriers.
+constexpr int kEvictOneCta = 8192;
 
 struct EvictCounts {
     int above, level;  // kept whatever happens (sink, recent, above the threshold); at the threshold
@@ -230,44 +241,63 @@ __device__ __forceinline__ int evict_len(const int32_t* seq_lens, int b, int max
     return S;
 }
 
-__global__ void __cluster_dims__(kEvictCtas, 1, 1) __launch_bounds__(kEvictThreads) evict_select_kernel(const EvictParams p) {
+template <int kCtas>
+__global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const EvictParams p) {
     namespace cg = cooperative_groups;
-    extern __shared__ uint32_t s_keys[];
+    extern __shared__ __align__(16) float s_mass[];
     __shared__ uint32_t s_hist[kEvictBins], s_total[kEvictBins];
     __shared__ uint32_t s_warp[kEvictWarps];
     __shared__ int s_bin;
     __shared__ uint32_t s_above;
     __shared__ EvictCounts s_cta, s_counts[kEvictWarps];
     cg::cluster_group cluster = cg::this_cluster();
+    auto sync_all = [&] {
+        if constexpr (kCtas > 1) cluster.sync();
+        else __syncthreads();
+    };
     pdl_wait();
     pdl_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int rank = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+    const int rank = kCtas > 1 ? blockIdx.x : 0, kvh = blockIdx.y, b = blockIdx.z, at_all = rank * kEvictThreads + tid;
+    constexpr int kAll = kCtas * kEvictThreads;
     const size_t pitch = (size_t)p.max_pages * kPage, unit = (size_t)b * p.Hkv + kvh;
     const float* mass = p.mass + unit * pitch;
     float* mass_out = p.mass_out != nullptr ? p.mass_out + unit * pitch : nullptr;
     int32_t* kept = p.kept + unit * p.keep;
-    const int S = evict_len(p.seq_lens, b, p.max_pages, rank == 0 && kvh == 0 && tid == 0, p.status);
+    for (int i = at_all; i < p.read_words; i += kAll) p.read[unit * p.read_words + i] = 0;
+    if (unit == 0 && at_all == 0) *p.ticket = 0;
+    const int S = evict_len(p.seq_lens, b, p.max_pages, at_all == 0 && kvh == 0, p.status);
     const int stay = S < 0 ? 0 : min(S, p.keep);
-    if (rank == 0 && kvh == 0 && tid == 0) p.lens_out[b] = S < 0 ? __ldg(p.seq_lens + b) : stay;
-    if (mass_out != nullptr)
-        for (size_t i = stay + rank * kEvictThreads + tid; i < pitch; i += kEvictCtas * kEvictThreads) mass_out[i] = 0.0f;
+    if (at_all == 0 && kvh == 0) p.lens_out[b] = S < 0 ? __ldg(p.seq_lens + b) : stay;
+    if (mass_out != nullptr) {
+        const int first4 = (stay + 3) & ~3;
+        if (at_all < first4 - stay) mass_out[stay + at_all] = 0.0f;
+        for (size_t i = first4 / 4 + at_all; i < pitch / 4; i += kAll) reinterpret_cast<float4*>(mass_out)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
     if (S <= p.keep) {  // (the same for the whole cluster)
-        for (int i = rank * kEvictThreads + tid; i < stay; i += kEvictCtas * kEvictThreads) {
+        for (int i = at_all; i < stay; i += kAll) {
             kept[i] = i;
             if (mass_out != nullptr) mass_out[i] = __ldg(mass + i);
         }
         return;
     }
     const int lo = p.sink, hi = S - p.recent, H = p.keep - p.sink - p.recent;
-    // this CTA's tokens, and this warp's part of them
-    const int share = ((S + kEvictCtas - 1) / kEvictCtas + 127) & ~127;
+    // this CTA's tokens
+    const int share = ((S + kCtas - 1) / kCtas + 127) & ~127;
     const int t0 = min(S, rank * share), t1 = min(S, t0 + share);
     const bool held = share <= p.share_max;
+    // four tokens from t on (t a multiple of 4; behind t1 there may be anything)
+    auto mass4_at = [&](int t) {
+        return held ? *reinterpret_cast<const float4*>(s_mass + (t - t0)) : __ldg(reinterpret_cast<const float4*>(mass + t));
+    };
     auto key_of = [&](float v) { return v > 0.0f ? __float_as_uint(v) : 0u; };
-    auto key_at = [&](int t) { return held ? s_keys[t - t0] : key_of(__ldg(mass + t)); };
-    if (held)
-        for (int t = t0 + tid; t < t1; t += kEvictThreads) s_keys[t - t0] = key_of(__ldg(mass + t));
+    if (held) {
+        // (rows are read to the next multiple of 4: the pitch is one of 256)
+        const float4* src = reinterpret_cast<const float4*>(mass + t0);
+        const int n4 = (t1 - t0 + 3) / 4;
+#pragma unroll 4
+        for (int i = tid; i < n4; i += kEvictThreads) reinterpret_cast<float4*>(s_mass)[i] = __ldg(src + i);
+    }
 
     // the H-th largest candidate's key, from its upper bits down
     uint32_t prefix = 0, wanted = (uint32_t)H;  // keys that agree with `prefix` above the step's bits; still to be found among them
@@ -279,26 +309,38 @@ __global__ void __cluster_dims__(kEvictCtas, 1, 1) __launch_bounds__(kEvictThrea
             const int shift = shifts[step], bins = 1 << widths[step];
             for (int i = tid; i < kEvictBins; i += kEvictThreads) s_hist[i] = 0;
             __syncthreads();
-            for (int t = max(t0, lo) + tid; t < min(t1, hi); t += kEvictThreads) {
-                const uint32_t k = key_at(t);
-                if (step == 0 || (k >> (shift + widths[step])) == prefix) atomicAdd(&s_hist[(k >> shift) & (bins - 1)], 1u);
-            }
-            cluster.sync();
-            // CTA r adds up the r-th eighth of the bins and hands the sums to all
-            const int per = kEvictBins / kEvictCtas;
-            if (tid < per) {
-                uint32_t sum = 0;
+            const int c0 = max(t0, lo), c1 = min(t1, hi);
+#pragma unroll 2
+            for (int t = t0 + 4 * tid; t < c1; t += 4 * kEvictThreads) {
+                const float4 v = mass4_at(t);
+                const float e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                for (int r = 0; r < kEvictCtas; ++r) sum += *cluster.map_shared_rank(&s_hist[rank * per + tid], r);
-#pragma unroll
-                for (int r = 0; r < kEvictCtas; ++r) *cluster.map_shared_rank(&s_total[rank * per + tid], r) = sum;
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t k = key_of(e[q]);
+                    if (t + q >= c0 && t + q < c1 && (step == 0 || (k >> (shift + widths[step])) == prefix))
+                        atomicAdd(&s_hist[(k >> shift) & (bins - 1)], 1u);
+                }
             }
-            cluster.sync();
+            sync_all();
+            const uint32_t* total = s_hist;
+            if constexpr (kCtas > 1) {
+                // CTA r adds up the r-th eighth of the bins and hands the sums to all
+                constexpr int per = kEvictBins / kCtas;
+                if (tid < per) {
+                    uint32_t sum = 0;
+#pragma unroll
+                    for (int r = 0; r < kCtas; ++r) sum += *cluster.map_shared_rank(&s_hist[rank * per + tid], r);
+#pragma unroll
+                    for (int r = 0; r < kCtas; ++r) *cluster.map_shared_rank(&s_total[rank * per + tid], r) = sum;
+                }
+                cluster.sync();
+                total = s_total;
+            }
             // the bin in which the wanted-th largest lies: thread i has 4 bins, from the top down
             uint32_t mine[4], sum = 0;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                mine[q] = s_total[kEvictBins - 1 - (4 * tid + q)];
+                mine[q] = total[kEvictBins - 1 - (4 * tid + q)];
                 sum += mine[q];
             }
             uint32_t incl = sum;
@@ -327,25 +369,28 @@ __global__ void __cluster_dims__(kEvictCtas, 1, 1) __launch_bounds__(kEvictThrea
         }
         threshold = prefix;
     }
-    // wanted = tokens at the threshold that stay (the lowest ones)
-    const int part = ((t1 - t0 + kEvictWarps - 1) / kEvictWarps + 31) & ~31;
+    // wanted = tokens at the threshold that stay (the lowest ones); this warp's part of the CTA's tokens, four per lane and step
+    const int part = ((t1 - t0 + kEvictWarps - 1) / kEvictWarps + 127) & ~127;
     const int w0 = min(t1, t0 + warp * part), w1 = min(t1, w0 + part);
-    auto classify = [&](int t, bool& above, bool& level) {
-        above = level = false;
-        if (t >= w1) return;
-        if (t < lo || t >= hi) above = true;
-        else if (H > 0) {
-            const uint32_t k = key_at(t);
-            above = k > threshold;
-            level = k == threshold;
-        }
+    // of token t (weight v): 1 kept whatever happens, 1 << 16 at the threshold, 0 dropped
+    auto classify = [&](int t, float v) -> uint32_t {
+        if (t >= w1) return 0;
+        if (t < lo || t >= hi) return 1;
+        const uint32_t k = key_of(v);
+        return H == 0 ? 0u : (k > threshold ? 1u : (k == threshold ? 1u << 16 : 0u));
     };
     EvictCounts mine = {0, 0};
-    for (int t = w0 + lane; t - lane < w1; t += 32) {
-        bool above, level;
-        classify(t, above, level);
-        mine.above += __popc(__ballot_sync(0xffffffffu, above));
-        mine.level += __popc(__ballot_sync(0xffffffffu, level));
+#pragma unroll 2
+    for (int t = w0 + 4 * lane; t < w1; t += 128) {
+        const float4 v = mass4_at(t);
+        const uint32_t c = classify(t, v.x) + classify(t + 1, v.y) + classify(t + 2, v.z) + classify(t + 3, v.w);
+        mine.above += c & 0xffff;
+        mine.level += c >> 16;
+    }
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) {
+        mine.above += __shfl_xor_sync(0xffffffffu, mine.above, i);
+        mine.level += __shfl_xor_sync(0xffffffffu, mine.level, i);
     }
     if (lane == 0) s_counts[warp] = mine;
     __syncthreads();
@@ -354,102 +399,198 @@ __global__ void __cluster_dims__(kEvictCtas, 1, 1) __launch_bounds__(kEvictThrea
         if (q < warp) front.above += s_counts[q].above, front.level += s_counts[q].level;
         cta.above += s_counts[q].above, cta.level += s_counts[q].level;
     }
-    if (tid == 0) s_cta = cta;
-    cluster.sync();
-    for (int r = 0; r < rank; ++r) {
-        const EvictCounts c = *cluster.map_shared_rank(&s_cta, r);
-        front.above += c.above, front.level += c.level;
-    }
-    cluster.sync();  // no CTA leaves while another reads its shared memory
-    const int quota = (int)wanted;
-    const uint32_t below = (1u << lane) - 1u;
-    for (int t = w0 + lane; t - lane < w1; t += 32) {
-        bool above, level;
-        classify(t, above, level);
-        const uint32_t ma = __ballot_sync(0xffffffffu, above), ml = __ballot_sync(0xffffffffu, level);
-        const int lrank = front.level + __popc(ml & below);
-        if (above || (level && lrank < quota)) {
-            const int at = front.above + __popc(ma & below) + min(lrank, quota);
-            if (at < p.keep) {
-                kept[at] = t;
-                if (mass_out != nullptr) mass_out[at] = __ldg(mass + t);
-            }
+    if constexpr (kCtas > 1) {
+        if (tid == 0) s_cta = cta;
+        cluster.sync();
+        for (int r = 0; r < rank; ++r) {
+            const EvictCounts c = *cluster.map_shared_rank(&s_cta, r);
+            front.above += c.above, front.level += c.level;
         }
-        front.above += __popc(ma);
-        front.level += __popc(ml);
+        cluster.sync();  // no CTA leaves while another reads its shared memory
+    }
+    const int quota = (int)wanted;
+    for (int t = w0 + 4 * lane; t - 4 * lane < w1; t += 128) {
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (t < w1) v = mass4_at(t);
+        const float e[4] = {v.x, v.y, v.z, v.w};
+        uint32_t c[4], sum = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            c[q] = classify(t + q, e[q]);
+            sum += c[q];
+        }
+        uint32_t incl = sum;  // (128 tokens at most: no carry between the halves)
+#pragma unroll
+        for (int i = 1; i < 32; i <<= 1) {
+            const uint32_t u = __shfl_up_sync(0xffffffffu, incl, i);
+            if (lane >= i) incl += u;
+        }
+        const uint32_t all = __shfl_sync(0xffffffffu, incl, 31);
+        int above = front.above + (int)((incl - sum) & 0xffff), level = front.level + (int)((incl - sum) >> 16);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (c[q] == 1u || (c[q] != 0u && level < quota)) {
+                const int at = above + min(level, quota);
+                if (at < p.keep) {
+                    kept[at] = t + q;
+                    if (mass_out != nullptr) mass_out[at] = e[q];
+                }
+            }
+            above += c[q] & 0xffff;
+            level += c[q] >> 16;
+        }
+        front.above += all & 0xffff;
+        front.level += all >> 16;
     }
 }
 
 // ---- eviction: rows kept[i] -> i ------------------------------------------------------------------------------------------
-// In place: kept is ascending, so a row never moves up and the row that place i receives lies at or behind every place written
-// before. A CTA owns a 64-byte column of K or of V (or the code words) of one (sequence, kv-head) and takes its rows in order, a batch at
-// a time: all loads of a batch are complete (a barrier) before its first store, and a later batch reads rows behind all
-// places written so far, so its loads run ahead of those stores.
+// In place: kept is ascending, so a row never moves up, and place i may be written once the row that lies there, if it is a
+// kept one, has been read; that row goes to a place up to i. The rows of a (sequence, kv-head) are moved in pieces of 64, handed
+// out in order (a ticket); a CTA reads its piece into registers (a warp per row of K and V, 16 bytes per lane), says so, waits until
+// the pieces in front of its own whose rows lie on its places have been read, and writes. The pieces it waits for have been handed
+// out before, so they are on some running CTA and need nothing from this one; the wait is bounded all the same. Pieces of
+// different units are handed out in turn and a list's rows lie far behind their places, so the wait is over before it begins.
 constexpr int kMoveThreads = 256;
-constexpr int kMoveRows = 8;  // rows per thread and batch
-template <int kPieces>        // 16-byte pieces of a row per CTA
-__device__ __forceinline__ void evict_move(const EvictParams& p, uint4* pool, int row_pieces, int first_piece, int b, int kvh, int S) {
-    constexpr int kRowsPer = kMoveThreads / kPieces, kBatch = kRowsPer * kMoveRows;
-    const int32_t* kept = p.kept + ((size_t)b * p.Hkv + kvh) * p.keep;
-    const int piece = first_piece + threadIdx.x % kPieces, r0 = threadIdx.x / kPieces;
-    auto slot = [&](int token) {
-        int page = __ldg(p.page_table + (size_t)b * p.max_pages + token / kPage);
-        if (page < 0 || page >= p.num_pages) {
-            report(p.status, HA_ERR_BAD_PAGE);
-            return (size_t)-1;
-        }
-        return ((size_t)page * p.Hkv + kvh) * kPage + token % kPage;
-    };
-    uint4 v[2][kMoveRows];
-    uint32_t have[2] = {0, 0};
-    auto load = [&](int base, uint4 (&buf)[kMoveRows], uint32_t& mask) {
-        int src[kMoveRows];
-#pragma unroll
-        for (int k = 0; k < kMoveRows; ++k) {
-            const int i = base + k * kRowsPer + r0;
-            src[k] = i < p.keep ? __ldcg(kept + i) : i;
-        }
-        mask = 0;
-#pragma unroll
-        for (int k = 0; k < kMoveRows; ++k) {
-            const int i = base + k * kRowsPer + r0;
-            if (src[k] > i && src[k] < S) {
-                const size_t s = slot(src[k]);
-                if (s != (size_t)-1) {
-                    buf[k] = __ldcg(pool + s * row_pieces + piece);
-                    mask |= 1u << k;
-                }
-            }
-        }
-    };
-    auto store = [&](int base, const uint4 (&buf)[kMoveRows], uint32_t mask) {
-#pragma unroll
-        for (int k = 0; k < kMoveRows; ++k) {
-            if ((mask >> k) & 1u) {
-                const size_t s = slot(base + k * kRowsPer + r0);
-                if (s != (size_t)-1) pool[s * row_pieces + piece] = buf[k];
-            }
-        }
-    };
-    load(0, v[0], have[0]);
-    for (int base = 0; base < p.keep; base += 2 * kBatch) {
-        load(base + kBatch, v[1], have[1]);
-        __syncthreads();
-        store(base, v[0], have[0]);
-        load(base + 2 * kBatch, v[0], have[0]);
-        __syncthreads();
-        store(base + kBatch, v[1], have[1]);
+constexpr int kMoveWarps = kMoveThreads / 32;
+constexpr int kMovePiece = 64;                       // rows
+constexpr int kMoveRows = kMovePiece / kMoveWarps;   // rows per warp
+constexpr int kMoveCtasPerSm = 4;
+
+struct MovePiece {
+    uint32_t unit, piece;
+    int src, dst;  // lanes 0 .. 7 of a warp: its rows, as row numbers of the pool (-1: nothing to do)
+    bool moves;    // (the whole CTA) the sequence is cut
+};
+__device__ __forceinline__ MovePiece move_lookup(const EvictParams& p, uint32_t ticket, uint32_t units, uint32_t total, int warp, int lane) {
+    MovePiece m;
+    m.piece = ticket / units;
+    m.unit = ticket - m.piece * units;
+    m.src = m.dst = -1;
+    m.moves = false;
+    if (ticket >= total) return m;
+    const int b = (int)(m.unit / (uint32_t)p.Hkv), kvh = (int)m.unit - b * p.Hkv;
+    const int i = (int)m.piece * kMovePiece + warp * kMoveRows + lane;
+    const bool looks = lane < kMoveRows && i < p.keep;
+    const int S = evict_len(p.seq_lens, b, p.max_pages, false, p.status);
+    const int token = looks ? __ldcg(p.kept + (size_t)m.unit * p.keep + i) : i;
+    m.moves = S > p.keep;
+    if (m.moves && looks && token > i && token < S) {
+        const int32_t* table = p.page_table + (size_t)b * p.max_pages;
+        const int from = __ldg(table + token / kPage), to = __ldg(table + i / kPage);
+        if (from >= 0 && from < p.num_pages && to >= 0 && to < p.num_pages) {
+            m.src = (from * p.Hkv + kvh) * kPage + token % kPage;
+            m.dst = (to * p.Hkv + kvh) * kPage + i % kPage;
+        } else report(p.status, HA_ERR_BAD_PAGE);
     }
+    return m;
 }
-constexpr int kMoveColumns = 9;  // four of K, four of V, the code words
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictParams p) {
+
+// The pieces [lo, hi) in front of `piece` that have rows on its places, by a whole warp: lo is the number of pieces whose last
+// row lies in front of the places, hi that of those whose first row does not lie behind them.
+__device__ __forceinline__ void move_conflicts(const int32_t* kept, int keep, int piece, int lane, int& lo, int& hi) {
+    const int first = piece * kMovePiece, last = first + kMovePiece - 1;
+    int base[2] = {0, 0}, left[2] = {piece, piece};  // the answers lie in [base, base + left]
+    while (max(left[0], left[1]) > 0) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int step = (left[e] + 31) / 32;  // lane l looks at the last piece of the l-th part
+            const int at = base[e] + min(left[e], (lane + 1) * step) - 1;
+            bool in = false;
+            if (left[e] > 0 && lane * step < left[e]) {
+                const int row = e == 0 ? min(keep - 1, at * kMovePiece + kMovePiece - 1) : at * kMovePiece;
+                const int token = __ldcg(kept + row);
+                in = e == 0 ? token < first : token <= last;
+            }
+            const int parts = __popc(__ballot_sync(0xffffffffu, in));  // (ascending: the parts that lie in front as a whole)
+            const int skip = min(left[e], parts * step);
+            base[e] += skip;
+            left[e] = max(0, min(left[e] - skip, step - 1));
+        }
+    }
+    lo = base[0];
+    hi = base[1];
+}
+
+__global__ void __launch_bounds__(kMoveThreads, kMoveCtasPerSm) evict_move_kernel(const EvictParams p) {
+    __shared__ uint32_t s_ticket[2];
+    __shared__ int s_ok;
     pdl_wait();
     pdl_launch_dependents();
-    const int column = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
-    const int S = evict_len(p.seq_lens, b, p.max_pages, false, p.status);
-    if (S <= p.keep) return;
-    if (column < 8) evict_move<4>(p, column < 4 ? p.k_pages : p.v_pages, 16, (column & 3) * 4, b, kvh, S);
-    else if (p.hash_pages != nullptr) evict_move<1>(p, p.hash_pages, 1, 0, b, kvh, S);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t units = (uint32_t)(p.B * p.Hkv), total = units * (uint32_t)((p.keep + kMovePiece - 1) / kMovePiece);
+    if (tid == 0) s_ticket[0] = atomicAdd(p.ticket, 1u);
+    __syncthreads();
+    uint32_t ticket = s_ticket[0];
+    MovePiece m = move_lookup(p, ticket, units, total, warp, lane);
+    for (int round = 1; ticket < total; ++round) {
+        if (tid == 0) s_ticket[round & 1] = atomicAdd(p.ticket, 1u);
+        uint4 v[kMoveRows], code;
+        const size_t column = lane & 15;
+        const uint4* pool = (lane < 16 ? p.k_pages : p.v_pages) + column;
+#pragma unroll
+        for (int k = 0; k < kMoveRows; ++k) {
+            const int s = __shfl_sync(0xffffffffu, m.src, k);
+            if (s >= 0) v[k] = __ldcg(pool + (size_t)s * 16);
+        }
+        if (m.src >= 0 && p.hash_pages != nullptr) code = __ldcg(p.hash_pages + m.src);
+        int lo = 0, hi = 0;
+        if (m.moves && warp == 0) move_conflicts(p.kept + (size_t)m.unit * p.keep, p.keep, (int)m.piece, lane, lo, hi);
+        // Every thread's rows are read: the barrier takes a predicate formed from them, so that none is still on its way.
+        uint32_t arrived = m.src >= 0 && p.hash_pages != nullptr ? code.x : 0u;
+#pragma unroll
+        for (int k = 0; k < kMoveRows; ++k)
+            if (__shfl_sync(0xffffffffu, m.src, k) >= 0) arrived ^= v[k].x;
+        __syncthreads_or(arrived == 0x5bd1e995u);
+        if (m.moves && warp == 0) {
+            uint32_t* read = p.read + (size_t)m.unit * p.read_words;
+            if (lane == 0) {
+                __threadfence();
+                atomicOr(read + m.piece / 32, 1u << (m.piece & 31));
+            }
+            bool all = true;
+            for (int w0 = lo / 32; w0 * 32 < hi && all; w0 += 32) {
+                const int w = w0 + lane;
+                uint32_t want = 0;  // bits lo .. hi - 1
+                if (w * 32 < hi && w * 32 + 32 > lo) {
+                    want = 0xffffffffu;
+                    if (w * 32 < lo) want &= 0xffffffffu << (lo - w * 32);
+                    if (w * 32 + 32 > hi) want &= 0xffffffffu >> (w * 32 + 32 - hi);
+                }
+                bool done = want == 0;
+                for (int spin = 0; spin < (1 << 20); ++spin) {
+                    if (!done) {
+                        uint32_t have;
+                        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(have) : "l"(read + w) : "memory");
+                        done = (have & want) == want;
+                    }
+                    if (__all_sync(0xffffffffu, done) != 0) break;
+                    __nanosleep(100);
+                }
+                all = __all_sync(0xffffffffu, done) != 0;
+            }
+            if (lane == 0) {
+                __threadfence();
+                if (!all) report(p.status, HA_ERR_TIMEOUT);
+                s_ok = all ? 1 : 0;
+            }
+        }
+        // the next piece's rows are looked up under this one's wait
+        ticket = s_ticket[round & 1];
+        const MovePiece next = move_lookup(p, ticket, units, total, warp, lane);
+        __syncthreads();
+        if (m.moves && s_ok != 0) {
+            uint4* to_pool = (lane < 16 ? p.k_pages : p.v_pages) + column;
+#pragma unroll
+            for (int k = 0; k < kMoveRows; ++k) {
+                const int s = __shfl_sync(0xffffffffu, m.src, k), t = __shfl_sync(0xffffffffu, m.dst, k);
+                if (s >= 0) to_pool[(size_t)t * 16] = v[k];
+            }
+            if (m.src >= 0 && p.hash_pages != nullptr) p.hash_pages[m.dst] = code;
+        }
+        m = next;
+        __syncthreads();  // (s_ok has been read)
+    }
 }
 
 }  // namespace ha

@@ -82,6 +82,10 @@ int launch_tree(void (*kernel)(TreeAttentionParams, CUtensorMap, CUtensorMap), i
     return launch(tree_merge_kernel<kTile, kRows>, grid, dim3(kTreeMergeWarps * 32), st, 1, p, ctas) == cudaSuccess ? HA_OK : HA_ERR_LAUNCH;
 }
 
+// Words of one bit per 64 kept rows, for the largest budget a sequence can exceed.
+int evict_read_words(const ha_shape_t* s) { return (s->max_pages * (kPage / kMovePiece) + 31) / 32; }
+size_t evict_workspace(const ha_shape_t* s) { return 16 + (size_t)s->batch * s->num_kv_heads * evict_read_words(s) * sizeof(uint32_t); }
+
 }  // namespace
 }  // namespace ha
 
@@ -203,15 +207,21 @@ int ha_tree_commit(const ha_shape_t* shape, const ha_tree_t* tree, const uint32_
                    cudaSuccess ? HA_OK : HA_ERR_LAUNCH;
 }
 
+size_t ha_evict_workspace_bytes(const ha_shape_t* shape) { return check_shape(shape) == HA_OK ? evict_workspace(shape) : 0; }
+
 int ha_cache_evict(const ha_shape_t* shape, int32_t keep_tokens, int32_t init_budget, int32_t recent_budget, const float* mass, void* k_pages,
                    void* v_pages, uint32_t* hash_pages, const int32_t* page_table, const int32_t* seq_lens, int32_t* kept, float* mass_out,
-                   int32_t* lens_out, int32_t* status, void* stream) {
+                   int32_t* lens_out, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
     const int rc = check_shape(shape);
     if (rc != HA_OK) return rc;
     if (mass == nullptr || k_pages == nullptr || v_pages == nullptr || page_table == nullptr || seq_lens == nullptr || kept == nullptr ||
         lens_out == nullptr || status == nullptr || mass == mass_out || seq_lens == lens_out || !aligned16(k_pages) || !aligned16(v_pages) ||
-        !aligned16(hash_pages) || keep_tokens < 1 || init_budget < 0 || recent_budget < 0 || (long long)init_budget + recent_budget > keep_tokens)
+        !aligned16(hash_pages) || !aligned16(mass) || !aligned16(mass_out) || !aligned16(workspace) || keep_tokens < 1 || init_budget < 0 ||
+        recent_budget < 0 || (long long)init_budget + recent_budget > keep_tokens)
         return HA_ERR_BAD_ARG;
+    if (workspace == nullptr || workspace_bytes < evict_workspace(shape)) return HA_ERR_WORKSPACE;
+    if ((long long)shape->num_pages * shape->num_kv_heads * kPage > 0x7fffffffll) return HA_ERR_UNSUPPORTED_DIM;  // (row numbers are 32 bits)
+    const long long capacity = (long long)shape->max_pages * kPage;
     EvictParams p;
     p.mass = mass;
     p.mass_out = mass_out;
@@ -223,6 +233,9 @@ int ha_cache_evict(const ha_shape_t* shape, int32_t keep_tokens, int32_t init_bu
     p.v_pages = static_cast<uint4*>(v_pages);
     p.hash_pages = reinterpret_cast<uint4*>(hash_pages);
     p.status = status;
+    p.ticket = static_cast<uint32_t*>(workspace);
+    p.read = p.ticket + 4;
+    p.read_words = evict_read_words(shape);
     p.B = shape->batch;
     p.Hkv = shape->num_kv_heads;
     p.max_pages = shape->max_pages;
@@ -230,15 +243,22 @@ int ha_cache_evict(const ha_shape_t* shape, int32_t keep_tokens, int32_t init_bu
     p.keep = keep_tokens;
     p.sink = init_budget;
     p.recent = recent_budget;
-    const long long share = (((long long)shape->max_pages * kPage + kEvictCtas - 1) / kEvictCtas + 127) & ~127ll;
-    p.share_max = (int)std::min<long long>(share, kEvictShareCap);
-    const size_t smem = (size_t)p.share_max * sizeof(uint32_t);
-    if (cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return HA_ERR_LAUNCH;
+    int sms = 0;
+    if (sm_count(sms) != HA_OK) return HA_ERR_LAUNCH;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (launch_smem(evict_select_kernel, dim3(kEvictCtas, shape->num_kv_heads, shape->batch), dim3(kEvictThreads), smem, st, 1, p) != cudaSuccess)
+    const bool one = capacity <= kEvictOneCta;
+    const int ctas = one ? 1 : kEvictCtas;
+    p.share_max = (int)std::min<long long>(((capacity + ctas - 1) / ctas + 127) & ~127ll, kEvictShareCap);
+    const size_t smem = (size_t)p.share_max * sizeof(float);
+    auto select = one ? evict_select_kernel<1> : evict_select_kernel<kEvictCtas>;
+    if (cudaFuncSetAttribute(select, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+        launch_smem(select, dim3(ctas, shape->num_kv_heads, shape->batch), dim3(kEvictThreads), smem, st, one ? 1 : kEvictCtas, p) != cudaSuccess)
         return HA_ERR_LAUNCH;
-    return launch(evict_move_kernel, dim3(kMoveColumns, shape->num_kv_heads, shape->batch), dim3(kMoveThreads), st, 1, p) == cudaSuccess ? HA_OK
-                                                                                                                                           : HA_ERR_LAUNCH;
+    // (sequences are no longer than the capacity, so larger budgets move nothing)
+    if (keep_tokens >= capacity) return HA_OK;
+    const long long pieces = (long long)shape->batch * shape->num_kv_heads * ((keep_tokens + kMovePiece - 1) / kMovePiece);
+    return launch(evict_move_kernel, dim3((unsigned)std::min<long long>(pieces, (long long)sms * kMoveCtasPerSm)), dim3(kMoveThreads), st, 1, p) ==
+                   cudaSuccess ? HA_OK : HA_ERR_LAUNCH;
 }
 
 }  // extern "C"

@@ -368,17 +368,18 @@ constexpr int kTreeMergeWarps = 4;
 template <int kTile, int kRows>
 __global__ void __launch_bounds__(kTreeMergeWarps * 32) tree_merge_kernel(const TreeAttentionParams p, int ctas) {
     using Cut = DenseCut<kTile, kRows>;
-    pdl_wait();
-    pdl_launch_dependents();
+    // The lengths are read before the wait: the attention kernel in front does not write them, and what did has completed.
     const int lane = threadIdx.x & 31, r = blockIdx.z * kTreeMergeWarps + (threadIdx.x >> 5), b = blockIdx.y;
     const int max_groups = Cut::groups(p.seqs.T);
     const int kvh = blockIdx.x / max_groups, group = blockIdx.x - kvh * max_groups;
     int S, n;
     dense_seq(p.seqs, b, false, S, n);
     const int row = group * kRows + r;
-    if (row >= n * kGroup) return;
     long long quota, before;
     Cut::count(p.seqs, ctas, lane, b, quota, before);
+    pdl_wait();
+    pdl_launch_dependents();
+    if (row >= n * kGroup) return;
     const int tiles = (S + kTile - 1) / kTile;
     const long long start = before + (long long)(kvh * Cut::groups(n) + group) * tiles;
     const int c0 = (int)(start / quota), c1 = (int)((start + tiles - 1) / quota);

@@ -108,9 +108,9 @@ class TreeAccept:
 
     @staticmethod
     def empty(batch: int, device) -> "TreeAccept":
-        i32 = dict(dtype=torch.int32, device=device)
-        return TreeAccept(torch.empty(batch, MASK_WORDS, **i32), torch.empty(batch, **i32),
-                          torch.empty(batch, dtype=torch.int64, device=device), torch.empty(batch, **i32))
+        count = torch.empty(batch, dtype=torch.int32, device=device)
+        return TreeAccept(count.new_empty((batch, MASK_WORDS)), count, torch.empty(batch, dtype=torch.int64, device=device),
+                          torch.empty_like(count))
 
 
 def tree_accept(draft: torch.Tensor, parents: torch.Tensor, target: torch.Tensor, tree_lens: torch.Tensor | None,
@@ -163,6 +163,10 @@ class DenseDecodeContext:
         self.shape = _lib.HaShape(self.batch, self.num_kv_heads, GROUP, HEAD_DIM, PAGE, cache.max_pages, cache.num_pages, 1)
         self.workspace_bytes = int(self.lib.ha_tree_workspace_bytes(self.max_nodes))
         self.workspace = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=self.device)
+        self.evict_workspace_bytes = int(self.lib.ha_evict_workspace_bytes(self.shape))
+        if self.evict_workspace_bytes == 0:
+            raise ValueError("invalid shape for the CUDA library")
+        self.evict_workspace = torch.empty(self.evict_workspace_bytes, dtype=torch.uint8, device=self.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
 
     @property
@@ -292,6 +296,7 @@ class DenseDecodeContext:
             rc = self.lib.ha_cache_evict(
                 self.shape, keep_tokens, init_budget, recent_budget, mass.data_ptr(), c.k_pages.data_ptr(), c.v_pages.data_ptr(),
                 c.hash_pages.data_ptr(), c.page_table.data_ptr(), c.seq_lens.data_ptr(), kept.data_ptr(), mass_out.data_ptr(),
-                lens_out.data_ptr(), self.status.data_ptr(), _stream_ptr(self.device))
+                lens_out.data_ptr(), self.evict_workspace.data_ptr(), self.evict_workspace_bytes, self.status.data_ptr(),
+                _stream_ptr(self.device))
         _raise_on(rc, "ha_cache_evict")
         return kept, mass_out, lens_out

@@ -396,7 +396,10 @@ int ha_tree_commit(const ha_shape_t* shape, const ha_tree_t* tree, const uint32_
 int ha_cache_evict(const ha_shape_t* shape, int32_t keep_tokens, int32_t init_budget, int32_t recent_budget,
                    const float* mass, void* k_pages, void* v_pages, uint32_t* hash_pages, const int32_t* page_table,
                    const int32_t* seq_lens, int32_t* kept, float* mass_out, int32_t* lens_out,
-                   int32_t* status, void* stream);
+                   void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+/* Its workspace (0 for an invalid shape): needs no initialisation, keeps nothing between calls; one per call that may run at
+ * the same time. Host-only arithmetic.                                                                               */
+size_t ha_evict_workspace_bytes(const ha_shape_t* shape);
 
 #ifdef __cplusplus
 }

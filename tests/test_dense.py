@@ -612,7 +612,7 @@ def test_entry_points_refuse_bad_arguments_before_launching():
             setattr(s, k, v)
         assert attend(s) == mass(s) == _lib.HA_ERR_UNSUPPORTED_DIM
         assert lib.ha_tree_commit(s, tree, X, X, X, N, X, X, N, X, N) == _lib.HA_ERR_UNSUPPORTED_DIM
-        assert lib.ha_cache_evict(s, 10, 1, 1, X, X, X, N, X, X, X, N, ctypes.c_void_p(512), X, N) == _lib.HA_ERR_UNSUPPORTED_DIM
+        assert lib.ha_cache_evict(s, 10, 1, 1, X, X, X, N, X, X, X, N, ctypes.c_void_p(512), X, 1 << 40, X, N) == _lib.HA_ERR_UNSUPPORTED_DIM
     assert attend(t=_lib.HaTree(129, None, None)) == mass(t=_lib.HaTree(129, None, None)) == _lib.HA_ERR_UNSUPPORTED_DIM
     assert attend(t=_lib.HaTree(0, None, None)) == mass(t=_lib.HaTree(-1, None, None)) == bad
     for scale in (0.0, -1.0, math.nan, math.inf):
@@ -631,10 +631,11 @@ def test_entry_points_refuse_bad_arguments_before_launching():
     assert lib.ha_tree_commit(good, tree, N, X, X, N, X, X, N, X, N) == bad
     assert lib.ha_tree_commit(good, tree, ctypes.c_void_p(260), X, X, N, X, X, N, X, N) == bad
 
-    def evict(keep=10, sink=1, recent=1, m=X, mo=N, lens=X, lo=ctypes.c_void_p(512)):
-        return lib.ha_cache_evict(good, keep, sink, recent, m, X, X, N, X, lens, X, mo, lo, X, N)
+    def evict(keep=10, sink=1, recent=1, m=X, mo=N, lens=X, lo=ctypes.c_void_p(512), ws=X, n=1 << 40):
+        return lib.ha_cache_evict(good, keep, sink, recent, m, X, X, N, X, lens, X, mo, lo, ws, n, X, N)
 
     assert evict(keep=0) == evict(sink=-1) == evict(recent=-1) == evict(sink=6, recent=5) == evict(mo=X) == evict(lo=X) == evict(m=N) == bad
+    assert evict(ws=N) == evict(n=8) == _lib.HA_ERR_WORKSPACE
     assert evict(keep=2 ** 31 - 1, sink=2 ** 31 - 1, recent=2 ** 31 - 1) == bad
 
 
