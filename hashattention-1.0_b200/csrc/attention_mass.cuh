@@ -3,8 +3,23 @@
 //   mass[j] += sum_{i in rows, g} e^{c q_ig.k_j - lse_ig}   over the rows that see token j
 //
 // per (sequence, kv-head), with the log-sum-exps the attention left: one more pass over K, no V. The transposed product
-// K Q^T puts the tokens on the rows of the matrix instruction, so a token's sum stays inside a quad of lanes. No atomics: a
-// token's sum is formed by one warp in a fixed order.
+// S = K Q^T runs on the 5th-generation tensor cores (tcgen05): the 128 tokens of a tile are the lanes of tensor memory, the counted
+// query rows its columns, so a thread adds up its token's weights without another one's help. The query rows (4 per counted node,
+// up to 512) stay in shared memory as the B operand, N = 16 to 256 columns at a time, so few rows cost few products.
+//
+// Roles of the warps: 0 issues the products, 1 loads K tiles by TMA (two boxes of 64 elements x 128 tokens, 128-byte swizzle) into a
+// ring of 32 KB slots, 4 - 19 turn scores into weights, in two groups of eight that take every second tile (a buffer of 256 columns
+// of tensor memory each): four quarters of the lanes times two halves of the columns. The halves of a token's sum meet
+// in shared memory; no atomics, a token's sum is formed in a fixed order and stored by one thread, which has asked for the old
+// value before the scores arrive.
+//
+// With few rows the bytes of K bound it; with 256 and more the exponentials do: 16 a clock on an SM, 2048 clocks for the
+// 128 x 256 scores whose K tile takes 1400 to arrive at the copy rate and whose products take 1024.
+//
+// Precision: c * s and lse are numbers of magnitude 10 to 50 whose difference is exponentiated. The multiply-add rounds only that
+// difference; what the rounding of c and of lse * log2(e) to fp32 would add (1e-6 of a weight) is taken out: lse is multiplied by
+// the fp32 value of c over its exact one, and by what the products leave of a score (kScoreCut), in 64 bits (where weights matter,
+// c s = lse), rounded to fp32, and what that leaves is a factor of the row, 2^(rest), applied in the multiply-add of the sum.
 #pragma once
 
 #include "tree_attention.cuh"
@@ -18,23 +33,44 @@ struct AttentionMassParams {
     const float* lse;        // [B][T][Hq]
     const uint32_t* rows;    // [B][4] the nodes whose weights count, or null: all of the tree
     float* mass;             // [B][Hkv][max_pages * 256]
-    float scale_log2;
+    float scale_log2;        // c * log2(e), rounded
+    double lse_scale;        // log2(e) * scale_log2 / (c * log2(e)) * (1 - kScoreCut)
+    int q_rows;              // rows of the query operand: 4 T, to a multiple of 16
+    int slots;               // of the ring
 };
 
-constexpr int kMassTile = 64;
+constexpr int kMassTile = 128;
 constexpr int kMassMaxRows = kMaxNodes * kGroup;
-constexpr uint32_t kMassStage = 2 * kRowsHalf;  // K of a tile: 16 KB
-constexpr int kMassStages = 4;
-constexpr uint32_t kMassOffQ = kMassStages * kMassStage;               // [2 halves][512 rows][64] bf16, 128-byte swizzle
-constexpr uint32_t kMassQHalf = kMassMaxRows * 128;
-constexpr uint32_t kMassOffLse = kMassOffQ + 2 * kMassQHalf;           // [512] lse * log2(e), +inf where there is no row
-constexpr uint32_t kMassOffMask = kMassOffLse + kMassMaxRows * 4;      // [128] mask words of the counted nodes
-constexpr uint32_t kMassOffBar = kMassOffMask + kMaxNodes * 16;
-constexpr uint32_t kMassOffAbort = kMassOffBar + 2 * kMassStages * 8;
-constexpr uint32_t kMassSmemBytes = kMassOffAbort + 16 + 1024;
-static_assert(kMassSmemBytes <= 227 * 1024, "shared memory of one CTA");
+constexpr int kMassCols = 256;                  // columns of a buffer of tensor memory
+constexpr uint32_t kMassSlot = 2 * 128 * 128;   // K of a tile: 32 KB
+constexpr uint32_t kMassHalf = 128 * 128;
+constexpr int kMassMaxSlots = 6;
+constexpr int kMassWarp0 = 4;
+constexpr int kMassWarps = 16;
+constexpr int kMassThreads = (kMassWarp0 + kMassWarps) * 32;
+// Shared memory: the fixed part, then the ring, then the queries (two halves of 64 elements, 128 bytes a row).
+constexpr int kMassBarFull = 0;                               // [slots] the loader's arrival and the bytes of two copies
+constexpr int kMassBarEmpty = kMassBarFull + kMassMaxSlots;   // [slots] commit: the products have read the tile
+constexpr int kMassBarS = kMassBarEmpty + kMassMaxSlots;      // [2 groups] commit: scores complete
+constexpr int kMassBarRead = kMassBarS + 2;                   // [2 groups] 8 warps: scores read
+constexpr int kMassBarQ = kMassBarRead + 2;                   // 16 warps: the unit's queries are in place
+constexpr int kMassBarFinal = kMassBarQ + 1;
+constexpr int kMassBars = kMassBarFinal + 1;
+constexpr uint32_t kMassOffLse = 0;                                    // [512] -lse in powers of two, rounded; -inf where there is no row
+constexpr uint32_t kMassOffFactor = kMassOffLse + kMassMaxRows * 4;    // [512] the factor of the row
+constexpr uint32_t kMassOffVis = kMassOffFactor + kMassMaxRows * 4;    // [128 drafts] counted nodes that see the draft, one bit each
+constexpr uint32_t kMassOffPart = kMassOffVis + kMaxNodes * 16;        // [2 groups][2 tiles][128] sums of the second half of the columns
+constexpr uint32_t kMassOffBar = kMassOffPart + 2 * 2 * 128 * 4;
+constexpr uint32_t kMassOffTmem = kMassOffBar + kMassBars * 8;
+constexpr uint32_t kMassOffRing = (kMassOffTmem + 8 + 1023) / 1024 * 1024;
+__host__ __device__ constexpr size_t mass_smem_bytes(int slots, int q_rows) { return kMassOffRing + (size_t)slots * kMassSlot + (size_t)q_rows * 256 + 1024; }
+inline int mass_slots(int q_rows) {
+    int slots = kMassMaxSlots;
+    while (mass_smem_bytes(slots, q_rows) > 227 * 1024) --slots;
+    return slots;
+}
 
-// The i-th set bit of a node set restricted to the nodes below n (-1: there are fewer).
+// The i-th set bit of a node set (-1: there are fewer).
 __device__ __forceinline__ int nth_node(const uint4& set, int i) {
     const uint32_t w[4] = {set.x, set.y, set.z, set.w};
 #pragma unroll
@@ -58,37 +94,108 @@ __device__ __forceinline__ uint4 counted_nodes(const uint32_t* rows, int b, int 
     return set;
 }
 
-__global__ void __launch_bounds__(kRowsThreads, 1) attention_mass_rows_kernel(const AttentionMassParams p, const __grid_constant__ CUtensorMap k_map) {
+__global__ void __launch_bounds__(kMassThreads, 1) attention_mass_kernel(const AttentionMassParams p, const __grid_constant__ CUtensorMap k_map) {
     using Cursor = DenseCursor<kMassTile, kMassMaxRows>;
     extern __shared__ unsigned char mass_smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(mass_smem_raw) + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t sbase = tc_smem_u32(smem), bars = sbase + kMassOffBar;
-    volatile int* s_abort = reinterpret_cast<volatile int*>(smem + kMassOffAbort);
+    const uint32_t off_q = kMassOffRing + (uint32_t)p.slots * kMassSlot, q_half = (uint32_t)p.q_rows * 128u;
+    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + kMassOffTmem);
+    volatile int* s_abort = reinterpret_cast<volatile int*>(smem + kMassOffTmem + 4);
     float* s_lse = reinterpret_cast<float*>(smem + kMassOffLse);
-    uint4* s_mask = reinterpret_cast<uint4*>(smem + kMassOffMask);
-    auto full = [&](uint32_t s) { return bars + 8u * s; };
-    auto empty = [&](uint32_t s) { return bars + 8u * (kMassStages + s); };
+    float* s_factor = reinterpret_cast<float*>(smem + kMassOffFactor);
+    uint4* s_vis = reinterpret_cast<uint4*>(smem + kMassOffVis);
+    float* s_part = reinterpret_cast<float*>(smem + kMassOffPart);
+    auto bar = [&](int i) { return bars + 8u * (uint32_t)i; };
     if (tid == 0) {
-        for (uint32_t s = 0; s < (uint32_t)kMassStages; ++s) {
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full(s)));
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(empty(s)), "r"(kRowsWarps));
-        }
+        auto init = [&](int first, int n, uint32_t count) {
+            for (int i = first; i < first + n; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar(i)), "r"(count));
+        };
+        init(kMassBarFull, kMassMaxSlots, 1);
+        init(kMassBarEmpty, kMassMaxSlots, 1);
+        init(kMassBarS, 2, 1);
+        init(kMassBarRead, 2, kMassWarps / 2);
+        init(kMassBarQ, 1, kMassWarps);
+        init(kMassBarFinal, 1, 1);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem_u32(s_tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *s_tmem;
     pdl_wait();
     pdl_launch_dependents();
 
-    Cursor cur(p.seqs, lane, blockIdx.x == 0 && warp == 0);
-    DenseSegment seg;
-    uint32_t it = 0;
-    if (warp == kRowsWarps) {
-        bool ok = true;
+    // every lane waits for itself; the warp then agrees, so that warp-wide instructions are never executed by a part of it
+    auto wait = [&](int b, uint32_t parity) {
+        const bool ok = tc_wait(bar(b), parity, s_abort, p.seqs.status);
+        return __all_sync(0xffffffffu, ok) != 0;
+    };
+    Cursor cur(p.seqs, lane, blockIdx.x == 0 && warp == 1);
+    DenseSegment seg = {};
+    bool ok = true;
+    // Units of which no node counts are left out, by all roles alike. Otherwise: rows, and passes of up to 256 columns.
+    auto rows_of_unit = [&](uint4& set) {
+        set = counted_nodes(p.rows, seg.b, seg.n);
+        return (__popc(set.x) + __popc(set.y) + __popc(set.z) + __popc(set.w)) * kGroup;
+    };
+    const uint32_t slots = (uint32_t)p.slots;
+
+    if (warp == 0) {
+        // ---- the issuer: pass by pass for two tiles, one of each group, in turn ----------------------------------------------
+        uint32_t use = 0, items[2] = {0, 0}, segs = 0;  // tiles of the ring; passes of a group
+        auto wait_mma = [&](int b, uint32_t parity) {
+            const bool done = wait(b, parity);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            return done;
+        };
         while (ok && cur.next(seg)) {
+            uint4 set;
+            const int rows = rows_of_unit(set);
+            if (rows == 0) continue;
+            const int passes = (rows + kMassCols - 1) / kMassCols, count = seg.tile1 - seg.tile0;
+            if (!(ok = wait_mma(kMassBarQ, segs & 1))) break;
+            ++segs;
+            for (int i = 0; i < count && ok; i += 2) {
+                for (int pass = 0; pass < passes && ok; ++pass) {
+                    const uint32_t cols = (uint32_t)min(kMassCols, (rows - pass * kMassCols + 15) & ~15);
+                    for (int g = 0; g < 2 && i + g < count && ok; ++g) {
+                        const uint32_t at = use + (uint32_t)g, slot = at % slots;
+                        if (pass == 0 && !(ok = wait_mma(kMassBarFull + (int)slot, (at / slots) & 1))) break;
+                        // (the group's scores of the pass before have been read)
+                        if (!(ok = wait_mma(kMassBarRead + g, (items[g] & 1) ^ 1))) break;
+                        ++items[g];
+                        const uint32_t k_lo = tc_desc_lo(sbase + kMassOffRing + slot * kMassSlot);
+                        const uint32_t q_lo = tc_desc_lo(sbase + off_q + (uint32_t)(pass * kMassCols) * 128u);
+#pragma unroll
+                        for (uint32_t ks = 0; ks < 8; ++ks)
+                            tc_mma_ss(tmem + (uint32_t)(g * kMassCols), tc_desc(k_lo + tc_koff(ks, kMassHalf)), tc_desc(q_lo + tc_koff(ks, q_half)), tc_idesc(cols),
+                                      ks == 0 ? 0u : 1u);
+                        tc_commit(bar(kMassBarS + g));
+                        if (pass == passes - 1) tc_commit(bar(kMassBarEmpty + (int)slot));
+                    }
+                }
+                use += (uint32_t)min(2, count - i);
+            }
+        }
+        tc_commit(bar(kMassBarFinal));
+        for (int spin = 0; spin < (1 << 22) && __all_sync(0xffffffffu, tc_test(bar(kMassBarFinal), 0)) == 0; ++spin) {}
+    } else if (warp == 1) {
+        // ---- the loading warp: lane l holds the l-th page of a window of 32; one lane copies -----------------------------
+        uint32_t use = 0;
+        if (lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
+        while (ok && cur.next(seg)) {
+            uint4 set;
+            if (rows_of_unit(set) == 0) continue;
             int base = -64, page_l = 0;
-            for (int t = seg.tile0; t < seg.tile1 && ok; ++t, ++it) {
+            for (int t = seg.tile0; t < seg.tile1 && ok; ++t) {
                 const int pi = t / (kPage / kMassTile);
                 if (pi - base >= 32) {
                     base = pi;
@@ -96,96 +203,133 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attention_mass_rows_kernel(co
                 }
                 const int page = __shfl_sync(0xffffffffu, page_l, pi - base);
                 if (lane == 0) {
-                    const uint32_t s = it % kMassStages, dst = sbase + s * kMassStage;
-                    ok = tc_wait(empty(s), ((it / kMassStages) & 1) ^ 1, s_abort, p.seqs.status);
+                    const uint32_t slot = use % slots, dst = sbase + kMassOffRing + slot * kMassSlot, full = bar(kMassBarFull + (int)slot);
+                    const int y = (int)(((size_t)page * p.seqs.Hkv + seg.kvh) * kPage) + (t % (kPage / kMassTile)) * kMassTile;
+                    ok = tc_wait(bar(kMassBarEmpty + (int)slot), ((use / slots) & 1) ^ 1, s_abort, p.seqs.status);
                     if (ok) {
-                        const int y = (int)(((size_t)page * p.seqs.Hkv + seg.kvh) * kPage) + (t % (kPage / kMassTile)) * kMassTile;
-                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full(s)), "r"(kMassStage) : "memory");
-                        tc_tma_load(dst, &k_map, 0, y, full(s));
-                        tc_tma_load(dst + kRowsHalf, &k_map, 64, y, full(s));
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full), "r"(kMassSlot) : "memory");
+                        tc_tma_load(dst, &k_map, 0, y, full);
+                        tc_tma_load(dst + kMassHalf, &k_map, 64, y, full);
+                        ++use;
                     }
                 }
                 ok = __shfl_sync(0xffffffffu, ok, 0);
-                if (!ok) break;
             }
         }
+        // no copy is left in flight when the CTA ends (they have all landed unless the CTA gave up early)
         if (lane == 0)
-            for (uint32_t j = it > (uint32_t)kMassStages ? it - kMassStages : 0; j < it; ++j)
-                for (int spin = 0; spin < (1 << 22) && !tc_test(full(j % kMassStages), (j / kMassStages) & 1); ++spin) {}
-        return;
+            for (uint32_t j = use > slots ? use - slots : 0; j < use; ++j)
+                for (int spin = 0; spin < (1 << 22) && !tc_test(bar(kMassBarFull + (int)(j % slots)), (j / slots) & 1); ++spin) {}
+        __syncwarp();
+    } else if (warp >= kMassWarp0) {
+        // ---- weights -----------------------------------------------------------------------------------------------------
+        // A warp that gives up goes on through the units without waiting, so that the barriers among these warps are
+        // reached by all of them.
+        const int g = (warp - kMassWarp0) >> 3, part = ((warp - kMassWarp0) >> 2) & 1, quarter = warp & 3, r = quarter * 32 + lane;
+        const int t_all = tid - kMassWarp0 * 32;
+        const uint32_t t_s = tmem + ((uint32_t)quarter << 21) + (uint32_t)(g * kMassCols);
+        const f32x2 scale2 = pack2(p.scale_log2, p.scale_log2);
+        uint32_t items = 0;
+        while (cur.next(seg)) {
+            uint4 set;
+            const int rows = rows_of_unit(set);
+            if (rows == 0) continue;
+            const int passes = (rows + kMassCols - 1) / kMassCols, count = seg.tile1 - seg.tile0, padded = (rows + 15) & ~15, P = seg.S - seg.n;
+            // The counted query rows. (Every product of the unit before has been read: the barrier at the end of the loop.) A row
+            // that fills up the last 16 is a copy of the last one that counts for nothing.
+            for (int i = t_all; i < padded * 16; i += kMassWarps * 32) {
+                const int qr = i >> 4, c = i & 15, row = min(qr, rows - 1);
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.q + seg.b * p.q_batch + nth_node(set, row >> 2) * p.q_node +
+                                                                     (seg.kvh * kGroup + (row & 3)) * p.q_head) + c);
+                *reinterpret_cast<uint4*>(smem + off_q + (c >> 3) * q_half + tc_swizzled(qr, c & 7)) = v;
+            }
+            for (int i = t_all; i < padded; i += kMassWarps * 32) {
+                float l = -INFINITY, f = 0.0f;
+                if (i < rows) {
+                    const float lse = __ldg(p.lse + ((size_t)seg.b * p.seqs.T + nth_node(set, i >> 2)) * ((size_t)p.seqs.Hkv * kGroup) + seg.kvh * kGroup + (i & 3));
+                    if (lse != -INFINITY) {  // (a row that sees nothing counts for nothing)
+                        const double exact = (double)lse * p.lse_scale;
+                        l = -(float)exact;
+                        f = isfinite(l) ? exp2f((float)(-(double)l - exact)) : 1.0f;
+                    }
+                }
+                s_lse[i] = l;
+                s_factor[i] = f;
+            }
+            if (seg.tile1 * kMassTile > P && t_all < seg.n) {  // which counted nodes see draft t_all
+                uint32_t words[4] = {0, 0, 0, 0};
+#pragma unroll 1
+                for (int k = 0; k < rows / kGroup; ++k) words[k >> 5] |= dense_bit(dense_mask(p.seqs, seg.b, nth_node(set, k)), t_all) ? 1u << (k & 31) : 0u;
+                s_vis[t_all] = make_uint4(words[0], words[1], words[2], words[3]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            asm volatile("bar.sync 1, 512;" ::: "memory");  // (what a thread reads below others have written)
+            if (lane == 0) tc_arrive(bar(kMassBarQ));
+
+            float* mass = p.mass + ((size_t)seg.b * p.seqs.Hkv + seg.kvh) * ((size_t)p.seqs.max_pages * kPage);
+            for (int i = g; i < count; i += 2) {
+                const int j = (seg.tile0 + i) * kMassTile + r;
+                float old = 0.0f;
+                if (part == 0 && j < seg.S) old = __ldcg(mass + j);
+                const bool masked = (seg.tile0 + i + 1) * kMassTile > P;
+                uint4 vis = make_uint4(0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu);
+                if (masked && j >= P) vis = j < seg.S ? s_vis[j - P] : make_uint4(0, 0, 0, 0);
+                f32x2 s0 = pack2(0.0f, 0.0f), s1 = s0;
+                for (int pass = 0; pass < passes; ++pass, ++items) {
+                    if (ok) ok = wait(kMassBarS + g, items & 1);
+                    if (!ok) continue;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const int cols = min(kMassCols, padded - pass * kMassCols), half = ((cols >> 4) + 1) >> 1;  // pieces of 16 columns of part 0
+                    const int piece0 = part == 0 ? 0 : half, piece1 = part == 0 ? half : cols >> 4;
+                    uint32_t a[2][16];
+                    if (piece0 < piece1) tc_ld16_issue(t_s + 16u * (uint32_t)piece0, a[0]);
+                    auto piece = [&](int q, uint32_t (&v)[16], uint32_t (&ahead)[16]) {
+                        tc_ld16_wait(v);
+                        if (q + 1 < piece1) tc_ld16_issue(t_s + 16u * (uint32_t)(q + 1), ahead);
+                        const int col = pass * kMassCols + 16 * q;
+                        const float4* ls = reinterpret_cast<const float4*>(s_lse + col);
+                        const float4* fs = reinterpret_cast<const float4*>(s_factor + col);
+                        const int node = col >> 2;  // four nodes in 16 columns
+                        const uint32_t word = node < 64 ? (node < 32 ? vis.x : vis.y) : (node < 96 ? vis.z : vis.w);
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            const float4 l4 = ls[n], f4 = fs[n];
+                            float x0, x1, x2, x3;
+                            unpack2(fma2(pack2(__uint_as_float(v[4 * n]), __uint_as_float(v[4 * n + 1])), scale2, pack2(l4.x, l4.y)), x0, x1);
+                            unpack2(fma2(pack2(__uint_as_float(v[4 * n + 2]), __uint_as_float(v[4 * n + 3])), scale2, pack2(l4.z, l4.w)), x2, x3);
+                            float e0 = exp2_approx(x0), e1 = exp2_approx(x1), e2 = exp2_approx(x2), e3 = exp2_approx(x3);
+                            if (masked && ((word >> ((node + n) & 31)) & 1u) == 0) e0 = e1 = e2 = e3 = 0.0f;
+                            s0 = fma2(pack2(e0, e1), pack2(f4.x, f4.y), s0);
+                            s1 = fma2(pack2(e2, e3), pack2(f4.z, f4.w), s1);
+                        }
+                    };
+                    for (int q = piece0; q < piece1; q += 2) {
+                        piece(q, a[0], a[1]);
+                        if (q + 1 < piece1) piece(q + 1, a[1], a[0]);
+                    }
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) tc_arrive(bar(kMassBarRead + g));
+                }
+                float a0, a1, b0, b1;
+                unpack2(s0, a0, a1);
+                unpack2(s1, b0, b1);
+                const float sum = (a0 + a1) + (b0 + b1);
+                float* others = s_part + (2 * g + ((i >> 1) & 1)) * 128;  // (written again two tiles on, behind a barrier of the one between)
+                if (part == 1) others[r] = sum;
+                asm volatile("bar.sync %0, 64;" ::"r"(2 + 4 * g + quarter) : "memory");
+                if (part == 0 && ok && j < seg.S) mass[j] = old + (sum + others[r]);
+            }
+            asm volatile("bar.sync 1, 512;" ::: "memory");
+        }
     }
 
-    bool ok = true;
-    const uint32_t a_row = (uint32_t)(warp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7)), a_chunk = (uint32_t)(lane >> 4);
-    const uint32_t q_row = (uint32_t)(lane & 7), q_chunk = (uint32_t)(lane >> 3);
-    while (cur.next(seg)) {
-        const int P = seg.S - seg.n;
-        const uint4 set = counted_nodes(p.rows, seg.b, seg.n);
-        const int nodes = __popc(set.x) + __popc(set.y) + __popc(set.z) + __popc(set.w), rows = nodes * kGroup, row_tiles = (rows + 7) / 8;
-        // the counted query rows, 16 bytes per thread and step; a missing last row is a copy of the last one that counts for nothing
-        for (int i = tid; i < row_tiles * 8 * 16; i += kRowsWarps * 32) {
-            const int r = min(i >> 4, rows - 1), chunk = i & 15;
-            const int node = nth_node(set, r >> 2);
-            const uint4 w = __ldg(reinterpret_cast<const uint4*>(p.q + seg.b * p.q_batch + node * p.q_node + (seg.kvh * kGroup + (r & 3)) * p.q_head) + chunk);
-            *reinterpret_cast<uint4*>(smem + kMassOffQ + (chunk >> 3) * kMassQHalf + (uint32_t)(i >> 4) * 128u + (((uint32_t)(chunk & 7) ^ ((i >> 4) & 7u)) << 4)) = w;
-        }
-        for (int r = tid; r < row_tiles * 8; r += kRowsWarps * 32) {
-            float x = INFINITY;
-            if (r < rows) {
-                const int node = nth_node(set, r >> 2);
-                x = __ldg(p.lse + ((size_t)seg.b * p.seqs.T + node) * ((size_t)p.seqs.Hkv * kGroup) + seg.kvh * kGroup + (r & 3)) * 1.4426950408889634f;
-                if ((r & 3) == 0) s_mask[r >> 2] = dense_mask(p.seqs, seg.b, node);
-            }
-            s_lse[r] = x;
-        }
-        asm volatile("bar.sync 1, %0;" ::"n"(kRowsWarps * 32) : "memory");
-        float* mass = p.mass + ((size_t)seg.b * p.seqs.Hkv + seg.kvh) * ((size_t)p.seqs.max_pages * kPage);
-        for (int t = seg.tile0; t < seg.tile1; ++t, ++it) {
-            const uint32_t s = it % kMassStages, kb = sbase + s * kMassStage;
-            if (ok) ok = __all_sync(0xffffffffu, tc_wait(full(s), (it / kMassStages) & 1, s_abort, p.seqs.status)) != 0;
-            if (!ok) continue;
-            const int tok0 = t * kMassTile + warp * 16;
-            const int j0 = tok0 + (lane >> 2), j1 = j0 + 8;
-            uint32_t ka[8][4];
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks) ldmatrix4(kb + rows_at(a_row, 2 * ks + a_chunk), ka[ks]);
-            __syncwarp();
-            if (lane == 0) tc_arrive(empty(s));
-            const bool masked = tok0 + 16 > P;
-            float sum[2] = {0.0f, 0.0f};
-            for (int rt = 0; rt < row_tiles; ++rt) {
-                float c[4] = {};
-#pragma unroll
-                for (int k2 = 0; k2 < 4; ++k2) {
-                    uint32_t qf[4];
-                    const uint32_t chunk = 4 * k2 + q_chunk;
-                    ldmatrix4(sbase + kMassOffQ + (chunk >> 3) * kMassQHalf + (rt * 8 + q_row) * 128u + (((chunk & 7u) ^ q_row) << 4), qf);
-                    mma16816(c, ka[2 * k2], qf[0], qf[1]);
-                    mma16816(c, ka[2 * k2 + 1], qf[2], qf[3]);
-                }
-                const int r = rt * 8 + (lane & 3) * 2;
-                const float2 e = *reinterpret_cast<const float2*>(s_lse + r);
-                float w0 = exp2_approx(fmaf(c[0], p.scale_log2, -e.x)), w1 = exp2_approx(fmaf(c[1], p.scale_log2, -e.y));
-                float w2 = exp2_approx(fmaf(c[2], p.scale_log2, -e.x)), w3 = exp2_approx(fmaf(c[3], p.scale_log2, -e.y));
-                if (masked) {  // (a quad's two rows belong to one node)
-                    const uint4 words = s_mask[min(r >> 2, nodes - 1)];
-                    if (j0 >= seg.S || (j0 >= P && !dense_bit(words, j0 - P))) w0 = w1 = 0.0f;
-                    if (j1 >= seg.S || (j1 >= P && !dense_bit(words, j1 - P))) w2 = w3 = 0.0f;
-                }
-                sum[0] += w0 + w1;
-                sum[1] += w2 + w3;
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-                sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-            }
-            if ((lane & 3) == 0) {
-                if (j0 < seg.S) mass[j0] += sum[0];
-                if (j1 < seg.S) mass[j1] += sum[1];
-            }
-        }
-        asm volatile("bar.sync 1, %0;" ::"n"(kRowsWarps * 32) : "memory");
+    // ---- release tensor memory -----------------------------------------------------------------------------------------
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 0) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
 }
 

@@ -176,16 +176,21 @@ int ha_attention_mass(const ha_shape_t* shape, const ha_tree_t* tree, const void
     p.lse = lse;
     p.rows = rows;
     p.mass = mass;
-    p.scale_log2 = sm_scale * 1.4426950408889634f;
+    const double exact = (double)sm_scale * 1.4426950408889634074;
+    p.scale_log2 = (float)exact;
+    p.lse_scale = 1.4426950408889634074 * ((double)p.scale_log2 / exact) * (1.0 - kScoreCut);
+    p.q_rows = (tree->max_nodes * kGroup + 15) & ~15;
+    p.slots = mass_slots(p.q_rows);
+    const size_t smem = mass_smem_bytes(p.slots, p.q_rows);
     int sms = 0;
     CUtensorMap k_map;
     if (sm_count(sms) != HA_OK || !encode_row_map(&k_map, k_pages, (uint64_t)shape->num_pages * shape->num_kv_heads * kPage, kMassTile) ||
-        cudaFuncSetAttribute(attention_mass_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMassSmemBytes) != cudaSuccess)
+        cudaFuncSetAttribute(attention_mass_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return HA_ERR_LAUNCH;
     const long long tiles = (long long)shape->batch * shape->num_kv_heads * shape->max_pages * (kPage / kMassTile);
     const int ctas = (int)std::min<long long>(tiles, sms);
-    return launch_smem(attention_mass_rows_kernel, dim3(ctas), dim3(kRowsThreads), kMassSmemBytes, static_cast<cudaStream_t>(stream), 1, p, k_map) ==
-                   cudaSuccess ? HA_OK : HA_ERR_LAUNCH;
+    return launch_smem(attention_mass_kernel, dim3(ctas), dim3(kMassThreads), smem, static_cast<cudaStream_t>(stream), 1, p, k_map) == cudaSuccess
+               ? HA_OK : HA_ERR_LAUNCH;
 }
 
 int ha_tree_commit(const ha_shape_t* shape, const ha_tree_t* tree, const uint32_t* accepted, void* k_pages, void* v_pages, uint32_t* hash_pages,

@@ -75,6 +75,11 @@ __device__ __forceinline__ bool any_nonfinite(uint4 w) {
     return bad(w.x) || bad(w.y) || bad(w.z) || bad(w.w);
 }
 
+// Natural log-sum-exp of a row from its maximum (in powers of two, a score as the products gave it) and sum.
+__device__ __forceinline__ float natural_lse(float M, float sum) {
+    return sum == 0.0f ? -INFINITY : (fmaf(M, (float)kScoreCut, M) + log2f(sum)) * 0.6931471805599453f;
+}
+
 // The output row and log-sum-exp of (sequence, node, query head): 4 dimensions per lane.
 __device__ __forceinline__ void store_row(const TreeAttentionParams& p, int b, int node, int qh, int lane, float4 acc, float M, float L) {
     const size_t row = ((size_t)b * p.seqs.T + node) * ((size_t)p.seqs.Hkv * kGroup) + qh;
@@ -83,7 +88,7 @@ __device__ __forceinline__ void store_row(const TreeAttentionParams& p, int b, i
     w.x = tc_pack_bf16(acc.x * inv, acc.y * inv);
     w.y = tc_pack_bf16(acc.z * inv, acc.w * inv);
     reinterpret_cast<uint2*>(p.out + row * kHeadDim)[lane] = w;
-    if (lane == 0 && p.lse != nullptr) p.lse[row] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+    if (lane == 0 && p.lse != nullptr) p.lse[row] = natural_lse(M, L);
 }
 
 template <int MT>

@@ -465,7 +465,7 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
                 }
                 if (mine && (kWide ? half : group) == 0) {
                     if (!seg.whole()) p.part_ml[part] = make_float2(M, sum);
-                    else if (p.lse != nullptr) p.lse[out_row] = sum == 0.0f ? -INFINITY : (M + log2f(sum)) * 0.6931471805599453f;
+                    else if (p.lse != nullptr) p.lse[out_row] = natural_lse(M, sum);
                 }
             }
             // the queries and O make room for the next unit: every product of this one is complete, and what was read of the other
