@@ -81,10 +81,6 @@ __device__ __forceinline__ int nth_node(const uint4& set, int i) {
     }
     return -1;
 }
-__device__ __forceinline__ uint4 first_nodes(int n) {
-    auto word = [&](int k) { return n >= 32 * k + 32 ? 0xffffffffu : (n <= 32 * k ? 0u : (1u << (n - 32 * k)) - 1u); };
-    return make_uint4(word(0), word(1), word(2), word(3));
-}
 __device__ __forceinline__ uint4 counted_nodes(const uint32_t* rows, int b, int n) {
     uint4 set = first_nodes(n);
     if (rows != nullptr) {

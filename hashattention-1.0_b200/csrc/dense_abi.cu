@@ -78,8 +78,14 @@ int launch_tree(void (*kernel)(TreeAttentionParams, CUtensorMap, CUtensorMap), i
     const int ctas = (int)std::min<long long>(tiles, std::min(sms, kDenseMaxCtas));
     if (launch_smem(kernel, dim3(ctas), dim3(threads), smem_bytes, st, 1, p, k_map, v_map) != cudaSuccess) return HA_ERR_LAUNCH;
     const int rows_max = std::min(kRows, p.seqs.T * kGroup);
-    const dim3 grid(shape->num_kv_heads * groups, shape->batch, (rows_max + kTreeMergeWarps - 1) / kTreeMergeWarps);
-    return launch(tree_merge_kernel<kTile, kRows>, grid, dim3(kTreeMergeWarps * 32), st, 1, p, ctas) == cudaSuccess ? HA_OK : HA_ERR_LAUNCH;
+    cudaError_t e;
+    if constexpr (kRows <= 32) {
+        const dim3 grid(shape->num_kv_heads * groups, shape->batch, (rows_max + kTreeMergeWarps - 1) / kTreeMergeWarps);
+        e = launch(tree_merge_kernel<kTile, kRows>, grid, dim3(kTreeMergeWarps * 32), st, 1, p, ctas);
+    } else {
+        e = launch(tree_merge_tc_kernel<kRows>, dim3(shape->num_kv_heads * groups * 4, shape->batch, (rows_max + 31) / 32), dim3(kTaMergeThreads), st, 1, p, ctas);
+    }
+    return e == cudaSuccess ? HA_OK : HA_ERR_LAUNCH;
 }
 
 // Words of one bit per 64 kept rows, for the largest budget a sequence can exceed.

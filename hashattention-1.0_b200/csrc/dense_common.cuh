@@ -56,6 +56,17 @@ __device__ __forceinline__ bool dense_bit(const uint4& m, int j) {
     return (w >> (j & 31)) & 1u;
 }
 
+// The nodes below n as a set.
+__device__ __forceinline__ uint4 first_nodes(int n) {
+    auto word = [&](int k) { return n >= 32 * k + 32 ? 0xffffffffu : (n <= 32 * k ? 0u : (1u << (n - 32 * k)) - 1u); };
+    return make_uint4(word(0), word(1), word(2), word(3));
+}
+
+// a / b for a >= 0, b > 0: in 32 bits where they fit
+__device__ __forceinline__ long long dense_div(long long a, long long b) {
+    return (a | b) >> 32 == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 // The cut. A unit is a (sequence, kv-head, group of kRows query rows); its tokens are tiles of kTile. The tiles of all units,
 // in order, are cut into gridDim.x ranges of equal length: the CTAs finish together whatever the lengths of the sequences,
 // and a unit lies in at most a few CTAs. A range covers whole units but for its first and its last one, so a CTA
@@ -76,13 +87,15 @@ struct DenseCut {
             total += t;
             if (b < b_stop) front += t;
         }
+        total = warp_sum(total);
+        before = warp_sum(front);
+        quota = quota_of(total, ctas);
+    }
+    static __device__ __forceinline__ long long quota_of(long long total, int ctas) { return max(1ll, dense_div(total + ctas - 1, ctas)); }
+    static __device__ __forceinline__ long long warp_sum(long long v) {
 #pragma unroll
-        for (int i = 16; i > 0; i >>= 1) {
-            total += __shfl_xor_sync(0xffffffffu, total, i);
-            front += __shfl_xor_sync(0xffffffffu, front, i);
-        }
-        quota = max(1ll, (total + ctas - 1) / ctas);
-        before = front;
+        for (int i = 16; i > 0; i >>= 1) v += __shfl_xor_sync(0xffffffffu, v, i);
+        return v;
     }
 };
 
@@ -102,14 +115,25 @@ struct DenseCursor {
     bool first;
     long long left;
     __device__ DenseCursor(const DenseSeqs& d_, int lane, bool reporter) : d(d_), b(0), S(0), n(0), tiles(0), groups(0), unit(0), tile(0), first(true), left(0) {
-        long long quota, unused, before = 0, total = 0;
-        Cut::count(d, gridDim.x, lane, 0, quota, unused);
-        const long long at = quota * blockIdx.x;
-        bool found = false;
-        for (int b0 = 0; b0 < d.B; b0 += 32) {
-            int S_ = 0, n_ = 0;
-            long long t = 0;
-            if (b0 + lane < d.B) t = Cut::seq_tiles(d, b0 + lane, reporter, S_, n_);
+        // lane = sequence; the last 32 sequences stay in registers (all of them, as a rule)
+        int S_ = 0, n_ = 0;
+        long long t = 0, total = 0;
+        const int last = (d.B - 1) & ~31;
+        for (int b0 = 0; b0 <= last; b0 += 32) {
+            S_ = n_ = 0;
+            t = b0 + lane < d.B ? Cut::seq_tiles(d, b0 + lane, reporter, S_, n_) : 0;
+            total += t;
+        }
+        total = Cut::warp_sum(total);
+        const long long quota = Cut::quota_of(total, gridDim.x), at = quota * blockIdx.x;
+        if (at >= total) return;
+        left = min(quota, total - at);
+        long long before = 0;
+        for (int b0 = 0; b0 <= last; b0 += 32) {
+            if (last > 0) {
+                S_ = n_ = 0;
+                t = b0 + lane < d.B ? Cut::seq_tiles(d, b0 + lane, false, S_, n_) : 0;
+            }
             long long incl = t;
 #pragma unroll
             for (int i = 1; i < 32; i <<= 1) {
@@ -117,8 +141,7 @@ struct DenseCursor {
                 if (lane >= i) incl += u;
             }
             const uint32_t reached = __ballot_sync(0xffffffffu, before + incl > at);
-            if (reached != 0 && !found) {
-                found = true;
+            if (reached != 0) {
                 const int l = __ffs(reached) - 1;
                 const long long in = __shfl_sync(0xffffffffu, at - (before + incl - t), l);
                 b = b0 + l;
@@ -126,13 +149,12 @@ struct DenseCursor {
                 n = __shfl_sync(0xffffffffu, n_, l);
                 tiles = (S + kTile - 1) / kTile;
                 groups = Cut::groups(n);
-                unit = (int)(in / tiles);
+                unit = (int)dense_div(in, tiles);
                 tile = (int)(in - (long long)unit * tiles);
+                break;
             }
             before += __shfl_sync(0xffffffffu, incl, 31);
         }
-        total = before;
-        left = found ? min(quota, total - at) : 0;
     }
     __device__ bool next(DenseSegment& s) {
         if (left <= 0) return false;

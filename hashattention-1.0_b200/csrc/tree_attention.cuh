@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(kTreeMergeWarps * 32) tree_merge_kernel(const 
     if (row >= n * kGroup) return;
     const int tiles = (S + kTile - 1) / kTile;
     const long long start = before + (long long)(kvh * Cut::groups(n) + group) * tiles;
-    const int c0 = (int)(start / quota), c1 = (int)((start + tiles - 1) / quota);
+    const int c0 = (int)dense_div(start, quota), c1 = (int)dense_div(start + tiles - 1, quota);
     if (c0 == c1) return;  // one CTA had the whole unit
     auto at = [&](int c) { return (size_t)(2 * c + (c == c0 && c0 * quota != start ? 1 : 0)) * kRows + r; };
 
@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(kTreeMergeWarps * 32) tree_merge_kernel(const 
         for (int i = 16; i > 0; i >>= 1) part += __shfl_xor_sync(0xffffffffu, part, i);
         sum += part;
         const int count = min(32, c1 - cb + 1);
-#pragma unroll 4
+#pragma unroll 8
         for (int i = 0; i < count; ++i) {
             const float w = __shfl_sync(0xffffffffu, f, i);
             const float4 a = __ldcg(reinterpret_cast<const float4*>(p.part_acc + at(cb + i) * kHeadDim) + lane);

@@ -9,14 +9,17 @@
 //     at the end of the unit, each group of softmax warps reading a quarter of the columns of both.
 //   * up to 256 rows (kWide): stream w has rows 128 w .. 128 w + 127, and a tile of K and V serves both.
 //
-// Roles of the warps: 0 issues the products, 4 - 19 are the softmax warps (eight per stream: a thread has
-// 64 of a row's 128 columns, and the two halves of a row agree on its maximum, as bf16, through shared memory), 2 loads: K and
-// V tiles by TMA (two boxes of 64 elements x 128 tokens, 128-byte swizzle) into a ring of 32 KB slots, K and V of a tile in turn. Streams that take different tiles have a ring of three slots each, so that a barrier is waited for
-// in every phase by the one who uses it; those that share tiles share a ring of five.
+// Roles of the warps: 0 issues the products, 1 loads K and V tiles by TMA (two boxes of 64 elements x 128 tokens, 128-byte
+// swizzle) into a ring of 32 KB slots, K and V of a tile in turn, 4 - 19 are the softmax warps, eight per stream: a thread has 64 of
+// a row's 128 columns, and the two halves of a row agree on its maximum, as bf16, through shared memory. Streams that take
+// different tiles have a ring of three slots each, streams that share tiles a ring of five; a barrier is waited for in every
+// phase by the one who uses it.
 //
-// A stream's S takes the place of its last P: its product Q K^T is issued behind P V of the tile before, in the tensor core's
-// order, so S complete means O complete too, and the softmax warps may rescale O (which they do only when a row's maximum has
-// grown by more than 2^8) without another barrier.
+// One warp issues for both streams, P V of a tile and Q K^T of the stream's next one back to back: the streams then take turns at
+// the tensor core (two issuers leave them in step: both wait for their softmax at the same time). S takes the place of P, so S
+// complete means O complete too, and the softmax warps may rescale O (which they do only when a row's maximum has grown by more
+// than 2^8) without another barrier. P is announced in two parts of 64 tokens (32 of each half): the first one's product runs under
+// the exponentials of the second.
 //
 // The V rows behind a sequence's end, and V rows of drafts with an infinity or NaN in them, are zeroed in shared memory before
 // the product sees them; the latter are added at the end to the rows that see them, by scalar arithmetic.
@@ -29,8 +32,8 @@ namespace ha {
 constexpr int kTaTile = 128;                       // tokens per tile
 constexpr uint32_t kTaSlot = 2 * 128 * 128;        // K or V of a tile: 32 KB
 constexpr uint32_t kTaHalf = 128 * 128;            // 64 elements of 128 rows
-constexpr int kTaLoadWarp = 2;
-constexpr int kTaSoftWarp0 = 4;                    // (a warp group of its own for the others; warps 1 and 3 do nothing)
+constexpr int kTaLoadWarp = 1;
+constexpr int kTaSoftWarp0 = 4;                    // (warps 2 and 3 do nothing)
 constexpr int kTaSoftWarps = 16;
 constexpr int kTaThreads = (kTaSoftWarp0 + kTaSoftWarps) * 32;
 
@@ -45,8 +48,8 @@ struct TaLayout {
     static constexpr int kBarFull = 0;                     // [rings][slots] the loader's arrival and the bytes of two copies
     static constexpr int kBarEmpty = kBarFull + kRings * kSlots;  // [rings][slots] commit: the products have read the slot
     static constexpr int kBarS = kBarEmpty + kRings * kSlots;     // [2] commit: S complete (and every product in front)
-    static constexpr int kBarP = kBarS + 2;                // [2] 8 warps: P is written
-    static constexpr int kBarO = kBarP + 2;                // [2] commit: the unit's last product is complete
+    static constexpr int kBarP = kBarS + 2;                // [2][2 parts] 8 warps: P is written
+    static constexpr int kBarO = kBarP + 4;                // [2] commit: the unit's last product is complete
     static constexpr int kBarQ = kBarO + 2;                // 16 warps: the unit's queries are in place, the last unit's results read
     static constexpr int kBarFinal = kBarQ + 1;            // commit: every product of the CTA is complete
     static constexpr int kBars = kBarFinal + 1;
@@ -107,7 +110,7 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
         init(L::kBarFull, L::kRings * L::kSlots, 1);
         init(L::kBarEmpty, L::kRings * L::kSlots, 1);
         init(L::kBarS, 2, 1);
-        init(L::kBarP, 2, 8);
+        init(L::kBarP, 4, 8);
         init(L::kBarO, 2, 1);
         init(L::kBarQ, 1, kTaSoftWarps);
         init(L::kBarFinal, 1, 1);
@@ -128,17 +131,11 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
 
     // every lane waits for itself; the warp then agrees, so that warp-wide instructions are never executed by a part of it
     auto wait = [&](int b, uint32_t parity) {
-        const bool ok = tc_wait(bar(b), parity, s_abort, p.seqs.status);
+        const bool ok = tc_wait_soon(bar(b), parity, s_abort, p.seqs.status);
         return __all_sync(0xffffffffu, ok) != 0;
     };
     // tiles of the segment that stream w takes
     auto stream_tiles = [&](const DenseSegment& s, int w) { return kWide ? s.tile1 - s.tile0 : (s.tile1 - s.tile0 + 1 - w) / 2; };
-
-    // Registers: 640 threads start with 96 each. The four warps that issue and load keep 56, the 16 softmax warps
-    // go up to 104: 128 x 56 + 512 x 104 <= 640 x 96.
-    static_assert((kTaSoftWarp0 * 32) * 56 + (kTaSoftWarps * 32) * 104 <= kTaThreads * 96, "registers of one CTA");
-    if (warp < kTaSoftWarp0) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    else asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
 
     DenseSegment seg;
     bool ok = true;
@@ -147,18 +144,17 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
         // ---- the issuer: P V of a stream's tile and Q K^T of its next one back to back, the streams in turn ----------------
         Cursor cur(p.seqs, lane, false);
         const uint32_t t_0 = __shfl_sync(0xffffffffu, tmem, 0);
-        uint32_t use[2] = {0, 0}, tiles[2] = {0, 0}, segs = 0;  // ring slots and tiles so far
+        uint32_t use_0 = 0, use_1 = 0, tiles_0 = 0, tiles_1 = 0, segs = 0;  // ring slots and tiles so far
         auto wait_mma = [&](int b, uint32_t parity) {
             const bool done = wait(b, parity);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             return done;
         };
-        auto ring_at = [&](int w) { return (uint32_t)((kWide ? 0 : w * L::kSlots)) + use[kWide ? 0 : w] % L::kSlots; };
-        auto ring_parity = [&](int w) { return (use[kWide ? 0 : w] / L::kSlots) & 1; };
+        auto ring_at = [&](int w) { return kWide || w == 0 ? use_0 % L::kSlots : (uint32_t)L::kSlots + use_1 % L::kSlots; };
+        auto ring_parity = [&](int w) { return ((kWide || w == 0 ? use_0 : use_1) / L::kSlots) & 1; };
         // S = Q K^T of stream w with the tile at the front of its ring; streams that share the tile release it together
         auto qk = [&](int w) {
             const uint32_t at = ring_at(w);
-            if (!(kWide && w == 1) && !wait_mma(L::kBarFull + (int)at, ring_parity(w))) return false;
             const uint32_t q_lo = tc_desc_lo(sbase + L::kOffQ + (kWide ? (uint32_t)w * kTaSlot : 0u));
             const uint32_t k_lo = tc_desc_lo(sbase + L::kOffRing + at * kTaSlot);
 #pragma unroll
@@ -166,57 +162,75 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
                 tc_mma_ss(t_0 + 128u * (uint32_t)w, tc_desc(q_lo + tc_koff(ks, kTaHalf)), tc_desc(k_lo + tc_koff(ks, kTaHalf)), tc_idesc(128), ks == 0 ? 0u : 1u);
             tc_commit(bar(L::kBarS + w));
             if (!kWide || w == 1) tc_commit(bar(L::kBarEmpty + (int)at));
-            return true;
         };
+        // O += P V, the part of the first 32 tokens of both halves of the tile, then the rest
         auto pv = [&](int w, bool first) {
-            if (!wait_mma(L::kBarP + w, tiles[w] & 1)) return false;
-            ++tiles[w];
             const uint32_t at = ring_at(w);
-            if (!(kWide && w == 1) && !wait_mma(L::kBarFull + (int)at, ring_parity(w))) return false;
             const uint32_t v_lo = ta_v_desc_lo(sbase + L::kOffRing + at * kTaSlot), t_s = t_0 + 128u * (uint32_t)w, t_o = t_s + 256u;
+            const uint32_t parity = (w == 0 ? tiles_0++ : tiles_1++) & 1;
 #pragma unroll
-            for (uint32_t ks = 0; ks < 8; ++ks) {
-                const uint64_t vd = tc_desc(v_lo + ks * (2048u >> 4));
-                tc_mma_ts(t_o, t_s + 16 * ks, vd, ta_pv_idesc(), first && ks == 0 ? 0u : 1u);
-                tc_mma_ts(t_o, t_s + 16 * ks + 8, vd, ta_pv_idesc(), 1u);
+            for (uint32_t part = 0; part < 2; ++part) {
+                if (!wait_mma(L::kBarP + 2 * w + (int)part, parity)) return false;
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const uint32_t ks = 4 * (i >> 1) + 2 * part + (i & 1);
+                    const uint64_t vd = tc_desc(v_lo + ks * (2048u >> 4));
+                    tc_mma_ts(t_o, t_s + 16 * ks, vd, ta_pv_idesc(), first && ks == 0 ? 0u : 1u);
+                    tc_mma_ts(t_o, t_s + 16 * ks + 8, vd, ta_pv_idesc(), 1u);
+                }
             }
             if (!kWide || w == 1) tc_commit(bar(L::kBarEmpty + (int)at));
             return true;
         };
+        auto slot_ready = [&](int w) { return wait(L::kBarFull + (int)ring_at(w), ring_parity(w)); };
         while (ok && cur.next(seg)) {
             if (!(ok = wait_mma(L::kBarQ, segs & 1))) break;
             ++segs;
             const int count0 = stream_tiles(seg, 0), count1 = stream_tiles(seg, 1);  // count1 = count0 or one less
             // `use` of a ring: the K tile of the stream's next product, then its V tile. Streams that share a ring: K of tile i is
             // used by both, then V of tile i - 1 ... so the place in the ring is set by hand.
+            // V of a tile and K of the next one are waited for before P is: the tensor core then gets both products without a pause
             if constexpr (kWide) {
-                const uint32_t base = use[0];
-                ok = qk(0) && qk(1);
+                if (!(ok = slot_ready(0))) break;
+                qk(0);
+                qk(1);
+#pragma unroll 1
                 for (int i = 0; i < count0 && ok; ++i) {
-                    for (int w = 0; w < 2 && ok; ++w) {
-                        use[0] = base + 2 * i + 1;
+                    const uint32_t v_at = ++use_0;
+                    if (!(ok = slot_ready(0))) break;
+                    if (i + 1 < count0) {
+                        ++use_0;
+                        if (!(ok = slot_ready(0))) break;
+                    }
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        use_0 = v_at;
                         if (!(ok = pv(w, i == 0))) break;
-                        use[0] = base + 2 * i + 2;
-                        if (i + 1 < count0) ok = qk(w);
+                        use_0 = v_at + 1;
+                        if (i + 1 < count0) qk(w);
                     }
                 }
-                use[0] = base + 2 * count0;
             } else {
-                ok = qk(0);
-                ++use[0];
-                if (ok && count1 > 0) {
-                    ok = qk(1);
-                    ++use[1];
+                if (!(ok = slot_ready(0))) break;
+                qk(0);
+                if (count1 > 0) {
+                    if (!(ok = slot_ready(1))) break;
+                    qk(1);
                 }
+#pragma unroll 1
                 for (int i = 0; i < count0 && ok; ++i) {
-                    for (int w = 0; w < 2 && ok; ++w) {
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
                         const int count = w == 0 ? count0 : count1;
+                        uint32_t& use = w == 0 ? use_0 : use_1;
                         if (i >= count) break;
+                        ++use;
+                        if (!(ok = slot_ready(w))) break;
                         if (!(ok = pv(w, i == 0))) break;
-                        ++use[w];
+                        ++use;
                         if (i + 1 < count) {
-                            ok = qk(w);
-                            ++use[w];
+                            if (!(ok = slot_ready(w))) break;
+                            qk(w);
                         }
                     }
                 }
@@ -250,12 +264,6 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
             const bool idle = quarter * 32 >= rows_left;
             const int node = (row0 + r) >> 2;
             const bool mine = r < rows_left;
-            uint4 mask = make_uint4(0, 0, 0, 0);
-            if (mine && seg.tile1 * kTaTile > P) {
-                mask = dense_mask(p.seqs, seg.b, node);
-                const uint4 f = first_nodes(seg.n);
-                mask.x &= f.x; mask.y &= f.y; mask.z &= f.z; mask.w &= f.w;
-            }
             // queries: row-major pieces of 16 bytes, rows behind the last one zero
             {
                 constexpr int kThreads = kWide ? 256 : 512;
@@ -280,6 +288,12 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) tc_arrive(bar(L::kBarQ));
+            }
+            uint4 mask = make_uint4(0, 0, 0, 0);
+            if (mine && seg.tile1 * kTaTile > P) {
+                mask = dense_mask(p.seqs, seg.b, node);
+                const uint4 f = first_nodes(seg.n);
+                mask.x &= f.x; mask.y &= f.y; mask.z &= f.z; mask.w &= f.w;
             }
             const int count = stream_tiles(seg, w);
             float m = -INFINITY, l = 0.0f;
@@ -311,34 +325,40 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
                 }
                 if (idle) {
                     __syncwarp();
-                    if (ok && lane == 0) tc_arrive(bar(L::kBarP + w));
+                    if (ok && lane < 2) tc_arrive(bar(L::kBarP + 2 * w + lane));
                     continue;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                uint32_t s[4][16];
+                // The scores are read twice, for the maximum and for the weights: held in between they would cost 64 registers.
+                uint32_t sa[16], sb[16], sc[16], sd[16];
+                auto hide = [&](int q, uint32_t (&v)[16]) {
+                    const uint32_t vis = visible32(mask, tok0 + 64 * half + 16 * q, P, seg.S);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) tc_ld16_issue(t_s + 16 * q, s[q]);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) tc_ld16_wait(s[q]);
-                if (masked) {
-#pragma unroll
-                    for (int q = 0; q < 4; q += 2) {
-                        const uint32_t vis = visible32(mask, tok0 + 64 * half + 16 * q, P, seg.S);
-#pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            if (((vis >> k) & 1u) == 0) s[q + (k >> 4)][k & 15] = 0xff800000u;  // -inf
-                    }
-                }
+                    for (int k = 0; k < 16; ++k)
+                        if (((vis >> k) & 1u) == 0) v[k] = 0xff800000u;  // -inf
+                };
                 float x0 = -INFINITY, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
+                auto largest = [&](int q, uint32_t (&v)[16]) {
+                    tc_ld16_wait(v);
+                    if (masked) hide(q, v);
 #pragma unroll
                     for (int k = 0; k < 16; k += 4) {
-                        x0 = fmaxf(x0, __uint_as_float(s[q][k]));
-                        x1 = fmaxf(x1, __uint_as_float(s[q][k + 1]));
-                        x2 = fmaxf(x2, __uint_as_float(s[q][k + 2]));
-                        x3 = fmaxf(x3, __uint_as_float(s[q][k + 3]));
+                        x0 = fmaxf(x0, __uint_as_float(v[k]));
+                        x1 = fmaxf(x1, __uint_as_float(v[k + 1]));
+                        x2 = fmaxf(x2, __uint_as_float(v[k + 2]));
+                        x3 = fmaxf(x3, __uint_as_float(v[k + 3]));
                     }
+                };
+                tc_ld16_issue(t_s, sa);
+                tc_ld16_issue(t_s + 16u, sb);
+                tc_ld16_issue(t_s + 32u, sc);
+                tc_ld16_issue(t_s + 48u, sd);
+                largest(0, sa);
+                largest(1, sb);
+                tc_ld16_issue(t_s, sa);  // (the second reading)
+                largest(2, sc);
+                largest(3, sd);
+                tc_ld16_issue(t_s + 16u, sb);
                 // the maximum of the row, as both halves know it (a reference for the exponents: its rounding does not matter)
                 const __nv_bfloat16 mine_max = __float2bfloat16_rn(fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * p.scale_log2);
                 s_max[half * 128 + r] = mine_max;
@@ -366,13 +386,14 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
                 const float ref = m == -INFINITY ? 0.0f : m;
                 const f32x2 nref2 = pack2(-ref, -ref);
                 f32x2 la = pack2(0.0f, 0.0f), lb = pack2(0.0f, 0.0f);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
+                auto weigh = [&](int q, uint32_t (&v)[16]) {
+                    tc_ld16_wait(v);
+                    if (masked) hide(q, v);
                     uint32_t out[16];  // one k-step of the A operand: words 0 .. 7 the hi halves, 8 .. 15 the lo halves
 #pragma unroll
                     for (int pr = 0; pr < 8; ++pr) {
                         float t0, t1;
-                        unpack2(fma2(pack2(__uint_as_float(s[q][2 * pr]), __uint_as_float(s[q][2 * pr + 1])), scale2, nref2), t0, t1);
+                        unpack2(fma2(pack2(__uint_as_float(v[2 * pr]), __uint_as_float(v[2 * pr + 1])), scale2, nref2), t0, t1);
                         const float e0 = exp2_approx(t0), e1 = exp2_approx(t1);
                         if (pr & 1) lb = add2(lb, pack2(e0, e1));
                         else la = add2(la, pack2(e0, e1));
@@ -384,12 +405,18 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
                         out[pr] = hi;
                         out[pr + 8] = tc_pack_bf16(l0, l1);
                     }
-                    tc_st16(t_s + 16 * q, out);
+                    if (q < 2) tc_ld16_issue(t_s + 16u * (uint32_t)(q + 2), v);
+                    tc_st16(t_s + 16u * (uint32_t)q, out);
+                };
+#pragma unroll
+                for (int part = 0; part < 2; ++part) {
+                    weigh(2 * part, sa);
+                    weigh(2 * part + 1, sb);
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) tc_arrive(bar(L::kBarP + 2 * w + part));
                 }
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) tc_arrive(bar(L::kBarP + w));
                 float a0, a1, b0, b1;
                 unpack2(la, a0, a1);
                 unpack2(lb, b0, b1);
@@ -399,7 +426,7 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
             if (ok) ok = wait(L::kBarO + w, seg_o & 1);
             ++seg_o;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            // sums of the halves, and of the streams that share the rows
+            // maxima and sums of the streams that share the rows
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             asm volatile("bar.sync 1, 512;" ::: "memory");  // (all products have read the queries, whose place this is)
             s_ml[(2 * w + half) * 128 + r] = make_float2(m, l);
@@ -419,7 +446,7 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
             if (ok && !idle) {
                 const bool second = !kWide && stream_tiles(seg, 1) > 0;  // (otherwise that stream's columns hold something else)
                 const size_t out_row = ((size_t)seg.b * p.seqs.T + node) * ((size_t)p.seqs.Hkv * kGroup) + seg.kvh * kGroup + (r & 3);
-                const size_t part = (size_t)(2 * blockIdx.x + seg.slot) * L::kRows + (kWide ? 128 * w : 0) + r;
+                const int row_in = (kWide ? 128 * w : 0) + r;  // of the unit
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                 const uint32_t bad = s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3];
                 const int q0 = kWide ? 4 * half : 2 * group, q1 = q0 + (kWide ? 4 : 2);
@@ -458,13 +485,14 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
                         dst[0] = make_uint4(words[0], words[1], words[2], words[3]);
                         dst[1] = make_uint4(words[4], words[5], words[6], words[7]);
                     } else {
-                        float4* dst = reinterpret_cast<float4*>(p.part_acc + part * kHeadDim + 16 * q);
+                        // [slot][dimensions / 4][row]: a warp's rows side by side
+                        float4* dst = reinterpret_cast<float4*>(p.part_acc) + ((size_t)(2 * blockIdx.x + seg.slot) * (kHeadDim / 4) + 4 * q) * L::kRows + row_in;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) dst[k] = make_float4(acc[4 * k], acc[4 * k + 1], acc[4 * k + 2], acc[4 * k + 3]);
+                        for (int k = 0; k < 4; ++k) dst[(size_t)k * L::kRows] = make_float4(acc[4 * k], acc[4 * k + 1], acc[4 * k + 2], acc[4 * k + 3]);
                     }
                 }
                 if (mine && (kWide ? half : group) == 0) {
-                    if (!seg.whole()) p.part_ml[part] = make_float2(M, sum);
+                    if (!seg.whole()) p.part_ml[(size_t)(2 * blockIdx.x + seg.slot) * L::kRows + row_in] = make_float2(M, sum);
                     else if (p.lse != nullptr) p.lse[out_row] = natural_lse(M, sum);
                 }
             }
@@ -523,6 +551,58 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
+}
+
+// The partial results of the units that several CTAs share: a thread has one row and four dimensions of it, a warp 32 rows
+// side by side (as they lie in the workspace), a CTA 32 rows x 32 dimensions; grid (Hkv * groups of T x 4, B, rows / 32).
+constexpr int kTaMergeThreads = 256;
+template <int kRows>
+__global__ void __launch_bounds__(kTaMergeThreads) tree_merge_tc_kernel(const TreeAttentionParams p, int ctas) {
+    using Cut = DenseCut<kTaTile, kRows>;
+    __shared__ uint2 s_out[32][9];  // [row][8 x 4 dimensions] bf16 (a column of padding)
+    // The lengths are read before the wait: the attention kernel in front does not write them, and what did has completed.
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.y;
+    const int max_groups = Cut::groups(p.seqs.T), x = blockIdx.x >> 2, kvh = x / max_groups, group = x - kvh * max_groups;
+    const int d4 = (blockIdx.x & 3) * 8 + warp, row0 = blockIdx.z * 32;
+    int S, n;
+    dense_seq(p.seqs, b, false, S, n);
+    long long quota, before;
+    Cut::count(p.seqs, ctas, lane, b, quota, before);
+    pdl_wait();
+    pdl_launch_dependents();
+    const int rows = min(kRows, n * kGroup - group * kRows);  // of the unit
+    if (row0 >= rows) return;
+    const int tiles = (S + kTaTile - 1) / kTaTile;
+    const long long start = before + (long long)(kvh * Cut::groups(n) + group) * tiles;
+    const int c0 = (int)dense_div(start, quota), c1 = (int)dense_div(start + tiles - 1, quota);
+    if (c0 == c1) return;  // one CTA had the whole unit
+    const int r = min(row0 + lane, rows - 1), first_slot = 2 * c0 + (c0 * quota != start ? 1 : 0);
+    auto slot = [&](int c) { return (size_t)(c == c0 ? first_slot : 2 * c); };
+    float M = -INFINITY;
+#pragma unroll 8
+    for (int c = c0; c <= c1; ++c) M = fmaxf(M, __ldcg(&p.part_ml[slot(c) * kRows + r]).x);
+    const float ref = M == -INFINITY ? 0.0f : M;
+    const float4* part = reinterpret_cast<const float4*>(p.part_acc) + (size_t)d4 * kRows + r;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float sum = 0.0f;
+#pragma unroll 8
+    for (int c = c0; c <= c1; ++c) {
+        const float2 ml = __ldcg(&p.part_ml[slot(c) * kRows + r]);
+        const float4 a = __ldcg(part + slot(c) * (kHeadDim / 4) * kRows);
+        const float f = exp2_approx(ml.x - ref);
+        sum = fmaf(ml.y, f, sum);
+        acc.x = fmaf(a.x, f, acc.x); acc.y = fmaf(a.y, f, acc.y);
+        acc.z = fmaf(a.z, f, acc.z); acc.w = fmaf(a.w, f, acc.w);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    s_out[lane][warp] = make_uint2(tc_pack_bf16(acc.x * inv, acc.y * inv), tc_pack_bf16(acc.z * inv, acc.w * inv));
+    auto out_row = [&](int row) {
+        return ((size_t)b * p.seqs.T + (group * kRows + row) / kGroup) * ((size_t)p.seqs.Hkv * kGroup) + kvh * kGroup + (row & (kGroup - 1));
+    };
+    if (d4 == 0 && row0 + lane < rows && p.lse != nullptr) p.lse[out_row(row0 + lane)] = natural_lse(M, sum);
+    __syncthreads();
+    const int row = threadIdx.x >> 3, piece = threadIdx.x & 7;  // 64 bytes of a row: eight threads
+    if (row0 + row < rows) reinterpret_cast<uint2*>(p.out + out_row(row0 + row) * kHeadDim)[(blockIdx.x & 3) * 8 + piece] = s_out[row][piece];
 }
 
 }  // namespace ha
