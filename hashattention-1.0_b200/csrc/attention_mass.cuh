@@ -91,7 +91,7 @@ __device__ __forceinline__ uint4 counted_nodes(const uint32_t* rows, int b, int 
 }
 
 __global__ void __launch_bounds__(kMassThreads, 1) attention_mass_kernel(const AttentionMassParams p, const __grid_constant__ CUtensorMap k_map) {
-    using Cursor = DenseCursor<kMassTile, kMassMaxRows>;
+    using Cursor = DenseCursor<kMassTile, kMassMaxRows, 0>;
     extern __shared__ unsigned char mass_smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(mass_smem_raw) + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;

@@ -25,6 +25,12 @@ int check_tree(const ha_tree_t* t) {
     return t->max_nodes > kMaxNodes ? HA_ERR_UNSUPPORTED_DIM : HA_OK;
 }
 
+// The kernels count the tiles of 64 tokens of all sequences, heads and groups of 16 rows in 32 bits.
+int check_tiles(const ha_shape_t* s, const ha_tree_t* t) {
+    const double groups = (double)((t->max_nodes * kGroup + 15) / 16), tiles = (double)s->max_pages * (kPage / kRowsTile);
+    return tiles > kMaxTiles / kRowsTile || tiles * groups * s->batch * s->num_kv_heads > kMaxTiles ? HA_ERR_UNSUPPORTED_DIM : HA_OK;
+}
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 DenseSeqs seqs_of(const ha_shape_t* s, const ha_tree_t* t, const int32_t* page_table, const int32_t* seq_lens, int32_t* status) {
@@ -63,7 +69,7 @@ size_t tree_workspace(int max_nodes) {
 }
 
 // The attention kernel and the merge behind it.
-template <int kTile, int kRows>
+template <int kTile, int kRows, int kCross>
 int launch_tree(void (*kernel)(TreeAttentionParams, CUtensorMap, CUtensorMap), int threads, size_t smem_bytes, const ha_shape_t* shape,
                 const TreeAttentionParams& p, cudaStream_t st) {
     int sms = 0;
@@ -73,7 +79,7 @@ int launch_tree(void (*kernel)(TreeAttentionParams, CUtensorMap, CUtensorMap), i
     if (!encode_row_map(&k_map, p.k_pages, rows, kTile) || !encode_row_map(&v_map, p.v_pages, rows, kTile)) return HA_ERR_LAUNCH;
     // (a per-device function attribute: set at every call, so that a process driving several GPUs is served)
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes) != cudaSuccess) return HA_ERR_LAUNCH;
-    const int groups = DenseCut<kTile, kRows>::groups(p.seqs.T);
+    const int groups = DenseCut<kTile, kRows, kCross>::groups(p.seqs.T);
     const long long tiles = (long long)shape->batch * shape->num_kv_heads * groups * shape->max_pages * (kPage / kTile);
     const int ctas = (int)std::min<long long>(tiles, std::min(sms, kDenseMaxCtas));
     if (launch_smem(kernel, dim3(ctas), dim3(threads), smem_bytes, st, 1, p, k_map, v_map) != cudaSuccess) return HA_ERR_LAUNCH;
@@ -83,7 +89,7 @@ int launch_tree(void (*kernel)(TreeAttentionParams, CUtensorMap, CUtensorMap), i
         const dim3 grid(shape->num_kv_heads * groups, shape->batch, (rows_max + kTreeMergeWarps - 1) / kTreeMergeWarps);
         e = launch(tree_merge_kernel<kTile, kRows>, grid, dim3(kTreeMergeWarps * 32), st, 1, p, ctas);
     } else {
-        e = launch(tree_merge_tc_kernel<kRows>, dim3(shape->num_kv_heads * groups * 4, shape->batch, (rows_max + 31) / 32), dim3(kTaMergeThreads), st, 1, p, ctas);
+        e = launch(tree_merge_tc_kernel<kRows>, dim3(shape->num_kv_heads * groups * kTaMergeParts, shape->batch, (rows_max + 31) / 32), dim3(kTaMergeThreads), st, 1, p, ctas);
     }
     return e == cudaSuccess ? HA_OK : HA_ERR_LAUNCH;
 }
@@ -139,6 +145,7 @@ int ha_tree_attention(const ha_shape_t* shape, const ha_tree_t* tree, const void
                       void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
     int rc = check_shape(shape);
     if (rc == HA_OK) rc = check_tree(tree);
+    if (rc == HA_OK) rc = check_tiles(shape, tree);
     if (rc != HA_OK) return rc;
     if (q == nullptr || k_pages == nullptr || v_pages == nullptr || page_table == nullptr || seq_lens == nullptr || out == nullptr || status == nullptr ||
         !(sm_scale > 0.0f) || !std::isfinite(sm_scale) || !aligned16(q) || !aligned16(out) || !aligned16(k_pages) || !aligned16(v_pages) ||
@@ -159,9 +166,9 @@ int ha_tree_attention(const ha_shape_t* shape, const ha_tree_t* tree, const void
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     p.k_pages = static_cast<const __nv_bfloat16*>(k_pages);
     p.v_pages = static_cast<const __nv_bfloat16*>(v_pages);
-    if (rows == 16) return launch_tree<kRowsTile, 16>(tree_attention_rows_kernel<1>, kRowsThreads, RowsLayout<1>::kSmemBytes, shape, p, st);
-    if (rows == 128) return launch_tree<kTaTile, 128>(tree_attention_tc_kernel<false>, kTaThreads, TaLayout<false>::kSmemBytes, shape, p, st);
-    return launch_tree<kTaTile, 256>(tree_attention_tc_kernel<true>, kTaThreads, TaLayout<true>::kSmemBytes, shape, p, st);
+    if (rows == 16) return launch_tree<kRowsTile, 16, kRowsCross>(tree_attention_rows_kernel<1>, kRowsThreads, RowsLayout<1>::kSmemBytes, shape, p, st);
+    if (rows == 128) return launch_tree<kTaTile, 128, TaLayout<false>::kCross>(tree_attention_tc_kernel<false>, kTaThreads, TaLayout<false>::kSmemBytes, shape, p, st);
+    return launch_tree<kTaTile, 256, TaLayout<true>::kCross>(tree_attention_tc_kernel<true>, kTaThreads, TaLayout<true>::kSmemBytes, shape, p, st);
 }
 
 int ha_attention_mass(const ha_shape_t* shape, const ha_tree_t* tree, const void* q, const int64_t* q_strides, const float* lse, const uint32_t* rows,
@@ -169,6 +176,7 @@ int ha_attention_mass(const ha_shape_t* shape, const ha_tree_t* tree, const void
                       void* stream) {
     int rc = check_shape(shape);
     if (rc == HA_OK) rc = check_tree(tree);
+    if (rc == HA_OK) rc = check_tiles(shape, tree);
     if (rc != HA_OK) return rc;
     if (q == nullptr || lse == nullptr || k_pages == nullptr || page_table == nullptr || seq_lens == nullptr || mass == nullptr || status == nullptr ||
         !(sm_scale > 0.0f) || !std::isfinite(sm_scale) || !aligned16(q) || !aligned16(k_pages) || !aligned16(tree->tree_mask) || !aligned16(rows) ||

@@ -62,37 +62,57 @@ __device__ __forceinline__ uint4 first_nodes(int n) {
     return make_uint4(word(0), word(1), word(2), word(3));
 }
 
-// a / b for a >= 0, b > 0: in 32 bits where they fit
-__device__ __forceinline__ long long dense_div(long long a, long long b) {
-    return (a | b) >> 32 == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
-}
+// a / b for a >= 0, b > 0 (unsigned: fewer instructions)
+__device__ __forceinline__ int dense_div(int a, int b) { return (int)((uint32_t)a / (uint32_t)b); }
+constexpr int kMaxTiles = 1 << 30;  // of all units of a call together, which the entry points check: counts of tiles are 32 bits
 
 // The cut. A unit is a (sequence, kv-head, group of kRows query rows); its tokens are tiles of kTile. The tiles of all units,
-// in order, are cut into gridDim.x ranges of equal length: the CTAs finish together whatever the lengths of the sequences,
-// and a unit lies in at most a few CTAs. A range covers whole units but for its first and its last one, so a CTA
+// in order, are cut into gridDim.x ranges of equal length (the quota): the CTAs finish together whatever the lengths of the
+// sequences, and a unit lies in at most a few CTAs. A range covers whole units but for its first and its last one, so a CTA
 // leaves at most two partial results: number 0 of its first unit, number 1 of its last.
-template <int kTile, int kRows>
+// A range that crosses from one unit into another pays for the end of a unit twice, which costs as much as kCross tiles. So where
+// the next larger quotas up to kCross more let every unit begin a range of its own, the smallest of those is taken, and the units
+// are seen as padded to whole ranges (their span).
+template <int kTile, int kRows, int kCross>
 struct DenseCut {
     static __host__ __device__ __forceinline__ int groups(int n) { return (n * kGroup + kRows - 1) / kRows; }
-    static __device__ __forceinline__ long long seq_tiles(const DenseSeqs& d, int b, bool reporter, int& S, int& n) {
-        dense_seq(d, b, reporter, S, n);
-        return (long long)((S + kTile - 1) / kTile) * groups(n) * d.Hkv;
+    static __device__ __forceinline__ int tiles_of(int S) { return dense_div(S + kTile - 1, kTile); }
+    static __device__ __forceinline__ int span_of(int tiles, int quota, bool whole) {
+        return whole ? dense_div(tiles + quota - 1, quota) * quota : tiles;
     }
-    // Tiles per CTA and the tiles in front of sequence b_stop, by a whole warp.
-    static __device__ void count(const DenseSeqs& d, int ctas, int lane, int b_stop, long long& quota, long long& before) {
-        long long total = 0, front = 0;
+    // The quota for `total` tiles, by a whole warp; lane b has the units of sequence b and their tiles (if B <= 32).
+    static __device__ __forceinline__ int quota_of(const DenseSeqs& d, int total, int ctas, int lane, int units, int tiles, bool& whole) {
+        const int even = max(1, dense_div(total + ctas - 1, ctas));
+        whole = false;
+        if (kCross == 0 || d.B > 32 || d.B * d.Hkv > ctas) return even;
+        const int mine = even + lane;  // lane i tries a quota larger by i
+        int need = 0;
+        for (int b = 0; b < d.B; ++b) need += __shfl_sync(0xffffffffu, units, b) * dense_div(__shfl_sync(0xffffffffu, tiles, b) + mine - 1, mine);
+        const uint32_t fits = __ballot_sync(0xffffffffu, need <= ctas && lane <= kCross);
+        whole = fits != 0;
+        return whole ? even + __ffs(fits) - 1 : even;
+    }
+    // The quota, the (padded) tiles in front of sequence b_stop and the span of its units, by a whole warp.
+    static __device__ void count(const DenseSeqs& d, int ctas, int lane, int b_stop, int& quota, int& before, int& span) {
+        int S, n, units = 0, tiles = 0, total = 0;
         for (int b = lane; b < d.B; b += 32) {
-            int S, n;
-            const long long t = seq_tiles(d, b, false, S, n);
-            total += t;
-            if (b < b_stop) front += t;
+            dense_seq(d, b, false, S, n);
+            tiles = tiles_of(S);
+            units = groups(n) * d.Hkv;
+            total += tiles * units;
         }
-        total = warp_sum(total);
-        before = warp_sum(front);
-        quota = quota_of(total, ctas);
+        bool whole;
+        quota = quota_of(d, warp_sum(total), ctas, lane, units, tiles, whole);
+        before = 0;
+        for (int b = lane; b < b_stop; b += 32) {
+            dense_seq(d, b, false, S, n);
+            before += span_of(tiles_of(S), quota, whole) * (groups(n) * d.Hkv);
+        }
+        before = warp_sum(before);
+        dense_seq(d, b_stop, false, S, n);
+        span = span_of(tiles_of(S), quota, whole);
     }
-    static __device__ __forceinline__ long long quota_of(long long total, int ctas) { return max(1ll, dense_div(total + ctas - 1, ctas)); }
-    static __device__ __forceinline__ long long warp_sum(long long v) {
+    static __device__ __forceinline__ int warp_sum(int v) {
 #pragma unroll
         for (int i = 16; i > 0; i >>= 1) v += __shfl_xor_sync(0xffffffffu, v, i);
         return v;
@@ -107,50 +127,54 @@ struct DenseSegment {
 };
 
 // Walks over the segments of a CTA's range. Built and advanced by a whole warp, all lanes alike.
-template <int kTile, int kRows>
+template <int kTile, int kRows, int kCross>
 struct DenseCursor {
-    using Cut = DenseCut<kTile, kRows>;
+    using Cut = DenseCut<kTile, kRows, kCross>;
     const DenseSeqs& d;
     int b, S, n, tiles, groups, unit, tile;
     bool first;
-    long long left;
+    int left;
     __device__ DenseCursor(const DenseSeqs& d_, int lane, bool reporter) : d(d_), b(0), S(0), n(0), tiles(0), groups(0), unit(0), tile(0), first(true), left(0) {
         // lane = sequence; the last 32 sequences stay in registers (all of them, as a rule)
         int S_ = 0, n_ = 0;
-        long long t = 0, total = 0;
+        int total = 0;
         const int last = (d.B - 1) & ~31;
+        auto units_of = [&] { return Cut::groups(n_) * d.Hkv; };
         for (int b0 = 0; b0 <= last; b0 += 32) {
             S_ = n_ = 0;
-            t = b0 + lane < d.B ? Cut::seq_tiles(d, b0 + lane, reporter, S_, n_) : 0;
-            total += t;
+            if (b0 + lane < d.B) dense_seq(d, b0 + lane, reporter, S_, n_);
+            total += Cut::tiles_of(S_) * units_of();
         }
         total = Cut::warp_sum(total);
-        const long long quota = Cut::quota_of(total, gridDim.x), at = quota * blockIdx.x;
-        if (at >= total) return;
-        left = min(quota, total - at);
-        long long before = 0;
+        bool whole;
+        const int quota = Cut::quota_of(d, total, gridDim.x, lane, units_of(), Cut::tiles_of(S_), whole), at = quota * blockIdx.x;
+        int before = 0;
         for (int b0 = 0; b0 <= last; b0 += 32) {
             if (last > 0) {
                 S_ = n_ = 0;
-                t = b0 + lane < d.B ? Cut::seq_tiles(d, b0 + lane, false, S_, n_) : 0;
+                if (b0 + lane < d.B) dense_seq(d, b0 + lane, false, S_, n_);
             }
-            long long incl = t;
+            const int t = Cut::span_of(Cut::tiles_of(S_), quota, whole) * units_of();
+            int incl = t;
 #pragma unroll
             for (int i = 1; i < 32; i <<= 1) {
-                const long long u = __shfl_up_sync(0xffffffffu, incl, i);
+                const int u = __shfl_up_sync(0xffffffffu, incl, i);
                 if (lane >= i) incl += u;
             }
             const uint32_t reached = __ballot_sync(0xffffffffu, before + incl > at);
             if (reached != 0) {
                 const int l = __ffs(reached) - 1;
-                const long long in = __shfl_sync(0xffffffffu, at - (before + incl - t), l);
+                const int in = __shfl_sync(0xffffffffu, at - (before + incl - t), l);
                 b = b0 + l;
                 S = __shfl_sync(0xffffffffu, S_, l);
                 n = __shfl_sync(0xffffffffu, n_, l);
-                tiles = (S + kTile - 1) / kTile;
+                tiles = Cut::tiles_of(S);
                 groups = Cut::groups(n);
-                unit = (int)dense_div(in, tiles);
-                tile = (int)(in - (long long)unit * tiles);
+                const int span = Cut::span_of(tiles, quota, whole);
+                unit = dense_div(in, span);
+                tile = in - unit * span;
+                // (the last range may be shorter, and so may the last one of a unit that is padded)
+                left = whole ? min(quota, (tiles - tile)) : min(quota, total - at);
                 break;
             }
             before += __shfl_sync(0xffffffffu, incl, 31);
@@ -166,7 +190,7 @@ struct DenseCursor {
                     ++b;  // (left > 0: there is one)
                     dense_seq(d, b, false, S, n);
                 } while (n == 0);
-                tiles = (S + kTile - 1) / kTile;
+                tiles = Cut::tiles_of(S);
                 groups = Cut::groups(n);
             }
         }
@@ -174,7 +198,7 @@ struct DenseCursor {
         s.kvh = unit / groups;
         s.group = unit - s.kvh * groups;
         s.tile0 = tile;
-        s.tile1 = (int)min((long long)tiles, tile + left);
+        s.tile1 = min(tiles, tile + left);
         s.slot = first ? 0 : 1;
         left -= s.tile1 - s.tile0;
         tile = s.tile1;
@@ -182,6 +206,19 @@ struct DenseCursor {
         return true;
     }
 };
+
+// Where the call's small arrays are read by every CTA behind the programmatic wait: their lines are asked into L2 in front of it
+// (a hint that reads nothing, so it does not matter whether the kernel in front still writes them). Whole CTA.
+__device__ __forceinline__ void dense_prefetch(const DenseSeqs& d) {
+    auto line = [](const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); };
+    const int at = threadIdx.x * 32;  // 128 bytes
+    if (at < d.B) {
+        line(d.seq_lens + at);
+        if (d.tree_lens != nullptr) line(d.tree_lens + at);
+    }
+    if (blockIdx.x == 0)
+        for (size_t i = at; i < (size_t)d.B * d.max_pages && i < (1u << 16); i += blockDim.x * 32) line(d.page_table + i);
+}
 
 // The matrix instructions (mma.sync and tcgen05 alike) cut their fp32 sums towards zero instead of rounding them. A score of 128
 // products in 8 steps comes out smaller by 1.0 to 1.25e-7 of itself on average (measured against 64 bits, with and without

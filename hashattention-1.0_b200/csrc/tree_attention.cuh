@@ -39,6 +39,7 @@ constexpr int kRowsWarps = 4;            // consumer warps, 16 tokens each
 constexpr int kRowsThreads = (kRowsWarps + 1) * 32;
 constexpr uint32_t kRowsHalf = kRowsTile * 128;      // 64 rows x 64 elements
 constexpr uint32_t kRowsStage = 4 * kRowsHalf;       // K and V of a tile: 32 KB
+constexpr int kRowsCross = 4;            // what a second unit in a CTA's range costs, in tiles (DenseCut)
 constexpr float kRescaleAt = 8.0f;       // a row's weights may grow to 2^8 before its sums are rescaled
 
 template <int MT>  // 16-row tiles of query rows
@@ -95,7 +96,7 @@ template <int MT>
 __global__ void __launch_bounds__(kRowsThreads, 1)
 tree_attention_rows_kernel(const TreeAttentionParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     using L = RowsLayout<MT>;
-    using Cursor = DenseCursor<kRowsTile, L::kRows>;
+    using Cursor = DenseCursor<kRowsTile, L::kRows, kRowsCross>;
     extern __shared__ unsigned char rows_smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(rows_smem_raw) + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -113,6 +114,7 @@ tree_attention_rows_kernel(const TreeAttentionParams p, const __grid_constant__ 
         asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
     }
+    dense_prefetch(p.seqs);
     __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
@@ -372,7 +374,7 @@ tree_attention_rows_kernel(const TreeAttentionParams p, const __grid_constant__ 
 constexpr int kTreeMergeWarps = 4;
 template <int kTile, int kRows>
 __global__ void __launch_bounds__(kTreeMergeWarps * 32) tree_merge_kernel(const TreeAttentionParams p, int ctas) {
-    using Cut = DenseCut<kTile, kRows>;
+    using Cut = DenseCut<kTile, kRows, kRowsCross>;
     // The lengths are read before the wait: the attention kernel in front does not write them, and what did has completed.
     const int lane = threadIdx.x & 31, r = blockIdx.z * kTreeMergeWarps + (threadIdx.x >> 5), b = blockIdx.y;
     const int max_groups = Cut::groups(p.seqs.T);
@@ -380,39 +382,43 @@ __global__ void __launch_bounds__(kTreeMergeWarps * 32) tree_merge_kernel(const 
     int S, n;
     dense_seq(p.seqs, b, false, S, n);
     const int row = group * kRows + r;
-    long long quota, before;
-    Cut::count(p.seqs, ctas, lane, b, quota, before);
+    int quota, before, span;
+    Cut::count(p.seqs, ctas, lane, b, quota, before, span);
+    const int tiles = Cut::tiles_of(S);
+    const int start = before + (kvh * Cut::groups(n) + group) * span;
+    const int c0 = dense_div(start, quota), c1 = dense_div(start + tiles - 1, quota);
+    auto at = [&](int c) { return (size_t)(2 * c + (c == c0 && c0 * quota != start ? 1 : 0)) * kRows + r; };
     pdl_wait();
     pdl_launch_dependents();
-    if (row >= n * kGroup) return;
-    const int tiles = (S + kTile - 1) / kTile;
-    const long long start = before + (long long)(kvh * Cut::groups(n) + group) * tiles;
-    const int c0 = (int)dense_div(start, quota), c1 = (int)dense_div(start + tiles - 1, quota);
-    if (c0 == c1) return;  // one CTA had the whole unit
-    auto at = [&](int c) { return (size_t)(2 * c + (c == c0 && c0 * quota != start ? 1 : 0)) * kRows + r; };
+    if (row >= n * kGroup || c0 == c1) return;  // (one CTA had the whole unit)
 
-    float M = -INFINITY;
-    for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, __ldcg(&p.part_ml[at(c)]).x);
-#pragma unroll
-    for (int i = 16; i > 0; i >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, i));
-    const float ref = M == -INFINITY ? 0.0f : M;
+    // 16 partial results at a time, all of their loads in flight together, in an order that is always the same
+    constexpr int kBatch = 16;
+    float M = -INFINITY, sum = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float sum = 0.0f;
-    for (int cb = c0; cb <= c1; cb += 32) {
-        float2 ml = make_float2(-INFINITY, 0.0f);
-        if (cb + lane <= c1) ml = __ldcg(&p.part_ml[at(cb + lane)]);
-        const float f = cb + lane <= c1 ? exp2_approx(ml.x - ref) : 0.0f;
-        float part = ml.y * f;  // (the sums of 32 partials in an order that is always the same)
+    for (int cb = c0; cb <= c1; cb += kBatch) {
+        const bool mine = lane < kBatch && cb + lane <= c1;
+        const float2 ml = mine ? __ldcg(&p.part_ml[at(cb + lane)]) : make_float2(-INFINITY, 0.0f);
+        float4 a[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            a[i] = cb + i <= c1 ? __ldcg(reinterpret_cast<const float4*>(p.part_acc + at(cb + i) * kHeadDim) + lane) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float top = fmaxf(M, ml.x);
+#pragma unroll
+        for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+        const float ref = top == -INFINITY ? 0.0f : top, f0 = exp2_approx(M - ref);
+        const float f = mine ? exp2_approx(ml.x - ref) : 0.0f;
+        float part = ml.y * f;
 #pragma unroll
         for (int i = 16; i > 0; i >>= 1) part += __shfl_xor_sync(0xffffffffu, part, i);
-        sum += part;
-        const int count = min(32, c1 - cb + 1);
-#pragma unroll 8
-        for (int i = 0; i < count; ++i) {
+        M = top;
+        sum = fmaf(sum, f0, part);
+        acc.x *= f0; acc.y *= f0; acc.z *= f0; acc.w *= f0;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
             const float w = __shfl_sync(0xffffffffu, f, i);
-            const float4 a = __ldcg(reinterpret_cast<const float4*>(p.part_acc + at(cb + i) * kHeadDim) + lane);
-            acc.x = fmaf(a.x, w, acc.x); acc.y = fmaf(a.y, w, acc.y);
-            acc.z = fmaf(a.z, w, acc.z); acc.w = fmaf(a.w, w, acc.w);
+            acc.x = fmaf(a[i].x, w, acc.x); acc.y = fmaf(a[i].y, w, acc.y);
+            acc.z = fmaf(a[i].z, w, acc.z); acc.w = fmaf(a[i].w, w, acc.w);
         }
     }
     store_row(p, b, row >> 2, kvh * kGroup + (row & 3), lane, acc, M, sum);

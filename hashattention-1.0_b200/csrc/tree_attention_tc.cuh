@@ -40,6 +40,7 @@ constexpr int kTaThreads = (kTaSoftWarp0 + kTaSoftWarps) * 32;
 template <bool kWide>
 struct TaLayout {
     static constexpr int kRows = kWide ? 256 : 128;
+    static constexpr int kCross = kWide ? 4 : 8;           // what a second unit in a CTA's range costs, in tiles (DenseCut)
     static constexpr int kRings = kWide ? 1 : 2;
     static constexpr int kSlots = kWide ? 5 : 3;           // per ring
     static constexpr uint32_t kOffQ = 0;                   // 128 rows x 128 each, K-major, 128-byte swizzle
@@ -93,7 +94,7 @@ template <bool kWide>
 __global__ void __launch_bounds__(kTaThreads, 1)
 tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     using L = TaLayout<kWide>;
-    using Cursor = DenseCursor<kTaTile, L::kRows>;
+    using Cursor = DenseCursor<kTaTile, L::kRows, L::kCross>;
     extern __shared__ unsigned char ta_smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ta_smem_raw) + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -103,6 +104,10 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
     uint32_t* s_bad = reinterpret_cast<uint32_t*>(smem + L::kOffBad);
     float2* s_ml = reinterpret_cast<float2*>(smem + L::kOffMl);
     auto bar = [&](int i) { return bars + 8u * (uint32_t)i; };
+    if (tid == 32 * kTaLoadWarp) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
+    }
     if (tid == 0) {
         auto init = [&](int first, int n, uint32_t count) {
             for (int i = first; i < first + n; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar(i)), "r"(count));
@@ -126,6 +131,7 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *s_tmem;
+    dense_prefetch(p.seqs);
     pdl_wait();
     pdl_launch_dependents();
 
@@ -137,12 +143,12 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
     // tiles of the segment that stream w takes
     auto stream_tiles = [&](const DenseSegment& s, int w) { return kWide ? s.tile1 - s.tile0 : (s.tile1 - s.tile0 + 1 - w) / 2; };
 
+    Cursor cur(p.seqs, lane, blockIdx.x == 0 && warp == kTaLoadWarp);  // (in front of the roles: the instructions come from memory once)
     DenseSegment seg;
     bool ok = true;
 
     if (warp == 0) {
         // ---- the issuer: P V of a stream's tile and Q K^T of its next one back to back, the streams in turn ----------------
-        Cursor cur(p.seqs, lane, false);
         const uint32_t t_0 = __shfl_sync(0xffffffffu, tmem, 0);
         uint32_t use_0 = 0, use_1 = 0, tiles_0 = 0, tiles_1 = 0, segs = 0;  // ring slots and tiles so far
         auto wait_mma = [&](int b, uint32_t parity) {
@@ -248,7 +254,6 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
         // ---- softmax warps -----------------------------------------------------------------------------------------------
         // A warp that gives up goes on through the units without waiting, so that the barriers among these warps are
         // reached by all of them.
-        Cursor cur(p.seqs, lane, false);
         const int group = (warp - kTaSoftWarp0) >> 2, w = group >> 1, half = group & 1;  // stream, half of the columns
         const int quarter = warp & 3, r = quarter * 32 + lane, ring = kWide ? 0 : w;      // quarter of the rows = tensor-memory lanes
         const int t_all = tid - kTaSoftWarp0 * 32, t_stream = t_all & 255;
@@ -329,18 +334,25 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
                     continue;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (masked) {  // tokens that the row does not see: taken out of S itself, so that the loops below are short
+#pragma unroll 1
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t v[16];
+                        tc_ld16_issue(t_s + 16u * (uint32_t)q, v);
+                        tc_ld16_wait(v);
+                        const uint32_t vis = visible32(mask, tok0 + 64 * half + 16 * q, P, seg.S);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            if (((vis >> k) & 1u) == 0) v[k] = 0xff800000u;  // -inf
+                        tc_st16(t_s + 16u * (uint32_t)q, v);
+                    }
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                }
                 // The scores are read twice, for the maximum and for the weights: held in between they would cost 64 registers.
                 uint32_t sa[16], sb[16], sc[16], sd[16];
-                auto hide = [&](int q, uint32_t (&v)[16]) {
-                    const uint32_t vis = visible32(mask, tok0 + 64 * half + 16 * q, P, seg.S);
-#pragma unroll
-                    for (int k = 0; k < 16; ++k)
-                        if (((vis >> k) & 1u) == 0) v[k] = 0xff800000u;  // -inf
-                };
                 float x0 = -INFINITY, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
-                auto largest = [&](int q, uint32_t (&v)[16]) {
+                auto largest = [&](uint32_t (&v)[16]) {
                     tc_ld16_wait(v);
-                    if (masked) hide(q, v);
 #pragma unroll
                     for (int k = 0; k < 16; k += 4) {
                         x0 = fmaxf(x0, __uint_as_float(v[k]));
@@ -353,11 +365,11 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
                 tc_ld16_issue(t_s + 16u, sb);
                 tc_ld16_issue(t_s + 32u, sc);
                 tc_ld16_issue(t_s + 48u, sd);
-                largest(0, sa);
-                largest(1, sb);
+                largest(sa);
+                largest(sb);
                 tc_ld16_issue(t_s, sa);  // (the second reading)
-                largest(2, sc);
-                largest(3, sd);
+                largest(sc);
+                largest(sd);
                 tc_ld16_issue(t_s + 16u, sb);
                 // the maximum of the row, as both halves know it (a reference for the exponents: its rounding does not matter)
                 const __nv_bfloat16 mine_max = __float2bfloat16_rn(fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * p.scale_log2);
@@ -388,7 +400,6 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
                 f32x2 la = pack2(0.0f, 0.0f), lb = pack2(0.0f, 0.0f);
                 auto weigh = [&](int q, uint32_t (&v)[16]) {
                     tc_ld16_wait(v);
-                    if (masked) hide(q, v);
                     uint32_t out[16];  // one k-step of the A operand: words 0 .. 7 the hi halves, 8 .. 15 the lo halves
 #pragma unroll
                     for (int pr = 0; pr < 8; ++pr) {
@@ -408,7 +419,7 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
                     if (q < 2) tc_ld16_issue(t_s + 16u * (uint32_t)(q + 2), v);
                     tc_st16(t_s + 16u * (uint32_t)q, out);
                 };
-#pragma unroll
+#pragma unroll 1  // (a short loop: at the first tile the instructions come from memory)
                 for (int part = 0; part < 2; ++part) {
                     weigh(2 * part, sa);
                     weigh(2 * part + 1, sb);
@@ -503,7 +514,6 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
         }
     } else if (warp == kTaLoadWarp) {
         // ---- the loading warp: lane l holds the l-th page of a window of 32; one lane copies -----------------------------
-        Cursor cur(p.seqs, lane, blockIdx.x == 0);
         uint32_t use[2] = {0, 0};
         auto copy = [&](int ring, const CUtensorMap* map, int y) {
             const uint32_t slot = use[ring] % L::kSlots, at = (uint32_t)(ring * L::kSlots) + slot, dst = sbase + L::kOffRing + at * kTaSlot;
@@ -515,10 +525,6 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
             ++use[ring];
             return true;
         };
-        if (lane == 0) {
-            asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
-            asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
-        }
         while (ok && cur.next(seg)) {
             int base = -64, page_l = 0;
             for (int t = seg.tile0; t < seg.tile1 && ok; ++t) {
@@ -553,56 +559,86 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
     }
 }
 
-// The partial results of the units that several CTAs share: a thread has one row and four dimensions of it, a warp 32 rows
-// side by side (as they lie in the workspace), a CTA 32 rows x 32 dimensions; grid (Hkv * groups of T x 4, B, rows / 32).
-constexpr int kTaMergeThreads = 256;
+// The partial results of the units that several CTAs share: a thread has one row and four dimensions of every second one of them,
+// a warp 32 rows side by side (as they lie in the workspace), a CTA 32 rows x 16 dimensions;
+// grid (Hkv * groups of T x 8, B, rows / 32).
+constexpr int kTaMergeThreads = 256, kTaMergeParts = 8, kTaMergeBatch = 12;
 template <int kRows>
 __global__ void __launch_bounds__(kTaMergeThreads) tree_merge_tc_kernel(const TreeAttentionParams p, int ctas) {
-    using Cut = DenseCut<kTaTile, kRows>;
-    __shared__ uint2 s_out[32][9];  // [row][8 x 4 dimensions] bf16 (a column of padding)
+    using Cut = DenseCut<kTaTile, kRows, TaLayout<(kRows > 128)>::kCross>;
+    __shared__ float4 s_acc[4][32];
+    __shared__ float2 s_ml[4][32];
+    __shared__ uint2 s_out[32][5];  // [row][4 x 4 dimensions] bf16 (a column of padding)
     // The lengths are read before the wait: the attention kernel in front does not write them, and what did has completed.
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.y;
-    const int max_groups = Cut::groups(p.seqs.T), x = blockIdx.x >> 2, kvh = x / max_groups, group = x - kvh * max_groups;
-    const int d4 = (blockIdx.x & 3) * 8 + warp, row0 = blockIdx.z * 32;
+    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) & 3, half = threadIdx.x >> 7, b = blockIdx.y;
+    const int max_groups = Cut::groups(p.seqs.T), x = blockIdx.x / kTaMergeParts, kvh = x / max_groups, group = x - kvh * max_groups;
+    const int d4 = (blockIdx.x % kTaMergeParts) * 4 + warp, row0 = blockIdx.z * 32;
     int S, n;
     dense_seq(p.seqs, b, false, S, n);
-    long long quota, before;
-    Cut::count(p.seqs, ctas, lane, b, quota, before);
+    int quota, before, span;
+    Cut::count(p.seqs, ctas, lane, b, quota, before, span);
+    const int rows = min(kRows, n * kGroup - group * kRows);  // of the unit
+    const int tiles = Cut::tiles_of(S), r = min(row0 + lane, rows - 1);
+    const int start = before + (kvh * Cut::groups(n) + group) * span;
+    const int c0 = dense_div(start, quota), c1 = dense_div(start + tiles - 1, quota), first_slot = 2 * c0 + (c0 * quota != start ? 1 : 0);
+    const float4* part = reinterpret_cast<const float4*>(p.part_acc) + (size_t)d4 * kRows + r;
     pdl_wait();
     pdl_launch_dependents();
-    const int rows = min(kRows, n * kGroup - group * kRows);  // of the unit
-    if (row0 >= rows) return;
-    const int tiles = (S + kTaTile - 1) / kTaTile;
-    const long long start = before + (long long)(kvh * Cut::groups(n) + group) * tiles;
-    const int c0 = (int)dense_div(start, quota), c1 = (int)dense_div(start + tiles - 1, quota);
-    if (c0 == c1) return;  // one CTA had the whole unit
-    const int r = min(row0 + lane, rows - 1), first_slot = 2 * c0 + (c0 * quota != start ? 1 : 0);
-    auto slot = [&](int c) { return (size_t)(c == c0 ? first_slot : 2 * c); };
-    float M = -INFINITY;
-#pragma unroll 8
-    for (int c = c0; c <= c1; ++c) M = fmaxf(M, __ldcg(&p.part_ml[slot(c) * kRows + r]).x);
-    const float ref = M == -INFINITY ? 0.0f : M;
-    const float4* part = reinterpret_cast<const float4*>(p.part_acc) + (size_t)d4 * kRows + r;
+    if (row0 >= rows || c0 == c1) return;  // (c0 == c1: one CTA had the whole unit)
+    float M = -INFINITY, sum = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float sum = 0.0f;
-#pragma unroll 8
-    for (int c = c0; c <= c1; ++c) {
-        const float2 ml = __ldcg(&p.part_ml[slot(c) * kRows + r]);
-        const float4 a = __ldcg(part + slot(c) * (kHeadDim / 4) * kRows);
+    auto rescale = [&](float top) {  // -> the reference of what is added next
+        const float ref = top == -INFINITY ? 0.0f : top, f = exp2_approx(M - ref);
+        M = top;
+        sum *= f;
+        acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+        return ref;
+    };
+    auto add = [&](float2 ml, float4 a, float ref) {
         const float f = exp2_approx(ml.x - ref);
         sum = fmaf(ml.y, f, sum);
         acc.x = fmaf(a.x, f, acc.x); acc.y = fmaf(a.y, f, acc.y);
         acc.z = fmaf(a.z, f, acc.z); acc.w = fmaf(a.w, f, acc.w);
+    };
+    for (int cb = c0 + half; cb <= c1; cb += 2 * kTaMergeBatch) {  // the loads of a batch in flight together
+        float2 ml[kTaMergeBatch];
+        float4 a[kTaMergeBatch];
+#pragma unroll
+        for (int k = 0; k < kTaMergeBatch; ++k) {
+            const int c = cb + 2 * k;
+            const size_t slot = (size_t)(c == c0 ? first_slot : 2 * c);
+            ml[k] = make_float2(-INFINITY, 0.0f);
+            a[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (c <= c1) {
+                ml[k] = __ldcg(&p.part_ml[slot * kRows + r]);
+                a[k] = __ldcg(part + slot * (kHeadDim / 4) * kRows);
+            }
+        }
+        float top = M;
+#pragma unroll
+        for (int k = 0; k < kTaMergeBatch; ++k) top = fmaxf(top, ml[k].x);
+        const float ref = rescale(top);
+#pragma unroll
+        for (int k = 0; k < kTaMergeBatch; ++k) add(ml[k], a[k], ref);
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    s_out[lane][warp] = make_uint2(tc_pack_bf16(acc.x * inv, acc.y * inv), tc_pack_bf16(acc.z * inv, acc.w * inv));
+    if (half == 1) {
+        s_acc[warp][lane] = acc;
+        s_ml[warp][lane] = make_float2(M, sum);
+    }
+    __syncthreads();
     auto out_row = [&](int row) {
         return ((size_t)b * p.seqs.T + (group * kRows + row) / kGroup) * ((size_t)p.seqs.Hkv * kGroup) + kvh * kGroup + (row & (kGroup - 1));
     };
-    if (d4 == 0 && row0 + lane < rows && p.lse != nullptr) p.lse[out_row(row0 + lane)] = natural_lse(M, sum);
+    if (half == 0) {
+        const float2 ml = s_ml[warp][lane];
+        add(ml, s_acc[warp][lane], rescale(fmaxf(M, ml.x)));
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        s_out[lane][warp] = make_uint2(tc_pack_bf16(acc.x * inv, acc.y * inv), tc_pack_bf16(acc.z * inv, acc.w * inv));
+        if (d4 == 0 && row0 + lane < rows && p.lse != nullptr) p.lse[out_row(row0 + lane)] = natural_lse(M, sum);
+    }
     __syncthreads();
-    const int row = threadIdx.x >> 3, piece = threadIdx.x & 7;  // 64 bytes of a row: eight threads
-    if (row0 + row < rows) reinterpret_cast<uint2*>(p.out + out_row(row0 + row) * kHeadDim)[(blockIdx.x & 3) * 8 + piece] = s_out[row][piece];
+    const int row = threadIdx.x >> 2, piece = threadIdx.x & 3;  // 32 bytes of a row: four threads
+    if (half == 0 && row0 + row < rows) reinterpret_cast<uint2*>(p.out + out_row(row0 + row) * kHeadDim)[d4 - warp + piece] = s_out[row][piece];
 }
 
 }  // namespace ha
