@@ -61,6 +61,26 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint
         "}\n" ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
 }
 
+// Eight products in a row, one thread elected for all of them (an election and what goes with it in front of each costs the
+// issuing warp 100 clocks more). Descriptors and tensor-memory addresses step inside the asm, so that they stay warp-uniform.
+// D = A . B^T over K = 128: A and B in shared memory, K-major, two blocks of 64 elements kBlock bytes apart.
+template <uint32_t kBlock>
+__device__ __forceinline__ void tc_mma_ss_k128(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q, r;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %3, %3;\n\tsetp.eq.b32 r, %3, %3;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "add.u64 a, %1, 2;\n\tadd.u64 b, %2, 2;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, r;\n\t"
+        "add.u64 a, %1, 4;\n\tadd.u64 b, %2, 4;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, r;\n\t"
+        "add.u64 a, %1, 6;\n\tadd.u64 b, %2, 6;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, r;\n\t"
+        "add.u64 a, %1, %4;\n\tadd.u64 b, %2, %4;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, r;\n\t"
+        "add.u64 a, %1, %4 + 2;\n\tadd.u64 b, %2, %4 + 2;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, r;\n\t"
+        "add.u64 a, %1, %4 + 4;\n\tadd.u64 b, %2, %4 + 4;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, r;\n\t"
+        "add.u64 a, %1, %4 + 6;\n\tadd.u64 b, %2, %4 + 6;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, r;\n\t"
+        "}\n" ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "n"(kBlock >> 4) : "memory");
+}
+
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
     asm volatile(
         "{\n\t"
@@ -114,6 +134,25 @@ __device__ __forceinline__ bool tc_wait_soon(uint32_t bar, uint32_t parity, vola
             : "=r"(done) : "r"(bar), "r"(parity) : "memory");
         if (done) return true;
         if (*abort_flag != 0) return false;
+    }
+    report(status, HA_ERR_TIMEOUT);
+    *abort_flag = 1;
+    return false;
+}
+
+// The same for two mbarriers, tested together, and a whole warp, whose lanes agree before they go on.
+__device__ __forceinline__ bool tc_wait_both(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1, volatile int* abort_flag, int32_t* status) {
+    for (int spin = 0; spin < (1 << 22); ++spin) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
+            "and.pred p, p, q;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done) : "r"(bar0), "r"(parity0), "r"(bar1), "r"(parity1) : "memory");
+        if (__all_sync(0xffffffffu, done != 0)) return true;
+        if (__any_sync(0xffffffffu, *abort_flag != 0)) return false;
     }
     report(status, HA_ERR_TIMEOUT);
     *abort_flag = 1;

@@ -10,7 +10,7 @@
 //   * up to 256 rows (kWide): stream w has rows 128 w .. 128 w + 127, and a tile of K and V serves both.
 //
 // Roles of the warps: 0 issues the products, 1 loads K and V tiles by TMA (two boxes of 64 elements x 128 tokens, 128-byte
-// swizzle) into a ring of 32 KB slots, K and V of a tile in turn, 4 - 19 are the softmax warps, eight per stream: a thread has 64 of
+// swizzle) into a ring of 32 KB slots, K and V of a tile in turn, 2 - 17 are the softmax warps, eight per stream: a thread has 64 of
 // a row's 128 columns, and the two halves of a row agree on its maximum, as bf16, through shared memory. Streams that take
 // different tiles have a ring of three slots each, streams that share tiles a ring of five; a barrier is waited for in every
 // phase by the one who uses it.
@@ -33,7 +33,7 @@ constexpr int kTaTile = 128;                       // tokens per tile
 constexpr uint32_t kTaSlot = 2 * 128 * 128;        // K or V of a tile: 32 KB
 constexpr uint32_t kTaHalf = 128 * 128;            // 64 elements of 128 rows
 constexpr int kTaLoadWarp = 1;
-constexpr int kTaSoftWarp0 = 4;                    // (warps 2 and 3 do nothing)
+constexpr int kTaSoftWarp0 = 2;
 constexpr int kTaSoftWarps = 16;
 constexpr int kTaThreads = (kTaSoftWarp0 + kTaSoftWarps) * 32;
 
@@ -65,6 +65,23 @@ struct TaLayout {
 // V as the B operand of O (128 x 128) += P (128 x 16) V (16 x 128): the 128 output columns run along the 128-byte rows
 // ("MN-major"), so blocks of 64 columns are kTaHalf apart and groups of 8 tokens 1024 bytes.
 __device__ __forceinline__ uint32_t ta_v_desc_lo(uint32_t saddr) { return ((saddr >> 4) & 0x3FFFu) | ((kTaHalf >> 4) << 16); }
+// O += P V over half of a tile's tokens: k-steps 0, 1, 4, 5 from the given addresses on, the hi and the lo half of P of each (as
+// tc_mma_ss_k128; `accumulate` is the first product's).
+__device__ __forceinline__ void ta_mma_pv(uint32_t tmem_d, uint32_t tmem_p, uint64_t desc_v, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q, r;\n\t.reg .b64 b;\n\t.reg .b32 a;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 r, %4, %4;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "add.u32 a, %1, 8;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], %2, %3, r;\n\t"
+        "add.u32 a, %1, 16;\n\tadd.u64 b, %2, 128;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, r;\n\t"
+        "add.u32 a, %1, 24;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, r;\n\t"
+        "add.u32 a, %1, 64;\n\tadd.u64 b, %2, 512;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, r;\n\t"
+        "add.u32 a, %1, 72;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, r;\n\t"
+        "add.u32 a, %1, 80;\n\tadd.u64 b, %2, 640;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, r;\n\t"
+        "add.u32 a, %1, 88;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, r;\n\t"
+        "}\n" ::"r"(tmem_d), "r"(tmem_p), "l"(desc_v), "r"(idesc), "r"(accumulate) : "memory");
+}
 __device__ __forceinline__ uint32_t ta_pv_idesc() { return tc_idesc(128) | (1u << 16); }
 
 __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -156,89 +173,48 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             return done;
         };
-        auto ring_at = [&](int w) { return kWide || w == 0 ? use_0 % L::kSlots : (uint32_t)L::kSlots + use_1 % L::kSlots; };
-        auto ring_parity = [&](int w) { return ((kWide || w == 0 ? use_0 : use_1) / L::kSlots) & 1; };
-        // S = Q K^T of stream w with the tile at the front of its ring; streams that share the tile release it together
-        auto qk = [&](int w) {
-            const uint32_t at = ring_at(w);
-            const uint32_t q_lo = tc_desc_lo(sbase + L::kOffQ + (kWide ? (uint32_t)w * kTaSlot : 0u));
-            const uint32_t k_lo = tc_desc_lo(sbase + L::kOffRing + at * kTaSlot);
-#pragma unroll
-            for (uint32_t ks = 0; ks < 8; ++ks)
-                tc_mma_ss(t_0 + 128u * (uint32_t)w, tc_desc(q_lo + tc_koff(ks, kTaHalf)), tc_desc(k_lo + tc_koff(ks, kTaHalf)), tc_idesc(128), ks == 0 ? 0u : 1u);
-            tc_commit(bar(L::kBarS + w));
-            if (!kWide || w == 1) tc_commit(bar(L::kBarEmpty + (int)at));
-        };
-        // O += P V, the part of the first 32 tokens of both halves of the tile, then the rest
-        auto pv = [&](int w, bool first) {
-            const uint32_t at = ring_at(w);
-            const uint32_t v_lo = ta_v_desc_lo(sbase + L::kOffRing + at * kTaSlot), t_s = t_0 + 128u * (uint32_t)w, t_o = t_s + 256u;
-            const uint32_t parity = (w == 0 ? tiles_0++ : tiles_1++) & 1;
-#pragma unroll
-            for (uint32_t part = 0; part < 2; ++part) {
-                if (!wait_mma(L::kBarP + 2 * w + (int)part, parity)) return false;
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    const uint32_t ks = 4 * (i >> 1) + 2 * part + (i & 1);
-                    const uint64_t vd = tc_desc(v_lo + ks * (2048u >> 4));
-                    tc_mma_ts(t_o, t_s + 16 * ks, vd, ta_pv_idesc(), first && ks == 0 ? 0u : 1u);
-                    tc_mma_ts(t_o, t_s + 16 * ks + 8, vd, ta_pv_idesc(), 1u);
-                }
-            }
-            if (!kWide || w == 1) tc_commit(bar(L::kBarEmpty + (int)at));
-            return true;
-        };
-        auto slot_ready = [&](int w) { return wait(L::kBarFull + (int)ring_at(w), ring_parity(w)); };
         while (ok && cur.next(seg)) {
             if (!(ok = wait_mma(L::kBarQ, segs & 1))) break;
             ++segs;
             const int count0 = stream_tiles(seg, 0), count1 = stream_tiles(seg, 1);  // count1 = count0 or one less
-            // `use` of a ring: the K tile of the stream's next product, then its V tile. Streams that share a ring: K of tile i is
-            // used by both, then V of tile i - 1 ... so the place in the ring is set by hand.
-            // V of a tile and K of the next one are waited for before P is: the tensor core then gets both products without a pause
-            if constexpr (kWide) {
-                if (!(ok = slot_ready(0))) break;
-                qk(0);
-                qk(1);
+            // Turn i of a stream: P V of its tile i - 1, then Q K^T of its tile i. A ring has K of a tile, V of it, K of the next ...; the
+            // streams that share one go through it alike, and the second one releases the slots. (One copy of the code for all turns:
+            // the first of them wait for instructions. Two waits a turn, two barriers each: a wait costs 300 clocks even
+            // where the barriers are complete, the products of a turn 1536, and four waits made this warp the bound.)
 #pragma unroll 1
-                for (int i = 0; i < count0 && ok; ++i) {
-                    const uint32_t v_at = ++use_0;
-                    if (!(ok = slot_ready(0))) break;
-                    if (i + 1 < count0) {
-                        ++use_0;
-                        if (!(ok = slot_ready(0))) break;
-                    }
-#pragma unroll
-                    for (int w = 0; w < 2; ++w) {
-                        use_0 = v_at;
-                        if (!(ok = pv(w, i == 0))) break;
-                        use_0 = v_at + 1;
-                        if (i + 1 < count0) qk(w);
-                    }
-                }
-            } else {
-                if (!(ok = slot_ready(0))) break;
-                qk(0);
-                if (count1 > 0) {
-                    if (!(ok = slot_ready(1))) break;
-                    qk(1);
-                }
-#pragma unroll 1
-                for (int i = 0; i < count0 && ok; ++i) {
-#pragma unroll
-                    for (int w = 0; w < 2; ++w) {
-                        const int count = w == 0 ? count0 : count1;
-                        uint32_t& use = w == 0 ? use_0 : use_1;
-                        if (i >= count) break;
-                        ++use;
-                        if (!(ok = slot_ready(w))) break;
-                        if (!(ok = pv(w, i == 0))) break;
-                        ++use;
-                        if (i + 1 < count) {
-                            if (!(ok = slot_ready(w))) break;
-                            qk(w);
-                        }
-                    }
+            for (int turn = 0; turn < 2 * (count0 + 1) && ok; ++turn) {
+                const int w = turn & 1, i = turn >> 1, count = w == 0 ? count0 : count1;
+                if (i > count || count == 0) continue;
+                uint32_t& use = w == 0 ? use_0 : use_1;
+                const uint32_t ring = kWide || w == 0 ? 0u : (uint32_t)L::kSlots, t_s = t_0 + 128u * (uint32_t)w, t_o = t_s + 256u;
+                const uint32_t v_use = use, k_use = i > 0 ? use + 1 : use;
+                const uint32_t v_at = ring + v_use % L::kSlots, k_at = ring + k_use % L::kSlots;
+                const int full_k = L::kBarFull + (int)k_at, full_v = L::kBarFull + (int)v_at;
+                const uint32_t full_k_parity = (k_use / L::kSlots) & 1, full_v_parity = (v_use / L::kSlots) & 1;
+                auto wait_both = [&](int b0, uint32_t parity0, int b1, uint32_t parity1) {
+                    const bool done = tc_wait_both(bar(b0), parity0, bar(b1), parity1, s_abort, p.seqs.status);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    return done;
+                };
+                if (i > 0) {  // O += P V: the first 32 tokens of both halves of the tile, then the rest
+                    const uint32_t parity = (w == 0 ? tiles_0 : tiles_1) & 1;
+                    const uint64_t vd = tc_desc(ta_v_desc_lo(sbase + L::kOffRing + v_at * kTaSlot));
+                    const int p0 = L::kBarP + 2 * w, p1 = p0 + 1;
+                    if (!(ok = wait_both(full_v, full_v_parity, p0, parity))) break;
+                    ta_mma_pv(t_o, t_s, vd, ta_pv_idesc(), i > 1 ? 1u : 0u);
+                    if (!(ok = i < count ? wait_both(full_k, full_k_parity, p1, parity) : wait_both(p1, parity, p1, parity))) break;
+                    ta_mma_pv(t_o, t_s + 32, vd + 256, ta_pv_idesc(), 1u);
+                    if (!kWide || w == 1) tc_commit(bar(L::kBarEmpty + (int)v_at));
+                    if (w == 0) ++tiles_0;
+                    else ++tiles_1;
+                    ++use;
+                } else if (!(ok = wait_both(full_k, full_k_parity, full_k, full_k_parity))) break;
+                if (i < count) {  // S = Q K^T
+                    tc_mma_ss_k128<kTaHalf>(t_s, tc_desc(tc_desc_lo(sbase + L::kOffQ + (kWide ? (uint32_t)w * kTaSlot : 0u))),
+                                            tc_desc(tc_desc_lo(sbase + L::kOffRing + k_at * kTaSlot)), tc_idesc(128));
+                    tc_commit(bar(L::kBarS + w));
+                    if (!kWide || w == 1) tc_commit(bar(L::kBarEmpty + (int)k_at));
+                    ++use;
                 }
             }
             // (for a unit without a tile for a stream too: its softmax warps then never run ahead of the issuer)
