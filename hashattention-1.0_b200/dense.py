@@ -144,9 +144,11 @@ def tree_accept(draft: torch.Tensor, parents: torch.Tensor, target: torch.Tensor
 class DenseDecodeContext:
     """Dense attention over one layer's paged cache for up to ``max_nodes`` new tokens per sequence (a tree of drafts; one
     token: the dense decode step), with its workspace. Creating it allocates; the calls do not, but for outputs that the
-    caller leaves out. One context per call that may run at the same time."""
+    caller leaves out. One context per call that may run at the same time; contexts whose calls follow one another on a stream
+    (the layers of a model) may share the workspaces of the first of them (``workspace_of``)."""
 
-    def __init__(self, cache: PagedHashKVCache, max_nodes: int = 1, sm_scale: float | None = None):
+    def __init__(self, cache: PagedHashKVCache, max_nodes: int = 1, sm_scale: float | None = None,
+                 workspace_of: "DenseDecodeContext | None" = None):
         if cache.device.type != "cuda":
             raise ValueError("the cache must live on a CUDA device")
         if not 1 <= max_nodes <= MAX_NODES:
@@ -162,11 +164,17 @@ class DenseDecodeContext:
             raise ValueError("sm_scale must be positive")
         self.shape = _lib.HaShape(self.batch, self.num_kv_heads, GROUP, HEAD_DIM, PAGE, cache.max_pages, cache.num_pages, 1)
         self.workspace_bytes = int(self.lib.ha_tree_workspace_bytes(self.max_nodes))
-        self.workspace = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=self.device)
         self.evict_workspace_bytes = int(self.lib.ha_evict_workspace_bytes(self.shape))
         if self.evict_workspace_bytes == 0:
             raise ValueError("invalid shape for the CUDA library")
-        self.evict_workspace = torch.empty(self.evict_workspace_bytes, dtype=torch.uint8, device=self.device)
+        if workspace_of is None:
+            self.workspace = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=self.device)
+            self.evict_workspace = torch.empty(self.evict_workspace_bytes, dtype=torch.uint8, device=self.device)
+        else:
+            o = workspace_of
+            if o.device != self.device or o.workspace_bytes < self.workspace_bytes or o.evict_workspace_bytes < self.evict_workspace_bytes:
+                raise ValueError("workspace_of must be a context on the same device with workspaces at least as large")
+            self.workspace, self.evict_workspace = o.workspace, o.evict_workspace
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
 
     @property

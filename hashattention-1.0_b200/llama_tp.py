@@ -12,7 +12,9 @@ output head are replicated. One process per GPU; the all-reduce is the NCCL coll
 Attention: the prompt is prefilled with dense causal attention (``scaled_dot_product_attention``, a
 library call), its keys / values go into this rank's paged cache and the key hashes are built once
 (``ha_hash_prefill``); every decode step is one ``ha_decode_step`` per layer on the rank's
-``Hkv / N`` kv-heads. A kv-head's keys, hash codes, hash MLPs and query heads live on one rank, so the
+``Hkv / N`` kv-heads. Trees of drafted tokens are verified with dense attention over the same cache, and a cache
+that has grown too long is cut by the attention weight its tokens received (:meth:`TPLlama.enable_trees`,
+:meth:`TPLlama.verify_tree`, :meth:`TPLlama.evict`). A kv-head's keys, hash codes, hash MLPs and query heads live on one rank, so the
 sparse-decode path itself needs no communication (SparseDecodeContext per layer).
 
 Weights are drawn per block of 1/8 of every sharded dimension from seeds that depend on (layer,
@@ -27,7 +29,8 @@ import torch
 import torch.distributed as dist
 import torch.nn.functional as F
 
-from .cache import PagedHashKVCache
+from .cache import PAGE, PagedHashKVCache
+from .dense import DenseDecodeContext, TreeAccept, tree_accept, tree_mask, unpack_nodes
 from .ops import Budget, SparseDecodeContext, rope_split
 from .synthetic import make_usa
 
@@ -134,6 +137,8 @@ class TPLlama:
         self.final_norm = torch.ones(cfg.dim, dtype=dtype, device=self.device)
         self.attention = attention
         self.pos = torch.zeros(batch, dtype=torch.int64, device=self.device)  # position of the next token per sequence
+        self.trees = None  # per layer, after enable_trees(): dense attention over the layer's cache
+        self.mass = None   # per layer: attention weight received by each cached token
         if attention == "cuda":
             budget = Budget(cfg.init_budget, cfg.heavy_budget, cfg.recent_budget)
             h0 = rank * self.hq
@@ -172,10 +177,15 @@ class TPLlama:
 
     # -- prefill: one sequence at a time, dense causal attention -----------------------------------
     @torch.no_grad()
-    def prefill(self, tokens: torch.Tensor) -> torch.Tensor:
-        """tokens [B, S] -> next-token ids [B] (greedy). Fills the caches and builds the key hashes."""
+    def prefill(self, tokens: torch.Tensor, observe: int = 0) -> torch.Tensor:
+        """tokens [B, S] -> next-token ids [B] (greedy). Fills the caches and builds the key hashes. ``observe``: the
+        received weights (``enable_trees(..., mass=True)``) start with those of the prompt's last ``observe`` tokens."""
         cfg = self.cfg
         B, S = tokens.shape
+        if observe:
+            if self.mass is None or not 1 <= observe <= min(S, self.trees[0].max_nodes):
+                raise ValueError(f"observe={observe} needs enable_trees(max_nodes >= observe, mass=True) and as many tokens")
+            seen = [torch.empty(B, observe, self.hq, cfg.head_dim, dtype=torch.bfloat16, device=self.device) for _ in self.layers]
         nxt = torch.empty(B, dtype=torch.int64, device=self.device)
         pos = torch.arange(S, device=self.device)
         for b in range(B):
@@ -188,6 +198,8 @@ class TPLlama:
                 att = F.scaled_dot_product_attention(qh[None], kh[None], vh[None], is_causal=True, enable_gqa=True)[0]
                 if self.attention == "cuda":
                     self.ctxs[i].cache.write_kv(b, kh, vh)  # (stored as bf16)
+                    if observe:
+                        seen[i][b] = q[S - observe:]
                 else:
                     if self.kv[i] is None:
                         self.kv[i] = (torch.zeros(B, self.hkv, S, cfg.head_dim, dtype=kh.dtype, device=self.device),
@@ -201,8 +213,103 @@ class TPLlama:
         if self.attention == "cuda":
             for ctx in self.ctxs:
                 ctx.hash_prefill()
+        if self.mass is not None:
+            for m in self.mass:
+                m.zero_()
+        if observe:
+            for i, tree in enumerate(self.trees):
+                tree.attention_mass(seen[i], tree.tree_attention(seen[i])[1], self.mass[i])
         self.pos.fill_(S)
         return nxt
+
+    # -- trees of drafted tokens, eviction -----------------------------------------------------------
+    def enable_trees(self, max_nodes: int, mass: bool = False) -> None:
+        """Prepares :meth:`verify_tree` for trees of up to ``max_nodes`` drafted tokens and, with ``mass``, keeps for every
+        layer the attention weight that each cached token has received (what :meth:`evict` goes by). Allocates; the
+        layers run one after another and share one workspace."""
+        if self.attention != "cuda":
+            raise ValueError("trees are verified on the paged cache: attention='cuda'")
+        self.trees = []
+        for ctx in self.ctxs:
+            self.trees.append(DenseDecodeContext(ctx.cache, max_nodes, workspace_of=self.trees[0] if self.trees else None))
+        self.mass = [t.new_mass() for t in self.trees] if mass else None
+
+    def _append_drafts(self, layer: int, k: torch.Tensor, v: torch.Tensor, first: torch.Tensor, tree_lens: torch.Tensor) -> None:
+        """k, v [B, T, Hkv, 128] -> the cache's tokens first[b] .. first[b] + tree_lens[b] - 1. Rows behind a tree's own repeat
+        its last one (in a sequence without drafts: put back the cache's last token)."""
+        cache = self.ctxs[layer].cache
+        n = tree_lens.long()[:, None]
+        row = torch.minimum(torch.arange(k.shape[1], device=self.device)[None], n - 1)      # [B, T]; -1: no drafts
+        token = (first.long()[:, None] + row).clamp(0, cache.max_pages * PAGE - 1)          # (lengths beyond that are reported)
+        page, slot = cache.page_table.long().gather(1, token // PAGE), token % PAGE
+        take = row.clamp_min(0)[..., None, None].expand(-1, -1, *k.shape[2:])
+        for pool, new in ((cache.k_pages, k), (cache.v_pages, v)):
+            new = torch.where((n > 0)[..., None, None], new.gather(1, take), pool[page, :, slot])
+            pool[page, :, slot] = new
+
+    def _tree_forward(self, draft, mask, tree_lens):
+        """Appends the drafts to every layer's cache (lengths and key hashes included) -> (logits [B, T, vocab], the layers'
+        queries and log-sum-exps, where the received weights are kept)."""
+        cfg = self.cfg
+        B, T = draft.shape
+        first = self.seq_lens.clone()
+        self.seq_lens += tree_lens
+        depth = unpack_nodes(mask).sum(-1) - 1                                     # ancestors of a node; -1 behind a tree
+        pos = (self.pos[:, None] + depth.clamp_min(0)).reshape(-1)
+        x = self.embed[torch.where(depth < 0, 0, draft).reshape(-1)]               # [B * T, dim]
+        kept = []
+        for i, layer in enumerate(self.layers):
+            h = rms_norm(x, layer.norm1, cfg.norm_eps)
+            q, k, v = rope_split(F.linear(h, layer.wqkv), pos, self.hq, self.hkv, cfg.rope_theta)
+            q = q.view(B, T, self.hq, cfg.head_dim)
+            self._append_drafts(i, k.view(B, T, self.hkv, -1), v.view(B, T, self.hkv, -1), first, tree_lens)
+            self.ctxs[i].hash_prefill(first)
+            att, lse = self.trees[i].tree_attention(q, mask, tree_lens)
+            if self.mass is not None:
+                kept.append((q, lse))
+            x = x + self.all_reduce(F.linear(att.view(B * T, -1), layer.wo))
+            x = x + self._mlp(layer, x)
+        return F.linear(rms_norm(x, self.final_norm, cfg.norm_eps), self.head).view(B, T, -1), kept
+
+    @torch.no_grad()
+    def verify_tree(self, draft: torch.Tensor, parents: torch.Tensor, tree_lens: torch.Tensor | None = None) -> TreeAccept:
+        """One round of speculative decoding: ``draft [B, T]`` int64 tokens of a tree per sequence (node 0: the token that is
+        certain, as the previous step returned it), ``parents [B, T]`` int32 (-1: a root), ``tree_lens [B]`` int32 where trees
+        are shorter than T. One pass with full attention over the cache, greedy acceptance, and the accepted path stays in the
+        cache: positions and lengths advance by ``count``, ``next_token`` is the next round's node 0 (or the next
+        :meth:`decode_step`'s token). With node 0 alone this is a dense decode step. Nothing synchronises with the host."""
+        if self.trees is None or draft.dim() != 2 or not 1 <= draft.shape[1] <= self.trees[0].max_nodes:
+            raise ValueError("verify_tree needs enable_trees(max_nodes) and a draft of [batch, 1 .. max_nodes] tokens")
+        if draft.shape[0] != self.batch:
+            raise ValueError(f"draft should have {self.batch} rows, but has {draft.shape[0]}")
+        status = self.trees[0].status
+        if tree_lens is None:
+            tree_lens = torch.full((self.batch,), draft.shape[1], dtype=torch.int32, device=self.device)
+        mask = tree_mask(parents, tree_lens, status=status)
+        logits, kept = self._tree_forward(draft, mask, tree_lens)
+        got = tree_accept(draft, parents, logits.float().argmax(-1), tree_lens, self.seq_lens, status=status)
+        for i, tree in enumerate(self.trees):
+            mass = None
+            if self.mass is not None:
+                mass = tree.attention_mass(*kept[i], self.mass[i], mask, tree_lens, rows=got.accepted)
+            tree.tree_commit(got.accepted, tree_lens, mass=mass)
+        self.seq_lens.copy_(got.seq_lens)
+        self.pos += got.count
+        return got
+
+    @torch.no_grad()
+    def evict(self, keep_tokens: int, init_budget: int | None = None, recent_budget: int | None = None) -> None:
+        """Cuts every sequence longer than ``keep_tokens`` to the tokens of each layer and kv-head that received the most
+        attention weight, beside the first ``init_budget`` and the last ``recent_budget`` (the decode step's, if left out).
+        Positions go on. Sparse decode steps add no weight: what they appended since the last tree is best covered by
+        ``recent_budget``."""
+        if self.mass is None:
+            raise ValueError("evict needs enable_trees(..., mass=True)")
+        init_budget = self.cfg.init_budget if init_budget is None else init_budget
+        recent_budget = self.cfg.recent_budget if recent_budget is None else recent_budget
+        for i, tree in enumerate(self.trees):
+            _, self.mass[i], lens = tree.cache_evict(self.mass[i], keep_tokens, init_budget, recent_budget)
+        self.seq_lens.copy_(lens)
 
     # -- one greedy decode step for the whole batch ------------------------------------------------
     @torch.no_grad()
@@ -236,7 +343,7 @@ class TPLlama:
 
     def check_status(self) -> None:
         if self.attention == "cuda":
-            for ctx in self.ctxs:
+            for ctx in self.ctxs + (self.trees or []):
                 ctx.check_status()
 
 
