@@ -29,7 +29,7 @@ import torch
 
 from . import _lib
 from .cache import GROUP, HEAD_DIM, PAGE, PagedHashKVCache
-from .ops import _call_range, _check, _raise_on, _stream_ptr, on_device
+from .ops import _check, _raise_on, _stream_ptr, library_call
 
 MAX_NODES = _lib.HA_MAX_TREE_NODES
 MASK_WORDS = MAX_NODES // 32
@@ -89,7 +89,7 @@ def tree_mask(parents: torch.Tensor, tree_lens: torch.Tensor | None = None, out:
     out = torch.empty(B, T, MASK_WORDS, dtype=torch.int32, device=dev) if out is None else out
     _check(out, "out", torch.int32, (B, T, MASK_WORDS), dev)
     status_ptr = _status_ptr(status, dev)
-    with on_device(dev), _call_range("ha_tree_mask"):
+    with library_call(dev, "ha_tree_mask"):
         rc = _lib.load().ha_tree_mask(parents.data_ptr(), tree_lens.data_ptr() if tree_lens is not None else None, B, T,
                                       out.data_ptr(), status_ptr, _stream_ptr(dev))
     _raise_on(rc, "ha_tree_mask")
@@ -132,7 +132,7 @@ def tree_accept(draft: torch.Tensor, parents: torch.Tensor, target: torch.Tensor
     _check(out.next_token, "next_token", torch.int64, (B,), dev)
     _check(out.seq_lens, "out.seq_lens", torch.int32, (B,), dev)
     status_ptr = _status_ptr(status, dev)
-    with on_device(dev), _call_range("ha_tree_accept"):
+    with library_call(dev, "ha_tree_accept"):
         rc = _lib.load().ha_tree_accept(draft.data_ptr(), parents.data_ptr(), target.data_ptr(),
                                         tree_lens.data_ptr() if tree_lens is not None else None, seq_lens.data_ptr(), B, T,
                                         out.accepted.data_ptr(), out.count.data_ptr(), out.next_token.data_ptr(),
@@ -163,6 +163,8 @@ class DenseDecodeContext:
         if not (self.sm_scale > 0.0 and math.isfinite(self.sm_scale)):
             raise ValueError("sm_scale must be positive")
         self.shape = _lib.HaShape(self.batch, self.num_kv_heads, GROUP, HEAD_DIM, PAGE, cache.max_pages, cache.num_pages, 1)
+        self._shape_ref = ctypes.byref(self.shape)
+        self._c_tree, self._c_strides = _lib.HaTree(), (ctypes.c_int64 * 3)()  # (filled in by each call)
         self.workspace_bytes = int(self.lib.ha_tree_workspace_bytes(self.max_nodes))
         self.evict_workspace_bytes = int(self.lib.ha_evict_workspace_bytes(self.shape))
         if self.evict_workspace_bytes == 0:
@@ -204,19 +206,23 @@ class DenseDecodeContext:
             raise ValueError(f"q must be torch.bfloat16, got {q.dtype}")
         if q.device != self.device:
             raise ValueError(f"q must live on {self.device}, got {q.device}")
-        strides = q.stride()
-        if strides[3] != 1 or any(s % 8 for s in strides[:3]) or q.data_ptr() % 16:
+        batch, node, head, one = q.stride()
+        if one != 1 or (batch | node | head) % 8 or q.data_ptr() % 16:
             raise ValueError("q's rows of 128 must be contiguous and start on 16-byte boundaries")
-        T = q.shape[1]
-        return T, self._tree_struct(T, tree_mask, tree_lens), (ctypes.c_int64 * 3)(*strides[:3])
+        T, strides = q.shape[1], self._c_strides
+        strides[0], strides[1], strides[2] = batch, node, head
+        return T, self._tree_struct(T, tree_mask, tree_lens), strides
 
     def _tree_struct(self, T, tree_mask, tree_lens):
+        tree = self._c_tree
+        tree.max_nodes, tree.tree_lens, tree.tree_mask = T, None, None
         if tree_mask is not None:
             _check(tree_mask, "tree_mask", torch.int32, (self.batch, T, MASK_WORDS), self.device)
+            tree.tree_mask = tree_mask.data_ptr()
         if tree_lens is not None:
             _check(tree_lens, "tree_lens", torch.int32, (self.batch,), self.device)
-        return _lib.HaTree(T, tree_lens.data_ptr() if tree_lens is not None else None,
-                           tree_mask.data_ptr() if tree_mask is not None else None)
+            tree.tree_lens = tree_lens.data_ptr()
+        return tree
 
     def _check_mass(self, mass, name="mass"):
         _check(mass, name, torch.float32, self.mass_shape, self.device)
@@ -236,9 +242,9 @@ class DenseDecodeContext:
         _check(out, "out", torch.bfloat16, (*size, HEAD_DIM), self.device)
         _check(lse, "lse", torch.float32, size, self.device)
         c = self.cache
-        with on_device(self.device), _call_range("ha_tree_attention"):
+        with library_call(self.device, "ha_tree_attention"):
             rc = self.lib.ha_tree_attention(
-                self.shape, tree, q.data_ptr(), strides, c.k_pages.data_ptr(), c.v_pages.data_ptr(), c.page_table.data_ptr(),
+                self._shape_ref, tree, q.data_ptr(), strides, c.k_pages.data_ptr(), c.v_pages.data_ptr(), c.page_table.data_ptr(),
                 c.seq_lens.data_ptr(), self.sm_scale, out.data_ptr(), lse.data_ptr(), self.workspace.data_ptr(),
                 self.workspace_bytes, self.status.data_ptr(), _stream_ptr(self.device))
         _raise_on(rc, "ha_tree_attention")
@@ -254,9 +260,9 @@ class DenseDecodeContext:
         if rows is not None:
             _check(rows, "rows", torch.int32, (self.batch, MASK_WORDS), self.device)
         c = self.cache
-        with on_device(self.device), _call_range("ha_attention_mass"):
+        with library_call(self.device, "ha_attention_mass"):
             rc = self.lib.ha_attention_mass(
-                self.shape, tree, q.data_ptr(), strides, lse.data_ptr(), rows.data_ptr() if rows is not None else None,
+                self._shape_ref, tree, q.data_ptr(), strides, lse.data_ptr(), rows.data_ptr() if rows is not None else None,
                 c.k_pages.data_ptr(), c.page_table.data_ptr(), c.seq_lens.data_ptr(), self.sm_scale, mass.data_ptr(),
                 self.status.data_ptr(), _stream_ptr(self.device))
         _raise_on(rc, "ha_attention_mass")
@@ -271,9 +277,9 @@ class DenseDecodeContext:
         if mass is not None:
             self._check_mass(mass)
         c = self.cache
-        with on_device(self.device), _call_range("ha_tree_commit"):
+        with library_call(self.device, "ha_tree_commit"):
             rc = self.lib.ha_tree_commit(
-                self.shape, tree, accepted.data_ptr(), c.k_pages.data_ptr(), c.v_pages.data_ptr(), c.hash_pages.data_ptr(),
+                self._shape_ref, tree, accepted.data_ptr(), c.k_pages.data_ptr(), c.v_pages.data_ptr(), c.hash_pages.data_ptr(),
                 c.page_table.data_ptr(), c.seq_lens.data_ptr(), mass.data_ptr() if mass is not None else None,
                 self.status.data_ptr(), _stream_ptr(self.device))
         _raise_on(rc, "ha_tree_commit")
@@ -300,9 +306,9 @@ class DenseDecodeContext:
         _check(lens_out, "lens_out", torch.int32, (self.batch,), self.device)
         if mass_out.data_ptr() == mass.data_ptr() or lens_out.data_ptr() == c.seq_lens.data_ptr():
             raise ValueError("mass_out and lens_out must be other tensors than mass and cache.seq_lens")
-        with on_device(self.device), _call_range("ha_cache_evict"):
+        with library_call(self.device, "ha_cache_evict"):
             rc = self.lib.ha_cache_evict(
-                self.shape, keep_tokens, init_budget, recent_budget, mass.data_ptr(), c.k_pages.data_ptr(), c.v_pages.data_ptr(),
+                self._shape_ref, keep_tokens, init_budget, recent_budget, mass.data_ptr(), c.k_pages.data_ptr(), c.v_pages.data_ptr(),
                 c.hash_pages.data_ptr(), c.page_table.data_ptr(), c.seq_lens.data_ptr(), kept.data_ptr(), mass_out.data_ptr(),
                 lens_out.data_ptr(), self.evict_workspace.data_ptr(), self.evict_workspace_bytes, self.status.data_ptr(),
                 _stream_ptr(self.device))

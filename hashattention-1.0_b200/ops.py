@@ -52,6 +52,8 @@ class Budget:
 
 
 def _check(t: torch.Tensor, name: str, dtype: torch.dtype, shape, device) -> None:
+    if type(t) is torch.Tensor and t.dtype is dtype and t.shape == shape and t.device == device and t.is_contiguous():
+        return
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a tensor")
     if t.dtype != dtype:
@@ -109,6 +111,27 @@ class _call_range:
         if self.pushed:
             torch.cuda.nvtx.range_pop()
         return False
+
+
+class _DeviceCallRange(_call_range):
+    def __init__(self, device, name: str):
+        super().__init__(name)
+        self.device = on_device(device)
+
+    def __enter__(self):
+        self.device.__enter__()
+        return super().__enter__()
+
+    def __exit__(self, *exc):
+        super().__exit__(*exc)
+        return self.device.__exit__(*exc)
+
+
+def library_call(device, name: str):
+    """``on_device(device)`` and ``_call_range(name)`` in one, or nothing where neither has anything to do."""
+    if not _nvtx_on and torch._C._cuda_getDevice() == device.index:
+        return _SAME_DEVICE
+    return _DeviceCallRange(device, name)
 
 
 class SparseDecodeContext:
