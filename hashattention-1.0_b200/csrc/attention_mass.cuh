@@ -5,21 +5,23 @@
 // per (sequence, kv-head), with the log-sum-exps the attention left: one more pass over K, no V. The transposed product
 // S = K Q^T runs on the 5th-generation tensor cores (tcgen05): the 128 tokens of a tile are the lanes of tensor memory, the counted
 // query rows its columns, so a thread adds up its token's weights without another one's help. The query rows (4 per counted node,
-// up to 512) stay in shared memory as the B operand, N = 16 to 256 columns at a time, so few rows cost few products.
+// up to 512) stay in shared memory as the B operand, N = 16 to 128 columns at a time, so few rows cost few products.
 //
 // Roles of the warps: 0 issues the products, 1 loads K tiles by TMA (two boxes of 64 elements x 128 tokens, 128-byte swizzle) into a
-// ring of 32 KB slots, 4 - 19 turn scores into weights, in two groups of eight that take every second tile (a buffer of 256 columns
-// of tensor memory each): four quarters of the lanes times two halves of the columns. The halves of a token's sum meet
-// in shared memory; no atomics, a token's sum is formed in a fixed order and stored by one thread, which has asked for the old
-// value before the scores arrive.
+// ring of 32 KB slots, 4 - 19 turn scores into weights, in two groups of eight that take every second tile (two buffers of 128 columns
+// of tensor memory each, so that the next products run under the exponentials; with one of 256 a group stood still for 1700 of 7500
+// clocks): four quarters of the lanes times two halves of the columns. The halves of a token's sum meet
+// in shared memory; a token's sum is formed in a fixed order and added by one thread in one piece (a reduction in L2: a load of the
+// old value cost 1300 clocks a tile).
 //
 // With few rows the bytes of K bound it; with 256 and more the exponentials do: 16 a clock on an SM, 2048 clocks for the
 // 128 x 256 scores whose K tile takes 1400 to arrive at the copy rate and whose products take 1024.
 //
 // Precision: c * s and lse are numbers of magnitude 10 to 50 whose difference is exponentiated. The multiply-add rounds only that
-// difference; what the rounding of c and of lse * log2(e) to fp32 would add (1e-6 of a weight) is taken out: lse is multiplied by
-// the fp32 value of c over its exact one, and by what the products leave of a score (kScoreCut), in 64 bits (where weights matter,
-// c s = lse), rounded to fp32, and what that leaves is a factor of the row, 2^(rest), applied in the multiply-add of the sum.
+// difference. What the rounding of c to fp32 would add, and what the products leave of a score (kScoreCut), is taken out of lse in
+// 64 bits (where weights matter, c s = lse); what is left is the rounding of lse * log2(e) to fp32, half an ulp of 16 to 64: up to
+// 1.3e-6 of a row's weights, to either side. (A factor per row that takes that out as well was read from shared memory for every
+// score: 4096 clocks for two tiles of 256 rows, as long as their exponentials take, on top of the same for lse.)
 #pragma once
 
 #include "tree_attention.cuh"
@@ -41,7 +43,7 @@ struct AttentionMassParams {
 
 constexpr int kMassTile = 128;
 constexpr int kMassMaxRows = kMaxNodes * kGroup;
-constexpr int kMassCols = 256;                  // columns of a buffer of tensor memory
+constexpr int kMassCols = 128;                  // columns of a buffer of tensor memory
 constexpr uint32_t kMassSlot = 2 * 128 * 128;   // K of a tile: 32 KB
 constexpr uint32_t kMassHalf = 128 * 128;
 constexpr int kMassMaxSlots = 6;
@@ -51,15 +53,16 @@ constexpr int kMassThreads = (kMassWarp0 + kMassWarps) * 32;
 // Shared memory: the fixed part, then the ring, then the queries (two halves of 64 elements, 128 bytes a row).
 constexpr int kMassBarFull = 0;                               // [slots] the loader's arrival and the bytes of two copies
 constexpr int kMassBarEmpty = kMassBarFull + kMassMaxSlots;   // [slots] commit: the products have read the tile
-constexpr int kMassBarS = kMassBarEmpty + kMassMaxSlots;      // [2 groups] commit: scores complete
-constexpr int kMassBarRead = kMassBarS + 2;                   // [2 groups] 8 warps: scores read
-constexpr int kMassBarQ = kMassBarRead + 2;                   // 16 warps: the unit's queries are in place
+constexpr int kMassBarS = kMassBarEmpty + kMassMaxSlots;      // [2 groups][2 buffers] commit: scores complete
+constexpr int kMassBarRead = kMassBarS + 4;                   // [2 groups][2 buffers] 8 warps: scores read
+constexpr int kMassBarQ = kMassBarRead + 4;                   // 16 warps: the unit's queries are in place
 constexpr int kMassBarFinal = kMassBarQ + 1;
 constexpr int kMassBars = kMassBarFinal + 1;
 constexpr uint32_t kMassOffLse = 0;                                    // [512] -lse in powers of two, rounded; -inf where there is no row
-constexpr uint32_t kMassOffFactor = kMassOffLse + kMassMaxRows * 4;    // [512] the factor of the row
-constexpr uint32_t kMassOffVis = kMassOffFactor + kMassMaxRows * 4;    // [128 drafts] counted nodes that see the draft, one bit each
-constexpr uint32_t kMassOffPart = kMassOffVis + kMaxNodes * 16;        // [2 groups][2 tiles][128] sums of the second half of the columns
+constexpr uint32_t kMassOffNode = kMassOffLse + kMassMaxRows * 4;      // [128] the counted nodes
+constexpr uint32_t kMassOffVis = kMassOffNode + kMaxNodes * 4;         // [128 drafts] counted nodes that see the draft, one bit each
+constexpr uint32_t kMassOffPart = kMassOffVis + kMaxNodes * 16;        // [2 groups][2 tiles][128] sums of the second half of the columns;
+                                                                       // in front of a unit's tiles: [128] mask words of the counted nodes
 constexpr uint32_t kMassOffBar = kMassOffPart + 2 * 2 * 128 * 4;
 constexpr uint32_t kMassOffTmem = kMassOffBar + kMassBars * 8;
 constexpr uint32_t kMassOffRing = (kMassOffTmem + 8 + 1023) / 1024 * 1024;
@@ -70,17 +73,6 @@ inline int mass_slots(int q_rows) {
     return slots;
 }
 
-// The i-th set bit of a node set (-1: there are fewer).
-__device__ __forceinline__ int nth_node(const uint4& set, int i) {
-    const uint32_t w[4] = {set.x, set.y, set.z, set.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int c = __popc(w[k]);
-        if (i < c) return 32 * k + (int)__fns(w[k], 0, i + 1);
-        i -= c;
-    }
-    return -1;
-}
 __device__ __forceinline__ uint4 counted_nodes(const uint32_t* rows, int b, int n) {
     uint4 set = first_nodes(n);
     if (rows != nullptr) {
@@ -100,7 +92,8 @@ __global__ void __launch_bounds__(kMassThreads, 1) attention_mass_kernel(const A
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + kMassOffTmem);
     volatile int* s_abort = reinterpret_cast<volatile int*>(smem + kMassOffTmem + 4);
     float* s_lse = reinterpret_cast<float*>(smem + kMassOffLse);
-    float* s_factor = reinterpret_cast<float*>(smem + kMassOffFactor);
+    int* s_node = reinterpret_cast<int*>(smem + kMassOffNode);
+    uint4* s_mask = reinterpret_cast<uint4*>(smem + kMassOffPart);
     uint4* s_vis = reinterpret_cast<uint4*>(smem + kMassOffVis);
     float* s_part = reinterpret_cast<float*>(smem + kMassOffPart);
     auto bar = [&](int i) { return bars + 8u * (uint32_t)i; };
@@ -110,8 +103,8 @@ __global__ void __launch_bounds__(kMassThreads, 1) attention_mass_kernel(const A
         };
         init(kMassBarFull, kMassMaxSlots, 1);
         init(kMassBarEmpty, kMassMaxSlots, 1);
-        init(kMassBarS, 2, 1);
-        init(kMassBarRead, 2, kMassWarps / 2);
+        init(kMassBarS, 4, 1);
+        init(kMassBarRead, 4, kMassWarps / 2);
         init(kMassBarQ, 1, kMassWarps);
         init(kMassBarFinal, 1, 1);
         *s_abort = 0;
@@ -126,18 +119,20 @@ __global__ void __launch_bounds__(kMassThreads, 1) attention_mass_kernel(const A
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *s_tmem;
+    dense_prefetch(p.seqs);
+    if (tid == 32) asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
     pdl_wait();
     pdl_launch_dependents();
 
     // every lane waits for itself; the warp then agrees, so that warp-wide instructions are never executed by a part of it
     auto wait = [&](int b, uint32_t parity) {
-        const bool ok = tc_wait(bar(b), parity, s_abort, p.seqs.status);
+        const bool ok = tc_wait_soon(bar(b), parity, s_abort, p.seqs.status);
         return __all_sync(0xffffffffu, ok) != 0;
     };
     Cursor cur(p.seqs, lane, blockIdx.x == 0 && warp == 1);
     DenseSegment seg = {};
     bool ok = true;
-    // Units of which no node counts are left out, by all roles alike. Otherwise: rows, and passes of up to 256 columns.
+    // Units of which no node counts are left out, by all roles alike. Otherwise: rows, and passes of up to 128 columns.
     auto rows_of_unit = [&](uint4& set) {
         set = counted_nodes(p.rows, seg.b, seg.n);
         return (__popc(set.x) + __popc(set.y) + __popc(set.z) + __popc(set.w)) * kGroup;
@@ -163,18 +158,19 @@ __global__ void __launch_bounds__(kMassThreads, 1) attention_mass_kernel(const A
                 for (int pass = 0; pass < passes && ok; ++pass) {
                     const uint32_t cols = (uint32_t)min(kMassCols, (rows - pass * kMassCols + 15) & ~15);
                     for (int g = 0; g < 2 && i + g < count && ok; ++g) {
-                        const uint32_t at = use + (uint32_t)g, slot = at % slots;
-                        if (pass == 0 && !(ok = wait_mma(kMassBarFull + (int)slot, (at / slots) & 1))) break;
-                        // (the group's scores of the pass before have been read)
-                        if (!(ok = wait_mma(kMassBarRead + g, (items[g] & 1) ^ 1))) break;
-                        ++items[g];
+                        const uint32_t at = use + (uint32_t)g, slot = at % slots, item = items[g]++, buffer = 2u * (uint32_t)g + (item & 1);
+                        // (the tile is there; the scores that the buffer held have been read)
+                        const int full = kMassBarFull + (int)slot, read = kMassBarRead + (int)buffer;
+                        ok = tc_wait_both(bar(full), (at / slots) & 1, bar(read), ((item >> 1) & 1) ^ 1, s_abort, p.seqs.status);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         const uint32_t k_lo = tc_desc_lo(sbase + kMassOffRing + slot * kMassSlot);
                         const uint32_t q_lo = tc_desc_lo(sbase + off_q + (uint32_t)(pass * kMassCols) * 128u);
 #pragma unroll
                         for (uint32_t ks = 0; ks < 8; ++ks)
-                            tc_mma_ss(tmem + (uint32_t)(g * kMassCols), tc_desc(k_lo + tc_koff(ks, kMassHalf)), tc_desc(q_lo + tc_koff(ks, q_half)), tc_idesc(cols),
+                            tc_mma_ss(tmem + buffer * kMassCols, tc_desc(k_lo + tc_koff(ks, kMassHalf)), tc_desc(q_lo + tc_koff(ks, q_half)), tc_idesc(cols),
                                       ks == 0 ? 0u : 1u);
-                        tc_commit(bar(kMassBarS + g));
+                        tc_commit(bar(kMassBarS + (int)buffer));
                         if (pass == passes - 1) tc_commit(bar(kMassBarEmpty + (int)slot));
                     }
                 }
@@ -186,12 +182,15 @@ __global__ void __launch_bounds__(kMassThreads, 1) attention_mass_kernel(const A
     } else if (warp == 1) {
         // ---- the loading warp: lane l holds the l-th page of a window of 32; one lane copies -----------------------------
         uint32_t use = 0;
-        if (lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
+        bool first = true;
         while (ok && cur.next(seg)) {
             uint4 set;
-            if (rows_of_unit(set) == 0) continue;
+            const int rows = rows_of_unit(set);
+            if (rows == 0) continue;
             int base = -64, page_l = 0;
             for (int t = seg.tile0; t < seg.tile1 && ok; ++t) {
+                // Many query rows (32 KB and more) come in behind the first two tiles only, not behind a full ring's.
+                if (first && rows >= 128 && t == seg.tile0 + 2 && !(ok = wait(kMassBarQ, 0))) break;
                 const int pi = t / (kPage / kMassTile);
                 if (pi - base >= 32) {
                     base = pi;
@@ -211,6 +210,7 @@ __global__ void __launch_bounds__(kMassThreads, 1) attention_mass_kernel(const A
                 }
                 ok = __shfl_sync(0xffffffffu, ok, 0);
             }
+            first = false;
         }
         // no copy is left in flight when the CTA ends (they have all landed unless the CTA gave up early)
         if (lane == 0)
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(kMassThreads, 1) attention_mass_kernel(const A
         // reached by all of them.
         const int g = (warp - kMassWarp0) >> 3, part = ((warp - kMassWarp0) >> 2) & 1, quarter = warp & 3, r = quarter * 32 + lane;
         const int t_all = tid - kMassWarp0 * 32;
-        const uint32_t t_s = tmem + ((uint32_t)quarter << 21) + (uint32_t)(g * kMassCols);
+        const uint32_t t_g = tmem + ((uint32_t)quarter << 21) + (uint32_t)(2 * g * kMassCols);
         const f32x2 scale2 = pack2(p.scale_log2, p.scale_log2);
         uint32_t items = 0;
         while (cur.next(seg)) {
@@ -231,32 +231,43 @@ __global__ void __launch_bounds__(kMassThreads, 1) attention_mass_kernel(const A
             const int rows = rows_of_unit(set);
             if (rows == 0) continue;
             const int passes = (rows + kMassCols - 1) / kMassCols, count = seg.tile1 - seg.tile0, padded = (rows + 15) & ~15, P = seg.S - seg.n;
+            if (t_all < kMaxNodes && dense_bit(set, t_all)) {  // the counted nodes in order: a node's place is the number of those below it
+                const uint4 below = first_nodes(t_all);
+                s_node[__popc(set.x & below.x) + __popc(set.y & below.y) + __popc(set.z & below.z) + __popc(set.w & below.w)] = t_all;
+            }
+            asm volatile("bar.sync 1, 512;" ::: "memory");
             // The counted query rows. (Every product of the unit before has been read: the barrier at the end of the loop.) A row
             // that fills up the last 16 is a copy of the last one that counts for nothing.
+#pragma unroll 4
             for (int i = t_all; i < padded * 16; i += kMassWarps * 32) {
                 const int qr = i >> 4, c = i & 15, row = min(qr, rows - 1);
-                const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.q + seg.b * p.q_batch + nth_node(set, row >> 2) * p.q_node +
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.q + seg.b * p.q_batch + s_node[row >> 2] * p.q_node +
                                                                      (seg.kvh * kGroup + (row & 3)) * p.q_head) + c);
                 *reinterpret_cast<uint4*>(smem + off_q + (c >> 3) * q_half + tc_swizzled(qr, c & 7)) = v;
             }
-            for (int i = t_all; i < padded; i += kMassWarps * 32) {
-                float l = -INFINITY, f = 0.0f;
-                if (i < rows) {
-                    const float lse = __ldg(p.lse + ((size_t)seg.b * p.seqs.T + nth_node(set, i >> 2)) * ((size_t)p.seqs.Hkv * kGroup) + seg.kvh * kGroup + (i & 3));
-                    if (lse != -INFINITY) {  // (a row that sees nothing counts for nothing)
-                        const double exact = (double)lse * p.lse_scale;
-                        l = -(float)exact;
-                        f = isfinite(l) ? exp2f((float)(-(double)l - exact)) : 1.0f;
-                    }
+            if (t_all < padded) {
+                float l = -INFINITY;  // (so too for a row that sees nothing)
+                if (t_all < rows) {
+                    const float lse = __ldg(p.lse + ((size_t)seg.b * p.seqs.T + s_node[t_all >> 2]) * ((size_t)p.seqs.Hkv * kGroup) + seg.kvh * kGroup + (t_all & 3));
+                    if (lse != -INFINITY) l = -(float)((double)lse * p.lse_scale);
                 }
-                s_lse[i] = l;
-                s_factor[i] = f;
+                s_lse[t_all] = l;
             }
-            if (seg.tile1 * kMassTile > P && t_all < seg.n) {  // which counted nodes see draft t_all
-                uint32_t words[4] = {0, 0, 0, 0};
-#pragma unroll 1
-                for (int k = 0; k < rows / kGroup; ++k) words[k >> 5] |= dense_bit(dense_mask(p.seqs, seg.b, nth_node(set, k)), t_all) ? 1u << (k & 31) : 0u;
-                s_vis[t_all] = make_uint4(words[0], words[1], words[2], words[3]);
+            if (seg.tile1 * kMassTile > P) {  // which counted nodes see draft t_all
+                const int nodes = rows / kGroup;
+                if (t_all < nodes) s_mask[t_all] = dense_mask(p.seqs, seg.b, s_node[t_all]);
+                asm volatile("bar.sync 1, 512;" ::: "memory");
+                if (t_all < seg.n) {
+                    const uint32_t* column = reinterpret_cast<const uint32_t*>(s_mask) + (t_all >> 5);
+                    uint32_t words[4];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        words[w] = 0;
+#pragma unroll 8
+                        for (int k = 32 * w; k < min(nodes, 32 * w + 32); ++k) words[w] |= ((column[4 * k] >> (t_all & 31)) & 1u) << (k & 31);
+                    }
+                    s_vis[t_all] = make_uint4(words[0], words[1], words[2], words[3]);
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             asm volatile("bar.sync 1, 512;" ::: "memory");  // (what a thread reads below others have written)
@@ -265,18 +276,33 @@ __global__ void __launch_bounds__(kMassThreads, 1) attention_mass_kernel(const A
             float* mass = p.mass + ((size_t)seg.b * p.seqs.Hkv + seg.kvh) * ((size_t)p.seqs.max_pages * kPage);
             for (int i = g; i < count; i += 2) {
                 const int j = (seg.tile0 + i) * kMassTile + r;
-                float old = 0.0f;
-                if (part == 0 && j < seg.S) old = __ldcg(mass + j);
                 const bool masked = (seg.tile0 + i + 1) * kMassTile > P;
                 uint4 vis = make_uint4(0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu);
                 if (masked && j >= P) vis = j < seg.S ? s_vis[j - P] : make_uint4(0, 0, 0, 0);
                 f32x2 s0 = pack2(0.0f, 0.0f), s1 = s0;
                 for (int pass = 0; pass < passes; ++pass, ++items) {
-                    if (ok) ok = wait(kMassBarS + g, items & 1);
+                    const int buffer = 2 * g + (int)(items & 1);
+                    const uint32_t t_s = t_g + (items & 1) * kMassCols;
+                    if (ok) ok = wait(kMassBarS + buffer, (items >> 1) & 1);
                     if (!ok) continue;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const int cols = min(kMassCols, padded - pass * kMassCols), half = ((cols >> 4) + 1) >> 1;  // pieces of 16 columns of part 0
                     const int piece0 = part == 0 ? 0 : half, piece1 = part == 0 ? half : cols >> 4;
+                    if (masked) {  // what does not count becomes -inf in tensor memory, so that the loop below has nothing to ask
+#pragma unroll 1
+                        for (int q = piece0; q < piece1; ++q) {
+                            uint32_t v[16];
+                            tc_ld16_issue(t_s + 16u * (uint32_t)q, v);
+                            tc_ld16_wait(v);
+                            const int node = (pass * kMassCols + 16 * q) >> 2;  // four nodes in 16 columns
+                            const uint32_t word = node < 64 ? (node < 32 ? vis.x : vis.y) : (node < 96 ? vis.z : vis.w);
+#pragma unroll
+                            for (int k = 0; k < 16; ++k)
+                                if (((word >> ((node + (k >> 2)) & 31)) & 1u) == 0) v[k] = 0xff800000u;
+                            tc_st16(t_s + 16u * (uint32_t)q, v);
+                        }
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    }
                     uint32_t a[2][16];
                     if (piece0 < piece1) tc_ld16_issue(t_s + 16u * (uint32_t)piece0, a[0]);
                     auto piece = [&](int q, uint32_t (&v)[16], uint32_t (&ahead)[16]) {
@@ -284,19 +310,14 @@ __global__ void __launch_bounds__(kMassThreads, 1) attention_mass_kernel(const A
                         if (q + 1 < piece1) tc_ld16_issue(t_s + 16u * (uint32_t)(q + 1), ahead);
                         const int col = pass * kMassCols + 16 * q;
                         const float4* ls = reinterpret_cast<const float4*>(s_lse + col);
-                        const float4* fs = reinterpret_cast<const float4*>(s_factor + col);
-                        const int node = col >> 2;  // four nodes in 16 columns
-                        const uint32_t word = node < 64 ? (node < 32 ? vis.x : vis.y) : (node < 96 ? vis.z : vis.w);
 #pragma unroll
                         for (int n = 0; n < 4; ++n) {
-                            const float4 l4 = ls[n], f4 = fs[n];
+                            const float4 l4 = ls[n];
                             float x0, x1, x2, x3;
                             unpack2(fma2(pack2(__uint_as_float(v[4 * n]), __uint_as_float(v[4 * n + 1])), scale2, pack2(l4.x, l4.y)), x0, x1);
                             unpack2(fma2(pack2(__uint_as_float(v[4 * n + 2]), __uint_as_float(v[4 * n + 3])), scale2, pack2(l4.z, l4.w)), x2, x3);
-                            float e0 = exp2_approx(x0), e1 = exp2_approx(x1), e2 = exp2_approx(x2), e3 = exp2_approx(x3);
-                            if (masked && ((word >> ((node + n) & 31)) & 1u) == 0) e0 = e1 = e2 = e3 = 0.0f;
-                            s0 = fma2(pack2(e0, e1), pack2(f4.x, f4.y), s0);
-                            s1 = fma2(pack2(e2, e3), pack2(f4.z, f4.w), s1);
+                            s0 = add2(s0, pack2(exp2_approx(x0), exp2_approx(x1)));
+                            s1 = add2(s1, pack2(exp2_approx(x2), exp2_approx(x3)));
                         }
                     };
                     for (int q = piece0; q < piece1; q += 2) {
@@ -305,7 +326,7 @@ __global__ void __launch_bounds__(kMassThreads, 1) attention_mass_kernel(const A
                     }
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) tc_arrive(bar(kMassBarRead + g));
+                    if (lane == 0) tc_arrive(bar(kMassBarRead + buffer));
                 }
                 float a0, a1, b0, b1;
                 unpack2(s0, a0, a1);
@@ -314,7 +335,7 @@ __global__ void __launch_bounds__(kMassThreads, 1) attention_mass_kernel(const A
                 float* others = s_part + (2 * g + ((i >> 1) & 1)) * 128;  // (written again two tiles on, behind a barrier of the one between)
                 if (part == 1) others[r] = sum;
                 asm volatile("bar.sync %0, 64;" ::"r"(2 + 4 * g + quarter) : "memory");
-                if (part == 0 && ok && j < seg.S) mass[j] = old + (sum + others[r]);
+                if (part == 0 && ok && j < seg.S) atomicAdd(mass + j, sum + others[r]);  // (no other thread of the call adds to it)
             }
             asm volatile("bar.sync 1, 512;" ::: "memory");
         }

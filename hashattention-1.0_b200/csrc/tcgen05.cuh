@@ -177,6 +177,16 @@ __device__ __forceinline__ void tc_ld16_wait(uint32_t (&r)[16]) {
                  :: "memory");
 }
 
+// 16 words per thread into this thread's lane (complete after tcgen05.wait::st).
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+        :: "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+           "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+        : "memory");
+}
+
 // 16 words per thread, written over the columns of this thread's lane (complete after tcgen05.wait::st) or, if to_smem, as
 // four 16-byte chunks of shared memory. One asm under two predicates: as two branches of the program the compiler copies
 // all 16 registers for one of them.

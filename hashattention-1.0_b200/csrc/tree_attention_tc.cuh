@@ -84,15 +84,6 @@ __device__ __forceinline__ void ta_mma_pv(uint32_t tmem_d, uint32_t tmem_p, uint
 }
 __device__ __forceinline__ uint32_t ta_pv_idesc() { return tc_idesc(128) | (1u << 16); }
 
-__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
-        :: "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-           "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
-        : "memory");
-}
-
 // 32 tokens from token `base` on that a row with mask `m` (bits below n only) sees, one bit each.
 __device__ __forceinline__ uint32_t visible32(const uint4& m, int base, int P, int S) {
     uint32_t vis;
