@@ -206,10 +206,12 @@ class DenseDecodeContext:
             raise ValueError(f"q must be torch.bfloat16, got {q.dtype}")
         if q.device != self.device:
             raise ValueError(f"q must live on {self.device}, got {q.device}")
+        T = q.shape[1]
         batch, node, head, one = q.stride()
+        batch, node = (0 if B == 1 else batch), (0 if T == 1 else node)  # (of a single one the stride means nothing)
         if one != 1 or (batch | node | head) % 8 or q.data_ptr() % 16:
             raise ValueError("q's rows of 128 must be contiguous and start on 16-byte boundaries")
-        T, strides = q.shape[1], self._c_strides
+        strides = self._c_strides
         strides[0], strides[1], strides[2] = batch, node, head
         return T, self._tree_struct(T, tree_mask, tree_lens), strides
 

@@ -31,7 +31,7 @@ import torch.nn.functional as F
 
 from .cache import PAGE, PagedHashKVCache
 from .dense import DenseDecodeContext, TreeAccept, tree_accept, tree_mask, unpack_nodes
-from .ops import Budget, SparseDecodeContext, rope_split
+from .ops import Budget, SparseDecodeContext, _check, rope_split
 from .synthetic import make_usa
 
 BLOCKS = 8  # the finest partition of a sharded dimension (one kv-head's worth of every matrix)
@@ -280,8 +280,8 @@ class TPLlama:
         :meth:`decode_step`'s token). With node 0 alone this is a dense decode step. Nothing synchronises with the host."""
         if self.trees is None or draft.dim() != 2 or not 1 <= draft.shape[1] <= self.trees[0].max_nodes:
             raise ValueError("verify_tree needs enable_trees(max_nodes) and a draft of [batch, 1 .. max_nodes] tokens")
-        if draft.shape[0] != self.batch:
-            raise ValueError(f"draft should have {self.batch} rows, but has {draft.shape[0]}")
+        _check(draft, "draft", torch.int64, (self.batch, draft.shape[1]), self.trees[0].device)
+        _check(parents, "parents", torch.int32, tuple(draft.shape), self.trees[0].device)
         status = self.trees[0].status
         if tree_lens is None:
             tree_lens = torch.full((self.batch,), draft.shape[1], dtype=torch.int32, device=self.device)

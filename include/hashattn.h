@@ -332,6 +332,9 @@ int ha_rope_split(const void* qkv, const int64_t* positions, int32_t batch, int3
  * token P + i; a parent comes before its children. One new token per sequence is a tree of one node.
  * Sequences with n == 0 are left out: nothing of theirs is read or written. Lengths out of range (n < 0 or > max_nodes,
  * seq_len < n or beyond max_pages * page_size) are reported as HA_ERR_BAD_SEQ_LEN and left out too.
+ * ha_tree_attention and ha_attention_mass count tiles of 64 tokens in 32 bits: shapes with more than 2^30 of them (over all sequences,
+ * kv-heads and groups of 16 query rows, at max_pages each) are refused as HA_ERR_UNSUPPORTED_DIM.
+ * Cache codes of the LSH baseline depend on every key a cache has seen: after a commit or an eviction, ha_hash_prefill anew.
  * sel_stride of the shape is not used by these entry points (any value >= 1). ha_tree_mask and ha_tree_accept, which have no
  * context to report to, take status == NULL too.                                                                       */
 #define HA_MAX_TREE_NODES 128
