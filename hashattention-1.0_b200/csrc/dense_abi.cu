@@ -61,7 +61,10 @@ int q_strides_of(const ha_shape_t* s, const ha_tree_t* t, const int64_t* strides
     return (batch | node | head) % 8 == 0 && batch >= 0 && node >= 0 && head >= 0 ? HA_OK : HA_ERR_BAD_ARG;
 }
 
-// Query rows per CTA of the attention of trees of up to max_nodes nodes: a kernel each.
+// Query rows per CTA of the attention of trees of up to max_nodes nodes: a kernel each. Measured on both sides of the borders, us:
+//   4 nodes   16 rows on mma.sync / 128 on tcgen05   8192 tokens x 8 kv-heads 16.4 / 18.4, 8 x 33001 x 1 32.3 / 39.1, 16 x 16384 x 8 166 / 196
+//   8 nodes   32 rows on mma.sync / 128 on tcgen05   21.8 / 18.8, 49.7 / 39.8, 292 / 197 (131072 x 8: 154 / 97)
+//   40 nodes  groups of 128 rows / 256               20011 x 8 43.6 / 39.8; with 64 nodes 2 x 131072 x 8 444 / 361, 8192 x 8 29.5 / 30.6
 int rows_of(int max_nodes) { return max_nodes * kGroup <= 16 ? 16 : (max_nodes * kGroup <= 128 ? 128 : 256); }
 
 size_t tree_workspace(int max_nodes) {
@@ -89,7 +92,10 @@ int launch_tree(void (*kernel)(TreeAttentionParams, CUtensorMap, CUtensorMap), i
         const dim3 grid(shape->num_kv_heads * groups, shape->batch, (rows_max + kTreeMergeWarps - 1) / kTreeMergeWarps);
         e = launch(tree_merge_kernel<kTile, kRows>, grid, dim3(kTreeMergeWarps * 32), st, 1, p, ctas);
     } else {
-        e = launch(tree_merge_tc_kernel<kRows>, dim3(shape->num_kv_heads * groups * kTaMergeParts, shape->batch, (rows_max + 31) / 32), dim3(kTaMergeThreads), st, 1, p, ctas);
+        const bool few = 4ll * shape->batch * shape->num_kv_heads * groups < ctas;  // units: many partial results of each
+        const int parts = shape->num_kv_heads * groups * (few ? kTaMergeParts : kTaMergeParts / 4);
+        e = launch(few ? tree_merge_tc_kernel<kRows, 12, 1> : tree_merge_tc_kernel<kRows, 2, 4>, dim3(parts, shape->batch, (rows_max + 31) / 32),
+                   dim3(kTaMergeThreads), st, 1, p, ctas);
     }
     return e == cudaSuccess ? HA_OK : HA_ERR_LAUNCH;
 }
@@ -166,7 +172,7 @@ int ha_tree_attention(const ha_shape_t* shape, const ha_tree_t* tree, const void
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     p.k_pages = static_cast<const __nv_bfloat16*>(k_pages);
     p.v_pages = static_cast<const __nv_bfloat16*>(v_pages);
-    if (rows == 16) return launch_tree<kRowsTile, 16, kRowsCross>(tree_attention_rows_kernel<1>, kRowsThreads, RowsLayout<1>::kSmemBytes, shape, p, st);
+    if (rows == 16) return launch_tree<kRowsTile, 16, 0>(tree_attention_rows_kernel<1>, kRowsThreads, RowsLayout<1>::kSmemBytes, shape, p, st);
     if (rows == 128) return launch_tree<kTaTile, 128, TaLayout<false>::kCross>(tree_attention_tc_kernel<false>, kTaThreads, TaLayout<false>::kSmemBytes, shape, p, st);
     return launch_tree<kTaTile, 256, TaLayout<true>::kCross>(tree_attention_tc_kernel<true>, kTaThreads, TaLayout<true>::kSmemBytes, shape, p, st);
 }

@@ -70,9 +70,10 @@ constexpr int kMaxTiles = 1 << 30;  // of all units of a call together, which th
 // in order, are cut into gridDim.x ranges of equal length (the quota): the CTAs finish together whatever the lengths of the
 // sequences, and a unit lies in at most a few CTAs. A range covers whole units but for its first and its last one, so a CTA
 // leaves at most two partial results: number 0 of its first unit, number 1 of its last.
-// A range that crosses from one unit into another pays for the end of a unit twice, which costs as much as kCross tiles. So where
-// the next larger quotas up to kCross more let every unit begin a range of its own, the smallest of those is taken, and the units
-// are seen as padded to whole ranges (their span).
+// A range that crosses from one unit into another pays for the end of a unit twice, which costs as much as kCross tiles (11 us in
+// the tensor-core attention; 0: next to nothing). So where the next larger quotas up to kCross more let every unit begin a range of
+// its own, the smallest of those is taken, and the units are seen as padded to whole ranges (their span): 20011 tokens x 8 kv-heads
+// with 32 drafts 38.7 -> 31.0 us, 131072 x 8 with 8 drafts 110 -> 101, 40000 x 8 with 64 75 -> 68.
 template <int kTile, int kRows, int kCross>
 struct DenseCut {
     static __host__ __device__ __forceinline__ int groups(int n) { return (n * kGroup + kRows - 1) / kRows; }

@@ -5,10 +5,13 @@
 //
 // in one pass over K and V with a running maximum and sum per row. A CTA takes a range of token tiles (DenseCut) of 64 tokens:
 // 32 KB of K and V, copied by TMA in the 128-byte swizzle into a ring of stages. Four warps take 16 tokens of a tile each and
-// keep a maximum, a sum and 16 (or 32) x 128 sums of their own; they meet at the end of a unit only.
+// keep a maximum, a sum and 16 x 128 sums of their own; they meet at the end of a unit only.
 //
-// The products run on the warps' matrix instructions (m16n8k16, bf16 with fp32 sums): with 4 to 32 query rows, of which a tcgen05
-// tile of 128 would be mostly padding, the bytes of K and V bound the kernel and not the products. The weights e^{s - m} are
+// The products run on the warps' matrix instructions (m16n8k16, bf16 with fp32 sums): with 4 to 16 query rows, of which a tcgen05
+// tile of 128 would be mostly padding, the bytes of K and V bound the kernel and not the products (from 5 nodes on the
+// tensor-core kernel of tree_attention_tc.cuh is faster). 32 sequences of 16K to 64K tokens x 8 kv-heads take 790 to 840 us, 780 of
+// which are the bytes at the copy rate; 16 x 16384 x 8 164 us (floor 164), 131072 x 8 89 (82); 8192 x 8 13 to 17 and 701 x 8
+// 6.7 in a graph, of which the start and the second kernel are the most. The weights e^{s - m} are
 // handed to the second product as two bf16 (hi + lo, 16 bits of mantissa), so that their rounding does not show beside
 // the one of the bf16 output. The maximum a row's weights refer to moves only when a score passes it by more than 2^8: the
 // sums are fp32 and do not mind, and rescaling 16 x 128 of them at every new maximum would.
@@ -39,13 +42,12 @@ constexpr int kRowsWarps = 4;            // consumer warps, 16 tokens each
 constexpr int kRowsThreads = (kRowsWarps + 1) * 32;
 constexpr uint32_t kRowsHalf = kRowsTile * 128;      // 64 rows x 64 elements
 constexpr uint32_t kRowsStage = 4 * kRowsHalf;       // K and V of a tile: 32 KB
-constexpr int kRowsCross = 4;            // what a second unit in a CTA's range costs, in tiles (DenseCut)
 constexpr float kRescaleAt = 8.0f;       // a row's weights may grow to 2^8 before its sums are rescaled
 
-template <int MT>  // 16-row tiles of query rows
+template <int MT>  // 16-row tiles of query rows (1 is used)
 struct RowsLayout {
     static constexpr int kRows = 16 * MT;
-    static constexpr int kStages = MT == 1 ? 5 : 4;
+    static constexpr int kStages = 5;
     static constexpr int kAccPitch = kHeadDim + 4;
     static constexpr uint32_t kOffAcc = kStages * kRowsStage;                               // [4 warps][kRows][kAccPitch] floats
     static constexpr uint32_t kOffMl = kOffAcc + kRowsWarps * kRows * kAccPitch * 4;        // [4 warps][kRows] float2
@@ -96,7 +98,7 @@ template <int MT>
 __global__ void __launch_bounds__(kRowsThreads, 1)
 tree_attention_rows_kernel(const TreeAttentionParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     using L = RowsLayout<MT>;
-    using Cursor = DenseCursor<kRowsTile, L::kRows, kRowsCross>;
+    using Cursor = DenseCursor<kRowsTile, L::kRows, 0>;
     extern __shared__ unsigned char rows_smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(rows_smem_raw) + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -374,7 +376,7 @@ tree_attention_rows_kernel(const TreeAttentionParams p, const __grid_constant__ 
 constexpr int kTreeMergeWarps = 4;
 template <int kTile, int kRows>
 __global__ void __launch_bounds__(kTreeMergeWarps * 32) tree_merge_kernel(const TreeAttentionParams p, int ctas) {
-    using Cut = DenseCut<kTile, kRows, kRowsCross>;
+    using Cut = DenseCut<kTile, kRows, 0>;
     // The lengths are read before the wait: the attention kernel in front does not write them, and what did has completed.
     const int lane = threadIdx.x & 31, r = blockIdx.z * kTreeMergeWarps + (threadIdx.x >> 5), b = blockIdx.y;
     const int max_groups = Cut::groups(p.seqs.T);

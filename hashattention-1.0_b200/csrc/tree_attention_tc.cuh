@@ -21,6 +21,15 @@
 // than 2^8) without another barrier. P is announced in two parts of 64 tokens (32 of each half): the first one's product runs under
 // the exponentials of the second.
 //
+// What bounds it. A stream's turn is 24 products of 64 clocks (1536; the lo halves are 512 of them); the streams take turns every
+// 2300 to 2450 clocks, the rest being the issuing warp's waits and the way from scores to weights (1400 clocks to the first half
+// of P, 700 more to the second). Up to 128 rows: K and V of a tile take 2760 clocks at the copy rate, so a long cache is read at
+// 5.5 to 5.7 TB/s (131072 tokens x 8 kv-heads with 8 drafts: 97 us, floor 82). 256 rows: 790 TFLOP/s (1190 with the lo halves)
+// at 4 x 131072 x 8 with 64 drafts, 694 us, where the power limit has brought the clock to 1.36 GHz; in long runs 820.
+// Short calls: 5 us until the first scores, 3 for the end of a unit, 4 for the second kernel (20011 x 8 with 32 drafts: 29.6 us).
+// Loops are kept rolled where a CTA does only a few tiles: the instructions of its first tile come from memory, and took 9000 clocks
+// where a tile takes 2500.
+//
 // The V rows behind a sequence's end, and V rows of drafts with an infinity or NaN in them, are zeroed in shared memory before
 // the product sees them; the latter are added at the end to the rows that see them, by scalar arithmetic.
 #pragma once
@@ -526,20 +535,24 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
     }
 }
 
-// The partial results of the units that several CTAs share: a thread has one row and four dimensions of every second one of them,
-// a warp 32 rows side by side (as they lie in the workspace), a CTA 32 rows x 16 dimensions;
-// grid (Hkv * groups of T x 8, B, rows / 32).
-constexpr int kTaMergeThreads = 256, kTaMergeParts = 8, kTaMergeBatch = 12;
-template <int kRows>
+// The partial results of the units that several CTAs share: a thread has one row and four dimensions (of kSteps pieces of 16 in
+// turn) of every second one of them, a warp 32 rows side by side (as they lie in the workspace), a CTA 32 rows x 16 kSteps dimensions;
+// grid (Hkv * groups of T x 8 / kSteps, B, rows / 32). kBatch partial results are loaded together. Few units: each has many
+// partial results, and the CTAs are made small (12 at once, one step). Many units: two or three each, and what counts is how many
+// CTAs there are and how many fit an SM (2 at once, 4 steps; 16 sequences of 2000 tokens x 4 kv-heads with 48 drafts 70 -> 46 us a
+// call, 64 of 600 x 8 with 20 148 -> 92).
+constexpr int kTaMergeThreads = 256, kTaMergeParts = 8;
+template <int kRows, int kBatch, int kSteps>
 __global__ void __launch_bounds__(kTaMergeThreads) tree_merge_tc_kernel(const TreeAttentionParams p, int ctas) {
     using Cut = DenseCut<kTaTile, kRows, TaLayout<(kRows > 128)>::kCross>;
+    constexpr int kGrid = kTaMergeParts / kSteps;
     __shared__ float4 s_acc[4][32];
     __shared__ float2 s_ml[4][32];
     __shared__ uint2 s_out[32][5];  // [row][4 x 4 dimensions] bf16 (a column of padding)
     // The lengths are read before the wait: the attention kernel in front does not write them, and what did has completed.
     const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) & 3, half = threadIdx.x >> 7, b = blockIdx.y;
-    const int max_groups = Cut::groups(p.seqs.T), x = blockIdx.x / kTaMergeParts, kvh = x / max_groups, group = x - kvh * max_groups;
-    const int d4 = (blockIdx.x % kTaMergeParts) * 4 + warp, row0 = blockIdx.z * 32;
+    const int max_groups = Cut::groups(p.seqs.T), x = blockIdx.x / kGrid, kvh = x / max_groups, group = x - kvh * max_groups;
+    const int row0 = blockIdx.z * 32;
     int S, n;
     dense_seq(p.seqs, b, false, S, n);
     int quota, before, span;
@@ -548,64 +561,69 @@ __global__ void __launch_bounds__(kTaMergeThreads) tree_merge_tc_kernel(const Tr
     const int tiles = Cut::tiles_of(S), r = min(row0 + lane, rows - 1);
     const int start = before + (kvh * Cut::groups(n) + group) * span;
     const int c0 = dense_div(start, quota), c1 = dense_div(start + tiles - 1, quota), first_slot = 2 * c0 + (c0 * quota != start ? 1 : 0);
-    const float4* part = reinterpret_cast<const float4*>(p.part_acc) + (size_t)d4 * kRows + r;
     pdl_wait();
     pdl_launch_dependents();
     if (row0 >= rows || c0 == c1) return;  // (c0 == c1: one CTA had the whole unit)
-    float M = -INFINITY, sum = 0.0f;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    auto rescale = [&](float top) {  // -> the reference of what is added next
-        const float ref = top == -INFINITY ? 0.0f : top, f = exp2_approx(M - ref);
-        M = top;
-        sum *= f;
-        acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
-        return ref;
-    };
-    auto add = [&](float2 ml, float4 a, float ref) {
-        const float f = exp2_approx(ml.x - ref);
-        sum = fmaf(ml.y, f, sum);
-        acc.x = fmaf(a.x, f, acc.x); acc.y = fmaf(a.y, f, acc.y);
-        acc.z = fmaf(a.z, f, acc.z); acc.w = fmaf(a.w, f, acc.w);
-    };
-    for (int cb = c0 + half; cb <= c1; cb += 2 * kTaMergeBatch) {  // the loads of a batch in flight together
-        float2 ml[kTaMergeBatch];
-        float4 a[kTaMergeBatch];
+#pragma unroll 1
+    for (int step = 0; step < kSteps; ++step) {
+        const int d4 = ((int)(blockIdx.x % kGrid) * kSteps + step) * 4 + warp;
+        const float4* part = reinterpret_cast<const float4*>(p.part_acc) + (size_t)d4 * kRows + r;
+        float M = -INFINITY, sum = 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        auto rescale = [&](float top) {  // -> the reference of what is added next
+            const float ref = top == -INFINITY ? 0.0f : top, f = exp2_approx(M - ref);
+            M = top;
+            sum *= f;
+            acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+            return ref;
+        };
+        auto add = [&](float2 ml, float4 a, float ref) {
+            const float f = exp2_approx(ml.x - ref);
+            sum = fmaf(ml.y, f, sum);
+            acc.x = fmaf(a.x, f, acc.x); acc.y = fmaf(a.y, f, acc.y);
+            acc.z = fmaf(a.z, f, acc.z); acc.w = fmaf(a.w, f, acc.w);
+        };
+        for (int cb = c0 + half; cb <= c1; cb += 2 * kBatch) {  // the loads of a batch in flight together
+            float2 ml[kBatch];
+            float4 a[kBatch];
 #pragma unroll
-        for (int k = 0; k < kTaMergeBatch; ++k) {
-            const int c = cb + 2 * k;
-            const size_t slot = (size_t)(c == c0 ? first_slot : 2 * c);
-            ml[k] = make_float2(-INFINITY, 0.0f);
-            a[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (c <= c1) {
-                ml[k] = __ldcg(&p.part_ml[slot * kRows + r]);
-                a[k] = __ldcg(part + slot * (kHeadDim / 4) * kRows);
+            for (int k = 0; k < kBatch; ++k) {
+                const int c = cb + 2 * k;
+                const size_t slot = (size_t)(c == c0 ? first_slot : 2 * c);
+                ml[k] = make_float2(-INFINITY, 0.0f);
+                a[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (c <= c1) {
+                    ml[k] = __ldcg(&p.part_ml[slot * kRows + r]);
+                    a[k] = __ldcg(part + slot * (kHeadDim / 4) * kRows);
+                }
             }
+            float top = M;
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) top = fmaxf(top, ml[k].x);
+            const float ref = rescale(top);
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) add(ml[k], a[k], ref);
         }
-        float top = M;
-#pragma unroll
-        for (int k = 0; k < kTaMergeBatch; ++k) top = fmaxf(top, ml[k].x);
-        const float ref = rescale(top);
-#pragma unroll
-        for (int k = 0; k < kTaMergeBatch; ++k) add(ml[k], a[k], ref);
+        if (half == 1) {
+            s_acc[warp][lane] = acc;
+            s_ml[warp][lane] = make_float2(M, sum);
+        }
+        __syncthreads();
+        auto out_row = [&](int row) {
+            return ((size_t)b * p.seqs.T + (group * kRows + row) / kGroup) * ((size_t)p.seqs.Hkv * kGroup) + kvh * kGroup + (row & (kGroup - 1));
+        };
+        if (half == 0) {
+            const float2 ml = s_ml[warp][lane];
+            add(ml, s_acc[warp][lane], rescale(fmaxf(M, ml.x)));
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            s_out[lane][warp] = make_uint2(tc_pack_bf16(acc.x * inv, acc.y * inv), tc_pack_bf16(acc.z * inv, acc.w * inv));
+            if (d4 == 0 && row0 + lane < rows && p.lse != nullptr) p.lse[out_row(row0 + lane)] = natural_lse(M, sum);
+        }
+        __syncthreads();  // (and the other half's results have been read)
+        const int row = threadIdx.x >> 2, piece = threadIdx.x & 3;  // 32 bytes of a row: four threads
+        if (half == 0 && row0 + row < rows) reinterpret_cast<uint2*>(p.out + out_row(row0 + row) * kHeadDim)[d4 - warp + piece] = s_out[row][piece];
+        if (kSteps > 1) __syncthreads();
     }
-    if (half == 1) {
-        s_acc[warp][lane] = acc;
-        s_ml[warp][lane] = make_float2(M, sum);
-    }
-    __syncthreads();
-    auto out_row = [&](int row) {
-        return ((size_t)b * p.seqs.T + (group * kRows + row) / kGroup) * ((size_t)p.seqs.Hkv * kGroup) + kvh * kGroup + (row & (kGroup - 1));
-    };
-    if (half == 0) {
-        const float2 ml = s_ml[warp][lane];
-        add(ml, s_acc[warp][lane], rescale(fmaxf(M, ml.x)));
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        s_out[lane][warp] = make_uint2(tc_pack_bf16(acc.x * inv, acc.y * inv), tc_pack_bf16(acc.z * inv, acc.w * inv));
-        if (d4 == 0 && row0 + lane < rows && p.lse != nullptr) p.lse[out_row(row0 + lane)] = natural_lse(M, sum);
-    }
-    __syncthreads();
-    const int row = threadIdx.x >> 2, piece = threadIdx.x & 3;  // 32 bytes of a row: four threads
-    if (half == 0 && row0 + row < rows) reinterpret_cast<uint2*>(p.out + out_row(row0 + row) * kHeadDim)[d4 - warp + piece] = s_out[row][piece];
 }
 
 }  // namespace ha
