@@ -129,6 +129,7 @@ int ha_tree_accept(const int64_t* draft, const int32_t* parents, const int64_t* 
         next_token == nullptr || new_lens == nullptr || batch < 1 || max_nodes < 1 || !aligned16(accepted))
         return HA_ERR_BAD_ARG;
     if (max_nodes > kMaxNodes) return HA_ERR_UNSUPPORTED_DIM;
+    if (new_lens == seq_lens) return HA_ERR_BAD_ARG;  // (the commits still need the lengths with all drafts)
     TreeAcceptParams p;
     p.draft = reinterpret_cast<const long long*>(draft);
     p.parents = parents;

@@ -131,6 +131,8 @@ def tree_accept(draft: torch.Tensor, parents: torch.Tensor, target: torch.Tensor
     _check(out.count, "count", torch.int32, (B,), dev)
     _check(out.next_token, "next_token", torch.int64, (B,), dev)
     _check(out.seq_lens, "out.seq_lens", torch.int32, (B,), dev)
+    if out.seq_lens.data_ptr() == seq_lens.data_ptr():
+        raise ValueError("out.seq_lens must be another tensor than seq_lens, which the commits still need")
     status_ptr = _status_ptr(status, dev)
     with library_call(dev, "ha_tree_accept"):
         rc = _lib.load().ha_tree_accept(draft.data_ptr(), parents.data_ptr(), target.data_ptr(),

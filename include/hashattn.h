@@ -334,6 +334,7 @@ int ha_rope_split(const void* qkv, const int64_t* positions, int32_t batch, int3
  * seq_len < n or beyond max_pages * page_size) are reported as HA_ERR_BAD_SEQ_LEN and left out too.
  * ha_tree_attention and ha_attention_mass count tiles of 64 tokens in 32 bits: shapes with more than 2^30 of them (over all sequences,
  * kv-heads and groups of 16 query rows, at max_pages each) are refused as HA_ERR_UNSUPPORTED_DIM.
+ * ha_tree_commit and ha_cache_evict move rows in place: the pages they write to must not be shared between sequences.
  * Cache codes of the LSH baseline depend on every key a cache has seen: after a commit or an eviction, ha_hash_prefill anew.
  * sel_stride of the shape is not used by these entry points (any value >= 1). ha_tree_mask and ha_tree_accept, which have no
  * context to report to, take status == NULL too.                                                                       */
@@ -377,7 +378,8 @@ int ha_attention_mass(const ha_shape_t* shape, const ha_tree_t* tree, const void
 /* Greedy acceptance: from node 0 (the token that is certain) on, the lowest child whose drafted token is the target token of
  * its parent (target[b][i]: the token the model puts behind node i). draft, target [batch][max_nodes] int64, parents as
  * ha_tree_mask takes them. accepted [batch][4] <- the path's nodes, one bit each; count[b] <- their number; next_token[b] <-
- * the target of the path's last node (untouched where n == 0); new_lens[b] <- seq_lens[b] - n + count[b].               */
+ * the target of the path's last node (untouched where n == 0); new_lens[b] (not seq_lens, which the commits still need) <-
+ * seq_lens[b] - n + count[b].                                                                                       */
 int ha_tree_accept(const int64_t* draft, const int32_t* parents, const int64_t* target, const int32_t* tree_lens,
                    const int32_t* seq_lens, int32_t batch, int32_t max_nodes, uint32_t* accepted, int32_t* count,
                    int64_t* next_token, int32_t* new_lens, int32_t* status, void* stream);

@@ -68,6 +68,19 @@ def test_drawn_shapes(device, seed):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 5, 40])
+@pytest.mark.parametrize("scale", [300.0, 5000.0])
+def test_scores_of_many_thousands(device, n, scale):
+    """One token has all of a row's weight: the references that weights are taken against must not be coarser than fp32's range
+    allows (2^18 in powers of two here, where half an ulp of bf16 is 512)."""
+    x = Problem(device, [n + 700, n], [n, n], 2, n, seed=n)
+    x.ctx = ha.DenseDecodeContext(x.cache, n, sm_scale=scale)
+    x.scale = x.ctx.sm_scale
+    out, lse = x.ctx.tree_attention(x.q, x.mask, x.tree_lens)
+    x.check(out, lse)
+
+
+@pytest.mark.gpu
 def test_contexts_that_share_workspaces(device):
     a, b = Problem(device, [3000], [20], 4, seed=1), Problem(device, [2500], [7], 4, seed=2)
     ctx = ha.DenseDecodeContext(b.cache, 7, workspace_of=a.ctx)
@@ -100,3 +113,18 @@ def test_shapes_with_more_tiles_than_are_counted_are_refused():
         assert lib.ha_tree_attention(shape, tree, X, None, X, X, X, X, 0.1, X, None, X, 8, X, None) == want
         if ok is not None:
             assert lib.ha_attention_mass(shape, tree, X, None, X, None, X, X, X, 0.1, X, X, None) == want
+
+
+@pytest.mark.gpu
+def test_acceptance_does_not_write_the_lengths_that_the_commit_needs(device):
+    x = Problem(device, [300], [4], 1, seed=1)
+    out = ha.TreeAccept.empty(1, device)
+    same = ha.TreeAccept(out.accepted, out.count, out.next_token, x.cache.seq_lens)
+    tokens = torch.zeros(1, 4, dtype=torch.int64, device=device)
+    with pytest.raises(ValueError, match="seq_lens"):
+        ha.tree_accept(tokens, x.parents, tokens, x.tree_lens, x.cache.seq_lens, out=same)
+
+
+def test_the_library_refuses_acceptance_over_the_lengths():
+    lib, X, Y = _lib.load(), ctypes.c_void_p(256), ctypes.c_void_p(512)  # (never dereferenced)
+    assert lib.ha_tree_accept(X, X, X, None, Y, 1, 8, X, X, X, Y, None, None) == _lib.HA_ERR_BAD_ARG
