@@ -86,8 +86,10 @@ def tree_mask(parents: torch.Tensor, tree_lens: torch.Tensor | None = None, out:
     _check(parents, "parents", torch.int32, (B, T), dev)
     if tree_lens is not None:
         _check(tree_lens, "tree_lens", torch.int32, (B,), dev)
-    out = torch.empty(B, T, MASK_WORDS, dtype=torch.int32, device=dev) if out is None else out
-    _check(out, "out", torch.int32, (B, T, MASK_WORDS), dev)
+    if out is None:
+        out = torch.empty(B, T, MASK_WORDS, dtype=torch.int32, device=dev)
+    else:
+        _check(out, "out", torch.int32, (B, T, MASK_WORDS), dev)
     status_ptr = _status_ptr(status, dev)
     with library_call(dev, "ha_tree_mask"):
         rc = _lib.load().ha_tree_mask(parents.data_ptr(), tree_lens.data_ptr() if tree_lens is not None else None, B, T,
@@ -108,9 +110,9 @@ class TreeAccept:
 
     @staticmethod
     def empty(batch: int, device) -> "TreeAccept":
-        count = torch.empty(batch, dtype=torch.int32, device=device)
-        return TreeAccept(count.new_empty((batch, MASK_WORDS)), count, torch.empty(batch, dtype=torch.int64, device=device),
-                          torch.empty_like(count))
+        count = torch.empty(batch, dtype=torch.int32, device=device)  # (sizes as numbers: a tuple costs 1 us more)
+        return TreeAccept(torch.empty(batch, MASK_WORDS, dtype=torch.int32, device=device), count,
+                          torch.empty(batch, dtype=torch.int64, device=device), torch.empty_like(count))
 
 
 def tree_accept(draft: torch.Tensor, parents: torch.Tensor, target: torch.Tensor, tree_lens: torch.Tensor | None,
@@ -126,13 +128,15 @@ def tree_accept(draft: torch.Tensor, parents: torch.Tensor, target: torch.Tensor
     if tree_lens is not None:
         _check(tree_lens, "tree_lens", torch.int32, (B,), dev)
     _check(seq_lens, "seq_lens", torch.int32, (B,), dev)
-    out = TreeAccept.empty(B, dev) if out is None else out
-    _check(out.accepted, "accepted", torch.int32, (B, MASK_WORDS), dev)
-    _check(out.count, "count", torch.int32, (B,), dev)
-    _check(out.next_token, "next_token", torch.int64, (B,), dev)
-    _check(out.seq_lens, "out.seq_lens", torch.int32, (B,), dev)
-    if out.seq_lens.data_ptr() == seq_lens.data_ptr():
-        raise ValueError("out.seq_lens must be another tensor than seq_lens, which the commits still need")
+    if out is None:
+        out = TreeAccept.empty(B, dev)
+    else:
+        _check(out.accepted, "accepted", torch.int32, (B, MASK_WORDS), dev)
+        _check(out.count, "count", torch.int32, (B,), dev)
+        _check(out.next_token, "next_token", torch.int64, (B,), dev)
+        _check(out.seq_lens, "out.seq_lens", torch.int32, (B,), dev)
+        if out.seq_lens.data_ptr() == seq_lens.data_ptr():
+            raise ValueError("out.seq_lens must be another tensor than seq_lens, which the commits still need")
     status_ptr = _status_ptr(status, dev)
     with library_call(dev, "ha_tree_accept"):
         rc = _lib.load().ha_tree_accept(draft.data_ptr(), parents.data_ptr(), target.data_ptr(),
@@ -180,6 +184,9 @@ class DenseDecodeContext:
                 raise ValueError("workspace_of must be a context on the same device with workspaces at least as large")
             self.workspace, self.evict_workspace = o.workspace, o.evict_workspace
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        # (the context's own buffers, which stay where they are as long as it lives)
+        self._workspace_ptr, self._evict_workspace_ptr, self._status_ptr = (
+            t.data_ptr() for t in (self.workspace, self.evict_workspace, self.status))
 
     @property
     def mass_shape(self):
@@ -241,16 +248,20 @@ class DenseDecodeContext:
         T, tree, strides = self._tree(q, tree_mask, tree_lens)
         make = torch.zeros if tree_lens is not None else torch.empty
         size = (self.batch, T, self.num_q_heads)
-        out = make(*size, HEAD_DIM, dtype=torch.bfloat16, device=self.device) if out is None else out
-        lse = make(size, dtype=torch.float32, device=self.device) if lse is None else lse
-        _check(out, "out", torch.bfloat16, (*size, HEAD_DIM), self.device)
-        _check(lse, "lse", torch.float32, size, self.device)
+        if out is None:
+            out = make(*size, HEAD_DIM, dtype=torch.bfloat16, device=self.device)
+        else:
+            _check(out, "out", torch.bfloat16, (*size, HEAD_DIM), self.device)
+        if lse is None:
+            lse = make(*size, dtype=torch.float32, device=self.device)
+        else:
+            _check(lse, "lse", torch.float32, size, self.device)
         c = self.cache
         with library_call(self.device, "ha_tree_attention"):
             rc = self.lib.ha_tree_attention(
                 self._shape_ref, tree, q.data_ptr(), strides, c.k_pages.data_ptr(), c.v_pages.data_ptr(), c.page_table.data_ptr(),
-                c.seq_lens.data_ptr(), self.sm_scale, out.data_ptr(), lse.data_ptr(), self.workspace.data_ptr(),
-                self.workspace_bytes, self.status.data_ptr(), _stream_ptr(self.device))
+                c.seq_lens.data_ptr(), self.sm_scale, out.data_ptr(), lse.data_ptr(), self._workspace_ptr,
+                self.workspace_bytes, self._status_ptr, _stream_ptr(self.device))
         _raise_on(rc, "ha_tree_attention")
         return out, lse
 
@@ -268,7 +279,7 @@ class DenseDecodeContext:
             rc = self.lib.ha_attention_mass(
                 self._shape_ref, tree, q.data_ptr(), strides, lse.data_ptr(), rows.data_ptr() if rows is not None else None,
                 c.k_pages.data_ptr(), c.page_table.data_ptr(), c.seq_lens.data_ptr(), self.sm_scale, mass.data_ptr(),
-                self.status.data_ptr(), _stream_ptr(self.device))
+                self._status_ptr, _stream_ptr(self.device))
         _raise_on(rc, "ha_attention_mass")
         return mass
 
@@ -285,7 +296,7 @@ class DenseDecodeContext:
             rc = self.lib.ha_tree_commit(
                 self._shape_ref, tree, accepted.data_ptr(), c.k_pages.data_ptr(), c.v_pages.data_ptr(), c.hash_pages.data_ptr(),
                 c.page_table.data_ptr(), c.seq_lens.data_ptr(), mass.data_ptr() if mass is not None else None,
-                self.status.data_ptr(), _stream_ptr(self.device))
+                self._status_ptr, _stream_ptr(self.device))
         _raise_on(rc, "ha_tree_commit")
 
     def cache_evict(self, mass, keep_tokens: int, init_budget: int = 128, recent_budget: int = 128,
@@ -314,7 +325,7 @@ class DenseDecodeContext:
             rc = self.lib.ha_cache_evict(
                 self._shape_ref, keep_tokens, init_budget, recent_budget, mass.data_ptr(), c.k_pages.data_ptr(), c.v_pages.data_ptr(),
                 c.hash_pages.data_ptr(), c.page_table.data_ptr(), c.seq_lens.data_ptr(), kept.data_ptr(), mass_out.data_ptr(),
-                lens_out.data_ptr(), self.evict_workspace.data_ptr(), self.evict_workspace_bytes, self.status.data_ptr(),
+                lens_out.data_ptr(), self._evict_workspace_ptr, self.evict_workspace_bytes, self._status_ptr,
                 _stream_ptr(self.device))
         _raise_on(rc, "ha_cache_evict")
         return kept, mass_out, lens_out
