@@ -161,10 +161,16 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const TreeC
     }
     __syncthreads();
     const int P = S - n;
-    // the drafts lie on two pages at most
-    const int page0 = P / kPage;
-    const size_t base0 = ((size_t)dense_page(d, b, page0) * d.Hkv + kvh) * kPage;
-    const size_t base1 = (S - 1) / kPage > page0 ? ((size_t)dense_page(d, b, page0 + 1) * d.Hkv + kvh) * kPage : base0;
+    // The drafts lie on two pages at most. A page id out of range is no place to write to (page 0, which a reader may take instead, is
+    // another sequence's): then nothing of the sequence's moves, on no kv-head, the weights included. The ids are the same for the whole CTA.
+    const int page0 = P / kPage, page1 = (S - 1) / kPage;
+    const int32_t* table = d.page_table + (size_t)b * d.max_pages;
+    const int id0 = __ldg(table + page0), id1 = __ldg(table + page1);
+    if (id0 < 0 || id0 >= d.num_pages || id1 < 0 || id1 >= d.num_pages) {
+        if (tid == 0) report(d.status, HA_ERR_BAD_PAGE);
+        return;
+    }
+    const size_t base0 = ((size_t)id0 * d.Hkv + kvh) * kPage, base1 = ((size_t)id1 * d.Hkv + kvh) * kPage;
     auto slot = [&](int token) { return (token / kPage == page0 ? base0 : base1) + token % kPage; };
     const int per_row = p.hash_pages != nullptr ? 33 : 32;
     uint4 v[kCommitPieces];

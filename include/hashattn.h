@@ -386,6 +386,7 @@ int ha_tree_accept(const int64_t* draft, const int32_t* parents, const int64_t* 
 
 /* Moves the rows of the accepted nodes (any set of nodes) of one layer's cache to the front of the drafts, in order, in
  * place: K, V, the code words (hash_pages, optional) and the received weights (mass, optional; zero behind the accepted ones).
+ * Where a page id of the drafts is out of range (HA_ERR_BAD_PAGE in the status word) nothing of that sequence moves.
  * seq_lens are those before the commit and are not changed (the layers of a model share them): afterwards the sequence's
  * length is new_lens of ha_tree_accept.                                                                              */
 int ha_tree_commit(const ha_shape_t* shape, const ha_tree_t* tree, const uint32_t* accepted, void* k_pages, void* v_pages,

@@ -1,0 +1,58 @@
+"""What commit and eviction move, and what they leave alone: page ids and lengths that are out of range, rounds narrower than the
+context, capacities far above the lengths. Rows are compared bit by bit."""
+import pytest
+import torch
+
+import hashattention_b200 as ha
+from hashattention_b200 import _lib
+from test_dense import Problem, evict64, flat_rows
+
+
+def pools(cache):
+    """The three pools as integers (NaN compares)."""
+    return [cache.k_pages.view(torch.int16).clone(), cache.v_pages.view(torch.int16).clone(), cache.hash_pages.clone()]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [-1, 2 ** 31 - 1, "num_pages"])
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("owner", ["nobody", "a sequence"])
+def test_commit_writes_nothing_where_a_page_id_is_out_of_range(device, bad, which, owner):
+    """Drafts that cross from page 1 into page 2, one of the two ids out of range: no pool row changes, physical page 0 included,
+    and the sequences beside it are committed."""
+    n = 9
+    x = Problem(device, [515, 300, 515], [n, n, n], 2, n, seed=11)
+    table = x.cache.page_table
+    spare = sorted(set(range(x.cache.num_pages)) - set(table.flatten().tolist()))
+    # physical page 0: nobody's, or page 0 of the last sequence (the pool's pages change places with their contents)
+    zero = (table == 0).nonzero()
+    if owner == "a sequence":
+        if len(zero):
+            b, i = zero[0].tolist()
+            table[b, i] = table[2, 0]
+        table[2, 0] = 0
+    elif len(zero):
+        b, i = zero[0].tolist()
+        table[b, i] = spare[0] if spare[0] != 0 else spare[1]
+    for b in range(3):
+        x.write(b)
+    table[0, 1 + which] = x.cache.num_pages if bad == "num_pages" else bad
+    bits = torch.zeros(3, 128, dtype=torch.bool)
+    bits[0, [2, 5, 8]] = True   # moves in the sequence with the bad page
+    bits[1, [1, 3, 7]] = True   # moves beside it
+    bits[2, 0] = True           # moves nothing
+    mass = torch.rand(x.ctx.mass_shape, device=device)
+    before, old = pools(x.cache), mass.clone()
+    x.ctx.tree_commit(ha.pack_nodes(bits).to(device), x.tree_lens, mass=mass)
+    with pytest.raises(RuntimeError, match=rf"status {_lib.HA_ERR_BAD_PAGE}\)"):
+        x.ctx.check_status()
+    own = table[1].tolist()
+    P = 300 - n
+    for was, now in zip(before, pools(x.cache)):
+        others = [i for i in range(x.cache.num_pages) if i not in own]
+        assert torch.equal(now[others], was[others]), "rows of another sequence were moved"
+        flat_was, flat_now = was[own].transpose(0, 1).flatten(1, 2), now[own].transpose(0, 1).flatten(1, 2)
+        want = flat_was.clone()
+        want[:, P:P + 3] = flat_was[:, [P + 1, P + 3, P + 7]]
+        assert torch.equal(flat_now, want)
+    assert torch.equal(mass[0], old[0]), "the received weights moved without their rows"
