@@ -226,13 +226,15 @@ class TPLlama:
     def enable_trees(self, max_nodes: int, mass: bool = False) -> None:
         """Prepares :meth:`verify_tree` for trees of up to ``max_nodes`` drafted tokens and, with ``mass``, keeps for every
         layer the attention weight that each cached token has received (what :meth:`evict` goes by). Allocates; the
-        layers run one after another and share one workspace."""
+        layers run one after another and share one workspace. The weights stay in these tensors for good: captured rounds
+        hold their addresses."""
         if self.attention != "cuda":
             raise ValueError("trees are verified on the paged cache: attention='cuda'")
         self.trees = []
         for ctx in self.ctxs:
             self.trees.append(DenseDecodeContext(ctx.cache, max_nodes, workspace_of=self.trees[0] if self.trees else None))
         self.mass = [t.new_mass() for t in self.trees] if mass else None
+        self._evicted_mass = self.trees[0].new_mass() if mass else None  # what an eviction leaves, on its way back into a layer's
 
     def _append_drafts(self, layer: int, k: torch.Tensor, v: torch.Tensor, first: torch.Tensor, tree_lens: torch.Tensor) -> None:
         """k, v [B, T, Hkv, 128] -> the cache's tokens first[b] .. first[b] + tree_lens[b] - 1. Rows behind a tree's own repeat
@@ -308,7 +310,8 @@ class TPLlama:
         init_budget = self.cfg.init_budget if init_budget is None else init_budget
         recent_budget = self.cfg.recent_budget if recent_budget is None else recent_budget
         for i, tree in enumerate(self.trees):
-            _, self.mass[i], lens = tree.cache_evict(self.mass[i], keep_tokens, init_budget, recent_budget)
+            _, left, lens = tree.cache_evict(self.mass[i], keep_tokens, init_budget, recent_budget, mass_out=self._evicted_mass)
+            self.mass[i].copy_(left)
         self.seq_lens.copy_(lens)
 
     # -- one greedy decode step for the whole batch ------------------------------------------------
