@@ -101,7 +101,8 @@ def tree_mask(parents: torch.Tensor, tree_lens: torch.Tensor | None = None, out:
 @dataclass(frozen=True)
 class TreeAccept:
     """The accepted path of every sequence: its nodes as words ``[B, 4]`` int32, their number ``[B]`` int32, the token behind
-    the last one ``[B]`` int64, and the sequence's length once the path is committed ``[B]`` int32."""
+    the last one ``[B]`` int64 (left as it was where a sequence has no drafts; 0 in a new one), and the sequence's length once
+    the path is committed ``[B]`` int32."""
 
     accepted: torch.Tensor
     count: torch.Tensor
@@ -112,7 +113,7 @@ class TreeAccept:
     def empty(batch: int, device) -> "TreeAccept":
         count = torch.empty(batch, dtype=torch.int32, device=device)  # (sizes as numbers: a tuple costs 1 us more)
         return TreeAccept(torch.empty(batch, MASK_WORDS, dtype=torch.int32, device=device), count,
-                          torch.empty(batch, dtype=torch.int64, device=device), torch.empty_like(count))
+                          torch.zeros(batch, dtype=torch.int64, device=device), torch.empty_like(count))
 
 
 def tree_accept(draft: torch.Tensor, parents: torch.Tensor, target: torch.Tensor, tree_lens: torch.Tensor | None,

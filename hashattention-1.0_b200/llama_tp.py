@@ -279,7 +279,8 @@ class TPLlama:
         certain, as the previous step returned it), ``parents [B, T]`` int32 (-1: a root), ``tree_lens [B]`` int32 where trees
         are shorter than T. One pass with full attention over the cache, greedy acceptance, and the accepted path stays in the
         cache: positions and lengths advance by ``count``, ``next_token`` is the next round's node 0 (or the next
-        :meth:`decode_step`'s token). With node 0 alone this is a dense decode step. Nothing synchronises with the host."""
+        :meth:`decode_step`'s token; where a sequence has no drafts, ``draft[:, 0]`` still is). With node 0 alone this is a
+        dense decode step. Nothing synchronises with the host."""
         if self.trees is None or draft.dim() != 2 or not 1 <= draft.shape[1] <= self.trees[0].max_nodes:
             raise ValueError("verify_tree needs enable_trees(max_nodes) and a draft of [batch, 1 .. max_nodes] tokens")
         _check(draft, "draft", torch.int64, (self.batch, draft.shape[1]), self.trees[0].device)
@@ -289,7 +290,9 @@ class TPLlama:
             tree_lens = torch.full((self.batch,), draft.shape[1], dtype=torch.int32, device=self.device)
         mask = tree_mask(parents, tree_lens, status=status)
         logits, kept = self._tree_forward(draft, mask, tree_lens)
-        got = tree_accept(draft, parents, logits.float().argmax(-1), tree_lens, self.seq_lens, status=status)
+        got = TreeAccept.empty(self.batch, draft.device)
+        got.next_token.copy_(draft[:, 0])
+        tree_accept(draft, parents, logits.float().argmax(-1), tree_lens, self.seq_lens, out=got, status=status)
         for i, tree in enumerate(self.trees):
             mass = None
             if self.mass is not None:

@@ -51,6 +51,31 @@ def _chain(B, T, device):
 
 
 @pytest.mark.gpu
+def test_next_token_of_a_sequence_without_drafts(device):
+    """Where nothing was drafted there is no token behind the last accepted one: node 0's stays the next one in a model's round (the
+    embedding takes it), and acceptance by itself gives 0 in tensors of its own and leaves given ones alone."""
+    import hashattention_b200 as ha
+    model = _model(device, 3, 4)
+    _prefilled(model, [50, 40, 30])
+    draft = torch.randint(0, 1000, (3, 4), generator=torch.Generator().manual_seed(2)).to(device)
+    lens = torch.tensor([4, 0, 1], dtype=torch.int32, device=device)
+    torch.full((4096,), -7, dtype=torch.int64, device=device)  # (freed: what the allocator hands out next)
+    got = model.verify_tree(draft, _chain(3, 4, device), lens)
+    model.check_status()
+    assert got.count.tolist()[1] == 0 and int(got.next_token[1]) == int(draft[1, 0])
+    nxt = torch.empty(3, dtype=torch.int64, device=device)
+    model.decode_step(got.next_token, nxt)
+    model.check_status()
+    args = (draft, _chain(3, 4, device), draft, lens, model.seq_lens)
+    for size in (1, 3, 64, 512):
+        torch.full((size,), -7, dtype=torch.int64, device=device)
+    assert int(ha.tree_accept(*args).next_token[1]) == 0
+    out = ha.TreeAccept.empty(3, device)
+    out.next_token.fill_(77)
+    assert int(ha.tree_accept(*args, out=out).next_token[1]) == 77
+
+
+@pytest.mark.gpu
 def test_a_round_captured_before_an_eviction_goes_on_after_it(device):
     """The received weights stay in the tensors that a captured round adds to: replayed after an eviction it gives what the eager
     round gives."""
