@@ -29,6 +29,7 @@ import torch
 import torch.distributed as dist
 import torch.nn.functional as F
 
+from . import _lib
 from .cache import PAGE, PagedHashKVCache
 from .dense import DenseDecodeContext, TreeAccept, tree_accept, tree_mask, unpack_nodes
 from .ops import Budget, SparseDecodeContext, _check, rope_split
@@ -237,17 +238,26 @@ class TPLlama:
         self._evicted_mass = self.trees[0].new_mass() if mass else None  # what an eviction leaves, on its way back into a layer's
 
     def _append_drafts(self, layer: int, k: torch.Tensor, v: torch.Tensor, first: torch.Tensor, tree_lens: torch.Tensor) -> None:
-        """k, v [B, T, Hkv, 128] -> the cache's tokens first[b] .. first[b] + tree_lens[b] - 1. Rows behind a tree's own repeat
-        its last one (in a sequence without drafts: put back the cache's last token)."""
+        """k, v [B, T, Hkv, 128] -> the cache's tokens first[b] .. first[b] + tree_lens[b] - 1, which have to fit. Rows behind a
+        tree's own repeat its last one (in a sequence without drafts: put back the cache's last token)."""
         cache = self.ctxs[layer].cache
         n = tree_lens.long()[:, None]
         row = torch.minimum(torch.arange(k.shape[1], device=self.device)[None], n - 1)      # [B, T]; -1: no drafts
-        token = (first.long()[:, None] + row).clamp(0, cache.max_pages * PAGE - 1)          # (lengths beyond that are reported)
+        token = (first.long()[:, None] + row).clamp(0, cache.max_pages * PAGE - 1)          # (an empty cache has no last token)
         page, slot = cache.page_table.long().gather(1, token // PAGE), token % PAGE
         take = row.clamp_min(0)[..., None, None].expand(-1, -1, *k.shape[2:])
         for pool, new in ((cache.k_pages, k), (cache.v_pages, v)):
             new = torch.where((n > 0)[..., None, None], new.gather(1, take), pool[page, :, slot])
             pool[page, :, slot] = new
+
+    def _fitting_trees(self, tree_lens: torch.Tensor, nodes: int) -> torch.Tensor:
+        """``tree_lens`` with 0 in the place of those out of 0 .. ``nodes`` and of those that do not fit the cache behind their
+        sequence, which are reported (HA_ERR_BAD_SEQ_LEN, as the kernels do): such a sequence takes no part in the round."""
+        lens, status = self.seq_lens, self.trees[0].status
+        room = self.ctxs[0].cache.max_pages * PAGE - lens
+        fits = (tree_lens >= 0) & (tree_lens <= nodes) & ((tree_lens == 0) | (lens >= 0) & (tree_lens <= room))
+        status.copy_(torch.where((status == 0) & ~fits.all(), _lib.HA_ERR_BAD_SEQ_LEN, status))
+        return torch.where(fits, tree_lens, 0)
 
     def _tree_forward(self, draft, mask, tree_lens):
         """Appends the drafts to every layer's cache (lengths and key hashes included) -> (logits [B, T, vocab], the layers'
@@ -280,7 +290,8 @@ class TPLlama:
         are shorter than T. One pass with full attention over the cache, greedy acceptance, and the accepted path stays in the
         cache: positions and lengths advance by ``count``, ``next_token`` is the next round's node 0 (or the next
         :meth:`decode_step`'s token; where a sequence has no drafts, ``draft[:, 0]`` still is). With node 0 alone this is a
-        dense decode step. Nothing synchronises with the host."""
+        dense decode step. A sequence whose drafts do not fit its cache (:meth:`evict` makes room) is left as it is, with a
+        ``count`` of 0, and reported to :meth:`check_status`. Nothing synchronises with the host."""
         if self.trees is None or draft.dim() != 2 or not 1 <= draft.shape[1] <= self.trees[0].max_nodes:
             raise ValueError("verify_tree needs enable_trees(max_nodes) and a draft of [batch, 1 .. max_nodes] tokens")
         _check(draft, "draft", torch.int64, (self.batch, draft.shape[1]), self.trees[0].device)
@@ -288,6 +299,8 @@ class TPLlama:
         status = self.trees[0].status
         if tree_lens is None:
             tree_lens = torch.full((self.batch,), draft.shape[1], dtype=torch.int32, device=self.device)
+        _check(tree_lens, "tree_lens", torch.int32, (self.batch,), self.trees[0].device)
+        tree_lens = self._fitting_trees(tree_lens, draft.shape[1])
         mask = tree_mask(parents, tree_lens, status=status)
         logits, kept = self._tree_forward(draft, mask, tree_lens)
         got = TreeAccept.empty(self.batch, draft.device)

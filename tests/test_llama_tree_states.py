@@ -51,6 +51,72 @@ def _chain(B, T, device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("full", [768, 767, 761])
+def test_drafts_that_do_not_fit_are_reported_and_change_nothing(device, full):
+    """8 drafts behind 761 and more of 768 tokens: that sequence takes no part in the round and can be evicted and go on; the
+    sequence beside it gives, bit by bit, what it gives where the full one has no drafts."""
+    from hashattention_b200 import _lib
+    T = 8
+    draft = torch.randint(0, 1000, (2, T), generator=torch.Generator().manual_seed(2)).to(device)
+    results = []
+    for tree_lens in ([T, T], [0, T]):
+        model = _model(device, 2, T, mass=True, init_budget=16, recent_budget=16)
+        _prefilled(model, [full, 300])
+        for m in model.mass:
+            m.copy_(torch.rand(m.shape, generator=torch.Generator().manual_seed(6)))
+        before = _state(model)
+        got = model.verify_tree(draft, _chain(2, T, device), torch.tensor(tree_lens, dtype=torch.int32, device=device))
+        results.append((got, _state(model), model.ctxs[0].cache.page_table[1].long()))
+        if tree_lens[0]:
+            with pytest.raises(RuntimeError, match=rf"status {_lib.HA_ERR_BAD_SEQ_LEN}\)"):
+                model.check_status()
+            _assert_left_alone(model, before, 0)
+            assert int(got.count[0]) == 0 and not bool(got.accepted[0].any()) and int(got.seq_lens[0]) == full
+            assert int(got.next_token[0]) == int(draft[0, 0])  # still the token that is certain
+            # after an eviction the same drafts fit
+            model.evict(400)
+            assert model.seq_lens.tolist()[0] == 400
+            again = model.verify_tree(draft, _chain(2, T, device))
+            model.check_status()
+            assert int(again.count[0]) >= 1 and int(model.pos[0]) == full + int(again.count[0])
+        else:
+            model.check_status()
+    (a, sa, own), (b, sb, _) = results
+    assert torch.equal(a.accepted[1], b.accepted[1]) and int(a.next_token[1]) == int(b.next_token[1])
+    assert sa["lens"][1] == sb["lens"][1] == 300 + int(a.count[1]) and sa["pos"][1] == sb["pos"][1]
+    for p, q in zip(sa["pools"], sb["pools"]):
+        for s, t in zip(p, q):
+            assert torch.equal(s[own], t[own])
+
+
+@pytest.mark.gpu
+def test_drafts_that_just_fit_are_taken(device):
+    model = _model(device, 1, 8)
+    _prefilled(model, [760])
+    got = model.verify_tree(torch.zeros(1, 8, dtype=torch.int64, device=device), _chain(1, 8, device))
+    model.check_status()
+    assert int(got.count[0]) >= 1 and model.seq_lens.tolist() == [760 + int(got.count[0])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [9, -1, 2 ** 31 - 1])
+def test_tree_lens_out_of_range_are_reported_and_change_nothing(device, bad):
+    from hashattention_b200 import _lib
+    model = _model(device, 2, 8, mass=True)
+    _prefilled(model, [300, 300])
+    before = _state(model)
+    draft = torch.randint(0, 1000, (2, 8), generator=torch.Generator().manual_seed(2)).to(device)
+    got = model.verify_tree(draft, _chain(2, 8, device), torch.tensor([bad, 5], dtype=torch.int32, device=device))
+    with pytest.raises(RuntimeError, match=rf"status {_lib.HA_ERR_BAD_SEQ_LEN}\)"):
+        model.check_status()
+    _assert_left_alone(model, before, 0)
+    assert got.count.tolist()[0] == 0 and int(got.next_token[0]) == int(draft[0, 0])
+    assert int(got.count[1]) >= 1 and model.seq_lens.tolist() == [300, 300 + int(got.count[1])]
+    with pytest.raises(ValueError, match="tree_lens"):
+        model.verify_tree(draft, _chain(2, 8, device), torch.ones(2, dtype=torch.int64, device=device))
+
+
+@pytest.mark.gpu
 def test_next_token_of_a_sequence_without_drafts(device):
     """Where nothing was drafted there is no token behind the last accepted one: node 0's stays the next one in a model's round (the
     embedding takes it), and acceptance by itself gives 0 in tensors of its own and leaves given ones alone."""
