@@ -284,12 +284,20 @@ class DenseDecodeContext:
         _raise_on(rc, "ha_attention_mass")
         return mass
 
-    def tree_commit(self, accepted, tree_lens=None, mass: torch.Tensor | None = None) -> None:
+    def tree_commit(self, accepted, tree_lens=None, mass: torch.Tensor | None = None, max_nodes: int | None = None) -> None:
         """``ha_tree_commit``: moves the rows of the ``accepted [B, 4]`` nodes (K, V, codes, and ``mass``) to the front of
         the drafts. ``cache.seq_lens`` still counts all drafts and is left alone: copy ``TreeAccept.seq_lens`` into it when
-        every layer has been committed. ``tree_lens`` as in :meth:`tree_attention` (``None``: ``max_nodes`` of each)."""
+        every layer has been committed. ``tree_lens`` as in :meth:`tree_attention`; where it is ``None``, ``max_nodes`` says how
+        many drafts each sequence has (the ``T`` of the round's other calls, which nothing given here tells; a context for one
+        node knows)."""
         _check(accepted, "accepted", torch.int32, (self.batch, MASK_WORDS), self.device)
-        tree = self._tree_struct(self.max_nodes, None, tree_lens)
+        if max_nodes is None:
+            if tree_lens is None and self.max_nodes > 1:
+                raise ValueError("tree_commit needs tree_lens, or max_nodes = the drafts of each sequence in this round")
+            max_nodes = self.max_nodes
+        elif not 1 <= max_nodes <= self.max_nodes:
+            raise ValueError(f"max_nodes must be in 1 .. {self.max_nodes}, got {max_nodes}")
+        tree = self._tree_struct(int(max_nodes), None, tree_lens)
         if mass is not None:
             self._check_mass(mass)
         c = self.cache

@@ -56,3 +56,41 @@ def test_commit_writes_nothing_where_a_page_id_is_out_of_range(device, bad, whic
         want[:, P:P + 3] = flat_was[:, [P + 1, P + 3, P + 7]]
         assert torch.equal(flat_now, want)
     assert torch.equal(mass[0], old[0]), "the received weights moved without their rows"
+
+
+@pytest.mark.gpu
+def test_commit_without_tree_lens_needs_the_nodes_of_the_round(device):
+    """A context for 32 nodes in a round of 8 without tree_lens: attention and acceptance go by the round's width, and so does the
+    commit, which cannot know it from the words of the accepted path."""
+    T, S = 8, 300
+    x = Problem(device, [S, 200], [T, T], 2, T, "tree", seed=3)
+    ctx = ha.DenseDecodeContext(x.cache, 32)
+    out, lse = ctx.tree_attention(x.q, x.mask)
+    x.check(out, lse)
+    bits = torch.zeros(2, 128, dtype=torch.bool)
+    bits[0, [0, 2, 5]] = bits[1, [0, 7]] = True
+    words, mass = ha.pack_nodes(bits).to(device), torch.rand(ctx.mass_shape, device=device)
+    before, old = [flat_rows(x.cache, b) for b in range(2)], mass.clone()
+    with pytest.raises(ValueError, match="max_nodes"):
+        ctx.tree_commit(words, mass=mass)
+    for bad in (0, 33, -1):
+        with pytest.raises(ValueError, match="max_nodes"):
+            ctx.tree_commit(words, mass=mass, max_nodes=bad)
+    ctx.tree_commit(words, mass=mass, max_nodes=T)
+    ctx.check_status()
+    for b, path in enumerate(([0, 2, 5], [0, 7])):
+        P = x.lens[b] - T
+        path = torch.tensor(path, device=device)
+        for was, now in zip(before[b], flat_rows(x.cache, b)):
+            want = was.clone()
+            want[:, P:P + len(path)] = was[:, P + path]
+            kind = torch.int16 if now.dtype == torch.bfloat16 else torch.int32
+            assert torch.equal(now.view(kind), want.view(kind))
+        want = old[b].clone()
+        want[:, P:P + len(path)] = old[b][:, P + path]
+        want[:, P + len(path):P + T] = 0
+        assert torch.equal(mass[b], want)
+    # a context for one node has one width only
+    one = ha.DenseDecodeContext(x.cache, 1)
+    one.tree_commit(torch.ones(2, 4, dtype=torch.int32, device=device))
+    one.check_status()
