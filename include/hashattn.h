@@ -397,8 +397,9 @@ int ha_tree_commit(const ha_shape_t* shape, const ha_tree_t* tree, const uint32_
  * recent_budget and, of those in between, the ones with the largest mass (ties: the lowest token; negative values and NaN
  * count as 0), in their order. K, V and code rows (hash_pages, optional) move in place. kept [batch][num_kv_heads]
  * [keep_tokens] <- the former token numbers (entries behind a shorter sequence's end are left as they were); mass_out
- * (optional, not mass) <- the kept tokens' mass, zeros behind; lens_out (not seq_lens) <- the new lengths. Rotary positions are
- * in the keys already: later tokens keep counting from the former length.                                            */
+ * (optional, not mass) <- the kept tokens' mass, zeros behind; lens_out (not seq_lens) <- the new lengths. A sequence whose length
+ * is out of range passes its length and its whole row of mass on as they are. Rotary positions are in the keys already: later
+ * tokens keep counting from the former length.                                                                       */
 int ha_cache_evict(const ha_shape_t* shape, int32_t keep_tokens, int32_t init_budget, int32_t recent_budget,
                    const float* mass, void* k_pages, void* v_pages, uint32_t* hash_pages, const int32_t* page_table,
                    const int32_t* seq_lens, int32_t* kept, float* mass_out, int32_t* lens_out,

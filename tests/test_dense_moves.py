@@ -94,3 +94,21 @@ def test_commit_without_tree_lens_needs_the_nodes_of_the_round(device):
     one = ha.DenseDecodeContext(x.cache, 1)
     one.tree_commit(torch.ones(2, 4, dtype=torch.int32, device=device))
     one.check_status()
+
+
+@pytest.mark.gpu
+def test_eviction_keeps_the_weights_of_a_sequence_whose_length_is_out_of_range(device):
+    x = Problem(device, [700, 300, 500], [0, 0, 0], 2, 1, seed=2)
+    mass = torch.rand(x.ctx.mass_shape, device=device)
+    for bad in (10 ** 9, -5):
+        x.cache.seq_lens[1] = bad
+        before = pools(x.cache)
+        kept, mass_out, lens = x.ctx.cache_evict(mass, 600, 4, 4)  # (the others: one is cut, one is not)
+        with pytest.raises(RuntimeError, match=rf"status {_lib.HA_ERR_BAD_SEQ_LEN}\)"):
+            x.ctx.check_status()
+        assert lens.tolist() == [600, bad, 500] and bool((kept[1] == -1).all())
+        assert torch.equal(mass_out[1], mass[1])
+        assert torch.equal(mass_out[2, :, :500], mass[2, :, :500]) and bool((mass_out[2, :, 500:] == 0).all())
+        own = x.cache.page_table[1].tolist()
+        for was, now in zip(before, pools(x.cache)):
+            assert torch.equal(now[own], was[own])
