@@ -23,6 +23,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import threading
 from dataclasses import dataclass
 
 import torch
@@ -152,7 +153,8 @@ class DenseDecodeContext:
     """Dense attention over one layer's paged cache for up to ``max_nodes`` new tokens per sequence (a tree of drafts; one
     token: the dense decode step), with its workspace. Creating it allocates; the calls do not, but for outputs that the
     caller leaves out. One context per call that may run at the same time; contexts whose calls follow one another on a stream
-    (the layers of a model) may share the workspaces of the first of them (``workspace_of``)."""
+    (the layers of a model) may share the workspaces of the first of them (``workspace_of``). Python threads may enqueue through
+    one context, or through contexts that share workspaces: their calls take turns, on a stream that they have to share too."""
 
     def __init__(self, cache: PagedHashKVCache, max_nodes: int = 1, sm_scale: float | None = None,
                  workspace_of: "DenseDecodeContext | None" = None):
@@ -184,6 +186,9 @@ class DenseDecodeContext:
             if o.device != self.device or o.workspace_bytes < self.workspace_bytes or o.evict_workspace_bytes < self.evict_workspace_bytes:
                 raise ValueError("workspace_of must be a context on the same device with workspaces at least as large")
             self.workspace, self.evict_workspace = o.workspace, o.evict_workspace
+        # A call fills in the context's structs and launches two kernels that meet in the workspace, while the interpreter runs
+        # other threads: whole calls take turns.
+        self._turn = threading.Lock() if workspace_of is None else workspace_of._turn
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         # (the context's own buffers, which stay where they are as long as it lives)
         self._workspace_ptr, self._evict_workspace_ptr, self._status_ptr = (
@@ -246,23 +251,24 @@ class DenseDecodeContext:
         ``tree_mask`` lets each node see (``None``: a chain). ``tree_lens [B]``: drafted tokens of each sequence, the
         last ones of ``cache.seq_lens`` (``None``: T of each); rows behind them are left as they were (zeros, where the
         outputs are not given). Returns ``out [B, T, Hq, 128]`` bf16 and ``lse [B, T, Hq]`` f32 (natural logarithm)."""
-        T, tree, strides = self._tree(q, tree_mask, tree_lens)
-        make = torch.zeros if tree_lens is not None else torch.empty
-        size = (self.batch, T, self.num_q_heads)
-        if out is None:
-            out = make(*size, HEAD_DIM, dtype=torch.bfloat16, device=self.device)
-        else:
-            _check(out, "out", torch.bfloat16, (*size, HEAD_DIM), self.device)
-        if lse is None:
-            lse = make(*size, dtype=torch.float32, device=self.device)
-        else:
-            _check(lse, "lse", torch.float32, size, self.device)
-        c = self.cache
-        with library_call(self.device, "ha_tree_attention"):
-            rc = self.lib.ha_tree_attention(
-                self._shape_ref, tree, q.data_ptr(), strides, c.k_pages.data_ptr(), c.v_pages.data_ptr(), c.page_table.data_ptr(),
-                c.seq_lens.data_ptr(), self.sm_scale, out.data_ptr(), lse.data_ptr(), self._workspace_ptr,
-                self.workspace_bytes, self._status_ptr, _stream_ptr(self.device))
+        with self._turn:
+            T, tree, strides = self._tree(q, tree_mask, tree_lens)
+            make = torch.zeros if tree_lens is not None else torch.empty
+            size = (self.batch, T, self.num_q_heads)
+            if out is None:
+                out = make(*size, HEAD_DIM, dtype=torch.bfloat16, device=self.device)
+            else:
+                _check(out, "out", torch.bfloat16, (*size, HEAD_DIM), self.device)
+            if lse is None:
+                lse = make(*size, dtype=torch.float32, device=self.device)
+            else:
+                _check(lse, "lse", torch.float32, size, self.device)
+            c = self.cache
+            with library_call(self.device, "ha_tree_attention"):
+                rc = self.lib.ha_tree_attention(
+                    self._shape_ref, tree, q.data_ptr(), strides, c.k_pages.data_ptr(), c.v_pages.data_ptr(), c.page_table.data_ptr(),
+                    c.seq_lens.data_ptr(), self.sm_scale, out.data_ptr(), lse.data_ptr(), self._workspace_ptr,
+                    self.workspace_bytes, self._status_ptr, _stream_ptr(self.device))
         _raise_on(rc, "ha_tree_attention")
         return out, lse
 
@@ -270,17 +276,18 @@ class DenseDecodeContext:
         """``ha_attention_mass``: adds to ``mass`` (:attr:`mass_shape`, f32) the attention weight each cached token has in
         the rows of ``q``, given the ``lse`` that :meth:`tree_attention` returned for them. ``rows [B, 4]`` int32: the
         nodes whose weights count (``TreeAccept.accepted``; ``None``: all)."""
-        T, tree, strides = self._tree(q, tree_mask, tree_lens)
-        _check(lse, "lse", torch.float32, (self.batch, T, self.num_q_heads), self.device)
-        self._check_mass(mass)
-        if rows is not None:
-            _check(rows, "rows", torch.int32, (self.batch, MASK_WORDS), self.device)
-        c = self.cache
-        with library_call(self.device, "ha_attention_mass"):
-            rc = self.lib.ha_attention_mass(
-                self._shape_ref, tree, q.data_ptr(), strides, lse.data_ptr(), rows.data_ptr() if rows is not None else None,
-                c.k_pages.data_ptr(), c.page_table.data_ptr(), c.seq_lens.data_ptr(), self.sm_scale, mass.data_ptr(),
-                self._status_ptr, _stream_ptr(self.device))
+        with self._turn:
+            T, tree, strides = self._tree(q, tree_mask, tree_lens)
+            _check(lse, "lse", torch.float32, (self.batch, T, self.num_q_heads), self.device)
+            self._check_mass(mass)
+            if rows is not None:
+                _check(rows, "rows", torch.int32, (self.batch, MASK_WORDS), self.device)
+            c = self.cache
+            with library_call(self.device, "ha_attention_mass"):
+                rc = self.lib.ha_attention_mass(
+                    self._shape_ref, tree, q.data_ptr(), strides, lse.data_ptr(), rows.data_ptr() if rows is not None else None,
+                    c.k_pages.data_ptr(), c.page_table.data_ptr(), c.seq_lens.data_ptr(), self.sm_scale, mass.data_ptr(),
+                    self._status_ptr, _stream_ptr(self.device))
         _raise_on(rc, "ha_attention_mass")
         return mass
 
@@ -297,15 +304,16 @@ class DenseDecodeContext:
             max_nodes = self.max_nodes
         elif not 1 <= max_nodes <= self.max_nodes:
             raise ValueError(f"max_nodes must be in 1 .. {self.max_nodes}, got {max_nodes}")
-        tree = self._tree_struct(int(max_nodes), None, tree_lens)
-        if mass is not None:
-            self._check_mass(mass)
-        c = self.cache
-        with library_call(self.device, "ha_tree_commit"):
-            rc = self.lib.ha_tree_commit(
-                self._shape_ref, tree, accepted.data_ptr(), c.k_pages.data_ptr(), c.v_pages.data_ptr(), c.hash_pages.data_ptr(),
-                c.page_table.data_ptr(), c.seq_lens.data_ptr(), mass.data_ptr() if mass is not None else None,
-                self._status_ptr, _stream_ptr(self.device))
+        with self._turn:
+            tree = self._tree_struct(int(max_nodes), None, tree_lens)
+            if mass is not None:
+                self._check_mass(mass)
+            c = self.cache
+            with library_call(self.device, "ha_tree_commit"):
+                rc = self.lib.ha_tree_commit(
+                    self._shape_ref, tree, accepted.data_ptr(), c.k_pages.data_ptr(), c.v_pages.data_ptr(), c.hash_pages.data_ptr(),
+                    c.page_table.data_ptr(), c.seq_lens.data_ptr(), mass.data_ptr() if mass is not None else None,
+                    self._status_ptr, _stream_ptr(self.device))
         _raise_on(rc, "ha_tree_commit")
 
     def cache_evict(self, mass, keep_tokens: int, init_budget: int = 128, recent_budget: int = 128,
@@ -330,7 +338,7 @@ class DenseDecodeContext:
         _check(lens_out, "lens_out", torch.int32, (self.batch,), self.device)
         if mass_out.data_ptr() == mass.data_ptr() or lens_out.data_ptr() == c.seq_lens.data_ptr():
             raise ValueError("mass_out and lens_out must be other tensors than mass and cache.seq_lens")
-        with library_call(self.device, "ha_cache_evict"):
+        with self._turn, library_call(self.device, "ha_cache_evict"):
             rc = self.lib.ha_cache_evict(
                 self._shape_ref, keep_tokens, init_budget, recent_budget, mass.data_ptr(), c.k_pages.data_ptr(), c.v_pages.data_ptr(),
                 c.hash_pages.data_ptr(), c.page_table.data_ptr(), c.seq_lens.data_ptr(), kept.data_ptr(), mass_out.data_ptr(),
