@@ -11,7 +11,7 @@
 //
 // Roles of the warps: 0 issues the products, 1 loads K and V tiles by TMA (two boxes of 64 elements x 128 tokens, 128-byte
 // swizzle) into a ring of 32 KB slots, K and V of a tile in turn, 2 - 17 are the softmax warps, eight per stream: a thread has 64 of
-// a row's 128 columns, and the two halves of a row agree on its maximum, to 16 bits of mantissa, through shared memory. Streams that take
+// a row's 128 columns, and the two halves of a row agree on its maximum through shared memory. Streams that take
 // different tiles have a ring of three slots each, streams that share tiles a ring of five; a barrier is waited for in every
 // phase by the one who uses it.
 //
@@ -63,12 +63,12 @@ struct TaLayout {
     static constexpr int kBarQ = kBarO + 2;                // 16 warps: the unit's queries are in place, the last unit's results read
     static constexpr int kBarFinal = kBarQ + 1;            // commit: every product of the CTA is complete
     static constexpr int kBars = kBarFinal + 1;
-    static constexpr uint32_t kOffMax = kOffRing + kRings * kSlots * kTaSlot;  // [2 streams][2 halves][128] maxima of half rows: the upper 16 bits
-    static constexpr uint32_t kOffMaxLow = kOffMax + 2 * 2 * 128 * 2;          // ... and the next 8 (a whole word each has no room)
-    static constexpr uint32_t kOffBar = kOffMaxLow + 2 * 2 * 128;
+    static constexpr uint32_t kOffMax = kOffRing + kRings * kSlots * kTaSlot;  // [2 streams][2 halves][128] floats: maxima of half rows
+    static constexpr uint32_t kOffBar = kOffMax + 2 * 2 * 128 * 4;
     static constexpr uint32_t kOffTmem = kOffBar + kBars * 8;     // tmem base, abort flag
     static constexpr uint32_t kOffBad = (kOffTmem + 8 + 15) / 16 * 16;  // [4] nodes with an infinity or NaN in V
-    static constexpr uint32_t kSmemBytes = kOffBad + 16 + 1024;   // + slack to align the base to 1024 B
+    static constexpr uint32_t kAlign = 256;                       // of the array as declared
+    static constexpr uint32_t kSmemBytes = kOffBad + 16 + 1024 - kAlign;  // + slack to align the base to 1024 B
     static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
 };
 
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
 tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     using L = TaLayout<kWide>;
     using Cursor = DenseCursor<kTaTile, L::kRows, L::kCross>;
-    extern __shared__ unsigned char ta_smem_raw[];
+    extern __shared__ __align__(L::kAlign) unsigned char ta_smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ta_smem_raw) + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t sbase = tc_smem_u32(smem), bars = sbase + L::kOffBar;
@@ -236,8 +236,7 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
         const int t_all = tid - kTaSoftWarp0 * 32, t_stream = t_all & 255;
         const uint32_t t_lane = tmem + ((uint32_t)quarter << 21), t_s = t_lane + 128u * (uint32_t)w + 64u * (uint32_t)half;
         const uint32_t t_o = t_lane + 256u + 128u * (uint32_t)w + 64u * (uint32_t)half;
-        uint16_t* s_max = reinterpret_cast<uint16_t*>(smem + L::kOffMax) + (size_t)w * 256;
-        uint8_t* s_max_low = smem + L::kOffMaxLow + (size_t)w * 256;
+        float* s_max = reinterpret_cast<float*>(smem + L::kOffMax) + w * 256;
         const unsigned char* ring_mem = smem + L::kOffRing + (size_t)(ring * L::kSlots) * kTaSlot;
         uint32_t use = 0, tiles = 0, seg_o = 0;
         const f32x2 scale2 = pack2(p.scale_log2, p.scale_log2);
@@ -349,14 +348,12 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
                 largest(sc);
                 largest(sd);
                 tc_ld16_issue(t_s + 16u, sb);
-                // The maximum of the row, as both halves know it: a reference for the exponents, whose cut to 24 bits does not matter as
-                // long as it leaves 2^(x - reference) in range (2^-16 of x, where bf16 alone took 2^9 off a score of 2^18).
-                const uint32_t mine_max = __float_as_uint(fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * p.scale_log2) & 0xffffff00u;
-                s_max[half * 128 + r] = (uint16_t)(mine_max >> 16);
-                s_max_low[half * 128 + r] = (uint8_t)(mine_max >> 8);
+                // The maximum of the row, from both halves: the reference of its exponents, to the last bit (2^-16 of it less, and the
+                // weights of a score of 2^24 pass 2^128).
+                const float mine_max = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * p.scale_log2;
+                s_max[half * 128 + r] = mine_max;
                 asm volatile("bar.sync %0, 64;" ::"r"(2 + 4 * w + quarter) : "memory");
-                const int other = (half ^ 1) * 128 + r;
-                const float x = fmaxf(__uint_as_float(mine_max), __uint_as_float((uint32_t)s_max[other] << 16 | (uint32_t)s_max_low[other] << 8));
+                const float x = fmaxf(mine_max, s_max[(half ^ 1) * 128 + r]);
                 if (!ok) continue;
                 const bool grow = x > m + kRescaleAt;  // (from -inf: any score at all)
                 if (__any_sync(0xffffffffu, grow)) {

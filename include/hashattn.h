@@ -359,6 +359,7 @@ int ha_tree_mask(const int32_t* parents, const int32_t* tree_lens, int32_t batch
 /* out[b][i][h] = softmax(sm_scale * q[b][i][h] . K) V over the prefix and the nodes that node i sees, fp32 sums, bf16 output;
  * lse (optional) [batch][max_nodes][num_q_heads] f32: the natural log of the sum of e^(scaled scores). Rows of nodes behind
  * a tree's own are left as they were. A row that sees nothing (or only scores of -inf) gives zeros and an lse of -inf.
+ * Scaled scores of magnitudes up to 2^29 (beyond, half an ulp of one is more than fp32 has exponents for).
  * q [batch][max_nodes][num_q_heads][128] bf16 with strides q_strides[3] = {batch, node, head} in elements (HOST array;
  * multiples of 8, the 128 elements of a row contiguous), or contiguous if NULL: a view of a fused projection will do.
  * out is contiguous. sm_scale > 0.                                                                                  */
@@ -370,7 +371,8 @@ int ha_tree_attention(const ha_shape_t* shape, const ha_tree_t* tree, const void
 /* mass[b][j][t] += sum over the counted nodes i and the query heads h of kv-head j of the weight e^(score - lse[b][i][h])
  * that cached token t has in row (i, h); mass [batch][num_kv_heads][max_pages * page_size] f32. rows (optional) [batch][4]:
  * the nodes whose weights count, one bit each (an accepted path); NULL: all of the tree. q, q_strides, sm_scale, the tree
- * and lse as ha_tree_attention took and left them. Rows with an lse of -inf count for nothing.                      */
+ * and lse as ha_tree_attention took and left them. Rows with an lse of -inf count for nothing. A weight is off by what the
+ * rounding of score and lse to fp32 makes of it: about 2^-23 of their magnitude, relative to the weight.                */
 int ha_attention_mass(const ha_shape_t* shape, const ha_tree_t* tree, const void* q, const int64_t* q_strides,
                       const float* lse, const uint32_t* rows, const void* k_pages, const int32_t* page_table,
                       const int32_t* seq_lens, float sm_scale, float* mass, int32_t* status, void* stream);
