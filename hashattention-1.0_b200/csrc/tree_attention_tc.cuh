@@ -446,39 +446,41 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
                     if (second) tc_ld16_issue(t_lane + 384u + 16 * q, o1);
                     tc_ld16_wait(o0);
                     if (second) tc_ld16_wait(o1);
-                    if (!mine) continue;
-                    float acc[16];
+                    if (mine) {
+                        float acc[16];
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        acc[k] = __uint_as_float(o0[k]) * f0;
-                        if (second) acc[k] = fmaf(__uint_as_float(o1[k]), f1, acc[k]);
-                    }
-                    if (bad != 0) {
-                        const __nv_bfloat16* qr = p.q + seg.b * p.q_batch + (long long)node * p.q_node + (seg.kvh * kGroup + (r & 3)) * p.q_head;
-                        for (int t = 0; t < seg.n; ++t) {
-                            if (((s_bad[t >> 5] >> (t & 31)) & 1u) == 0 || !dense_bit(mask, t)) continue;
-                            const int j = P + t;
-                            const size_t at = (((size_t)dense_page(p.seqs, seg.b, j / kPage) * p.seqs.Hkv + seg.kvh) * kPage + j % kPage) * kHeadDim;
-                            float dot = 0.0f;
-                            for (int d = 0; d < kHeadDim; ++d) dot = fmaf(__bfloat162float(qr[d]), __bfloat162float(p.k_pages[at + d]), dot);
-                            const float e = exp2_approx(fmaf(dot, p.scale_log2, M == -INFINITY ? 0.0f : -M));
+                        for (int k = 0; k < 16; ++k) {
+                            acc[k] = __uint_as_float(o0[k]) * f0;
+                            if (second) acc[k] = fmaf(__uint_as_float(o1[k]), f1, acc[k]);
+                        }
+                        if (bad != 0) {
+                            const __nv_bfloat16* qr = p.q + seg.b * p.q_batch + (long long)node * p.q_node + (seg.kvh * kGroup + (r & 3)) * p.q_head;
+                            for (int t = 0; t < seg.n; ++t) {
+                                if (((s_bad[t >> 5] >> (t & 31)) & 1u) == 0 || !dense_bit(mask, t)) continue;
+                                const int j = P + t;
+                                const size_t at = (((size_t)dense_page(p.seqs, seg.b, j / kPage) * p.seqs.Hkv + seg.kvh) * kPage + j % kPage) * kHeadDim;
+                                float dot = 0.0f;
+                                for (int d = 0; d < kHeadDim; ++d) dot = fmaf(__bfloat162float(qr[d]), __bfloat162float(p.k_pages[at + d]), dot);
+                                const float e = exp2_approx(fmaf(dot, p.scale_log2, M == -INFINITY ? 0.0f : -M));
 #pragma unroll
-                            for (int k = 0; k < 16; ++k) acc[k] = fmaf(e, __bfloat162float(p.v_pages[at + 16 * q + k]), acc[k]);
+                                for (int k = 0; k < 16; ++k) acc[k] = fmaf(e, __bfloat162float(p.v_pages[at + 16 * q + k]), acc[k]);
+                            }
+                        }
+                        if (seg.whole()) {
+                            uint32_t words[8];
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) words[k] = tc_pack_bf16(acc[2 * k] * inv, acc[2 * k + 1] * inv);
+                            uint4* dst = reinterpret_cast<uint4*>(p.out + out_row * kHeadDim + 16 * q);
+                            dst[0] = make_uint4(words[0], words[1], words[2], words[3]);
+                            dst[1] = make_uint4(words[4], words[5], words[6], words[7]);
+                        } else {
+                            // [slot][dimensions / 4][row]: a warp's rows side by side
+                            float4* dst = reinterpret_cast<float4*>(p.part_acc) + ((size_t)(2 * blockIdx.x + seg.slot) * (kHeadDim / 4) + 4 * q) * L::kRows + row_in;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) dst[(size_t)k * L::kRows] = make_float4(acc[4 * k], acc[4 * k + 1], acc[4 * k + 2], acc[4 * k + 3]);
                         }
                     }
-                    if (seg.whole()) {
-                        uint32_t words[8];
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) words[k] = tc_pack_bf16(acc[2 * k] * inv, acc[2 * k + 1] * inv);
-                        uint4* dst = reinterpret_cast<uint4*>(p.out + out_row * kHeadDim + 16 * q);
-                        dst[0] = make_uint4(words[0], words[1], words[2], words[3]);
-                        dst[1] = make_uint4(words[4], words[5], words[6], words[7]);
-                    } else {
-                        // [slot][dimensions / 4][row]: a warp's rows side by side
-                        float4* dst = reinterpret_cast<float4*>(p.part_acc) + ((size_t)(2 * blockIdx.x + seg.slot) * (kHeadDim / 4) + 4 * q) * L::kRows + row_in;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) dst[(size_t)k * L::kRows] = make_float4(acc[4 * k], acc[4 * k + 1], acc[4 * k + 2], acc[4 * k + 3]);
-                    }
+                    __syncwarp();  // (the next piece is read by all lanes together)
                 }
                 if (mine && (kWide ? half : group) == 0) {
                     if (!seg.whole()) p.part_ml[(size_t)(2 * blockIdx.x + seg.slot) * L::kRows + row_in] = make_float2(M, sum);
