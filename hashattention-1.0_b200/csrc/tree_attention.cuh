@@ -17,7 +17,10 @@
 // sums are fp32 and do not mind, and rescaling 16 x 128 of them at every new maximum would.
 //
 // Tokens that a row does not see are taken out by selection, not by a weight of zero: an infinity or NaN in the K or V of a
-// token that only other branches of the tree see stays with those.
+// token that only other branches of the tree see stays with those. An infinity in a V row that a row does see is NaN in the products
+// (the lo half of its weight is negative or zero as often as not), where the average, whose weights are above zero, is
+// infinite. So a channel that came out NaN is looked up at the end, in the V rows themselves (v_classes): its average is
+// NaN if one of them is or if both infinities are among them. That reads V again, but only then.
 #pragma once
 
 #include "dense_common.cuh"
@@ -77,6 +80,34 @@ __device__ __forceinline__ bool any_nonfinite(uint4 w) {
     auto bad = [](uint32_t x) { return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u; };
     return bad(w.x) || bad(w.y) || bad(w.z) || bad(w.w);
 }
+
+// What a value makes of an average with weights above zero, as bits that add up by OR: 1 it is +inf or NaN, 2 it is -inf or NaN.
+__device__ __forceinline__ uint32_t value_class(float v) { return v != v ? 3u : (v == INFINITY ? 1u : (v == -INFINITY ? 2u : 0u)); }
+__device__ __forceinline__ float class_value(uint32_t c, float finite) {
+    return c == 0 ? finite : (c == 1 ? INFINITY : (c == 2 ? -INFINITY : __uint_as_float(0x7fffffffu)));
+}
+// The classes of the channels 16 q .. 16 q + 15 of V over the tokens [t0, t1) of a sequence (table: its row of the page table), by a
+// whole warp, a token per lane: bit k of the lower half and bit k of the upper half.
+__device__ __noinline__ uint32_t v_classes(const __nv_bfloat16* v_pages, const int32_t* table, int num_pages, int Hkv, int kvh, int t0, int t1, int q) {
+    uint32_t found = 0;
+#pragma unroll 4
+    for (int t = t0 + (int)(threadIdx.x & 31); t < t1; t += 32) {
+        int page = __ldg(table + t / kPage);
+        if (page < 0 || page >= num_pages) page = 0;  // (reported by the loading warp, which took the same)
+        const uint4* row = reinterpret_cast<const uint4*>(v_pages + (((size_t)page * Hkv + kvh) * kPage + t % kPage) * kHeadDim) + 2 * q;
+        const uint4 a = __ldg(row), b = __ldg(row + 1);
+        if (any_nonfinite(a) || any_nonfinite(b)) {
+            const uint32_t words[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t lo = value_class(bf16_lo(words[k])), hi = value_class(bf16_hi(words[k]));
+                found |= ((lo & 1u) | (hi & 1u) << 1) << (2 * k) | ((lo >> 1) | (hi >> 1) << 1) << (2 * k + 16);
+            }
+        }
+    }
+    return __reduce_or_sync(0xffffffffu, found);
+}
+__device__ __forceinline__ uint32_t class_of(uint32_t classes, int k) { return ((classes >> k) & 1u) | ((classes >> (16 + k)) & 1u) << 1; }
 
 // Natural log-sum-exp of a row from its maximum (in powers of two, a score as the products gave it) and sum.
 __device__ __forceinline__ float natural_lse(float M, float sum) {
@@ -342,6 +373,8 @@ tree_attention_rows_kernel(const TreeAttentionParams p, const __grid_constant__ 
             }
         asm volatile("bar.sync 1, %0;" ::"n"(kRowsWarps * 32) : "memory");
         const int rows = min(L::kRows, seg.n * kGroup - row0);
+        bool looked_up = false;  // what the prefix's V rows hold beside numbers, for a row that comes out NaN
+        uint32_t prefix_classes = 0;
         for (int r = warp; r < rows; r += kRowsWarps) {
             float2 ml[kRowsWarps];
             float M = -INFINITY, sum = 0.0f;
@@ -359,6 +392,27 @@ tree_attention_rows_kernel(const TreeAttentionParams p, const __grid_constant__ 
                 sum = fmaf(ml[w].y, f, sum);
                 acc.x = fmaf(a.x, f, acc.x); acc.y = fmaf(a.y, f, acc.y);
                 acc.z = fmaf(a.z, f, acc.z); acc.w = fmaf(a.w, f, acc.w);
+            }
+            if (__any_sync(0xffffffffu, !(acc.x == acc.x && acc.y == acc.y && acc.z == acc.z && acc.w == acc.w)) && sum >= 0.0f) {
+                // (with a sum of NaN the row is NaN; a sum of 0: scores of -inf only)
+                auto classes = [&](int t0, int t1) {  // of the lane's four channels
+                    uint32_t mine = 0;
+                    for (int q = 0; q < 8; ++q) {
+                        const uint32_t c = v_classes(p.v_pages, p.seqs.page_table + (size_t)seg.b * p.seqs.max_pages, p.seqs.num_pages, p.seqs.Hkv, seg.kvh, t0, t1, q);
+                        if (q == lane >> 2) mine = c >> (4 * (lane & 3));
+                    }
+                    return mine;
+                };
+                const int t0 = seg.tile0 * kRowsTile, t1 = min(seg.S, seg.tile1 * kRowsTile);
+                if (!looked_up) prefix_classes = classes(t0, min(P, t1));
+                looked_up = true;
+                uint32_t c = prefix_classes;
+                const uint4 words = dense_mask(p.seqs, seg.b, (row0 + r) >> 2);
+                for (int t = max(P, t0); t < t1; ++t)
+                    if (dense_bit(words, t - P)) c |= classes(t, t + 1);
+                if (sum == 0.0f) acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                else acc = make_float4(class_value(class_of(c, 0), acc.x), class_value(class_of(c, 1), acc.y),
+                                       class_value(class_of(c, 2), acc.z), class_value(class_of(c, 3), acc.w));
             }
             if (seg.whole()) {
                 if (ok) store_row(p, seg.b, (row0 + r) >> 2, seg.kvh * kGroup + ((row0 + r) & 3), lane, acc, M, sum);
@@ -422,6 +476,15 @@ __global__ void __launch_bounds__(kTreeMergeWarps * 32) tree_merge_kernel(const 
             acc.x = fmaf(a[i].x, w, acc.x); acc.y = fmaf(a[i].y, w, acc.y);
             acc.z = fmaf(a[i].z, w, acc.z); acc.w = fmaf(a[i].w, w, acc.w);
         }
+    }
+    if (__any_sync(0xffffffffu, !(acc.x == acc.x && acc.y == acc.y && acc.z == acc.z && acc.w == acc.w)) && sum > 0.0f) {
+        // (infinite partial results whose factor fp32 holds as zero, or of both signs)
+        uint32_t c[4] = {0, 0, 0, 0};
+        for (int k = c0; k <= c1; ++k) {
+            const float4 a = __ldcg(reinterpret_cast<const float4*>(p.part_acc + at(k) * kHeadDim) + lane);
+            c[0] |= value_class(a.x); c[1] |= value_class(a.y); c[2] |= value_class(a.z); c[3] |= value_class(a.w);
+        }
+        acc = make_float4(class_value(c[0], acc.x), class_value(c[1], acc.y), class_value(c[2], acc.z), class_value(c[3], acc.w));
     }
     store_row(p, b, row >> 2, kvh * kGroup + (row & 3), lane, acc, M, sum);
 }

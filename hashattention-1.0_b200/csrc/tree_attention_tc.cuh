@@ -31,7 +31,8 @@
 // where a tile takes 2500.
 //
 // The V rows behind a sequence's end, and V rows of drafts with an infinity or NaN in them, are zeroed in shared memory before
-// the product sees them; the latter are added at the end to the rows that see them, by scalar arithmetic.
+// the product sees them; the latter are added at the end to the rows that see them, by scalar arithmetic. What infinities of the
+// prefix, which every row sees, make of a channel is looked up at the end (v_classes).
 #pragma once
 
 #include "tree_attention.cuh"
@@ -446,13 +447,23 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
                     if (second) tc_ld16_issue(t_lane + 384u + 16 * q, o1);
                     tc_ld16_wait(o0);
                     if (second) tc_ld16_wait(o1);
-                    if (mine) {
-                        float acc[16];
+                    float acc[16];
+                    bool nan = false;
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            acc[k] = __uint_as_float(o0[k]) * f0;
-                            if (second) acc[k] = fmaf(__uint_as_float(o1[k]), f1, acc[k]);
-                        }
+                    for (int k = 0; k < 16; ++k) {
+                        acc[k] = __uint_as_float(o0[k]) * f0;
+                        if (second) acc[k] = fmaf(__uint_as_float(o1[k]), f1, acc[k]);
+                        nan |= acc[k] != acc[k];
+                    }
+                    nan = nan && mine && sum >= 0.0f;  // (with a sum of NaN the row is NaN)
+                    if (__any_sync(0xffffffffu, nan)) {
+                        const uint32_t classes = v_classes(p.v_pages, p.seqs.page_table + (size_t)seg.b * p.seqs.max_pages, p.seqs.num_pages, p.seqs.Hkv,
+                                                           seg.kvh, seg.tile0 * kTaTile, min(P, seg.tile1 * kTaTile), q);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            if (nan) acc[k] = sum == 0.0f ? 0.0f : class_value(class_of(classes, k), acc[k]);  // (0: scores of -inf only)
+                    }
+                    if (mine) {
                         if (bad != 0) {
                             const __nv_bfloat16* qr = p.q + seg.b * p.q_batch + (long long)node * p.q_node + (seg.kvh * kGroup + (r & 3)) * p.q_head;
                             for (int t = 0; t < seg.n; ++t) {
@@ -463,7 +474,10 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
                                 for (int d = 0; d < kHeadDim; ++d) dot = fmaf(__bfloat162float(qr[d]), __bfloat162float(p.k_pages[at + d]), dot);
                                 const float e = exp2_approx(fmaf(dot, p.scale_log2, M == -INFINITY ? 0.0f : -M));
 #pragma unroll
-                                for (int k = 0; k < 16; ++k) acc[k] = fmaf(e, __bfloat162float(p.v_pages[at + 16 * q + k]), acc[k]);
+                                for (int k = 0; k < 16; ++k) {
+                                    const float v = __bfloat162float(p.v_pages[at + 16 * q + k]);
+                                    acc[k] = fmaf(value_class(v) == 0 ? e : 1.0f, v, acc[k]);  // (any weight above zero: e may be one that fp32 holds as 0)
+                                }
                             }
                         }
                         if (seg.whole()) {
@@ -619,6 +633,15 @@ __global__ void __launch_bounds__(kTaMergeThreads) tree_merge_tc_kernel(const Tr
         if (half == 0) {
             const float2 ml = s_ml[warp][lane];
             add(ml, s_acc[warp][lane], rescale(fmaxf(M, ml.x)));
+            if (!(acc.x == acc.x && acc.y == acc.y && acc.z == acc.z && acc.w == acc.w) && sum > 0.0f) {
+                // (infinite partial results whose factor fp32 holds as zero, or of both signs)
+                uint32_t c[4] = {0, 0, 0, 0};
+                for (int k = c0; k <= c1; ++k) {
+                    const float4 a = __ldcg(part + (size_t)(k == c0 ? first_slot : 2 * k) * (kHeadDim / 4) * kRows);
+                    c[0] |= value_class(a.x); c[1] |= value_class(a.y); c[2] |= value_class(a.z); c[3] |= value_class(a.w);
+                }
+                acc = make_float4(class_value(c[0], acc.x), class_value(c[1], acc.y), class_value(c[2], acc.z), class_value(c[3], acc.w));
+            }
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             s_out[lane][warp] = make_uint2(tc_pack_bf16(acc.x * inv, acc.y * inv), tc_pack_bf16(acc.z * inv, acc.w * inv));
             if (d4 == 0 && row0 + lane < rows && p.lse != nullptr) p.lse[out_row(row0 + lane)] = natural_lse(M, sum);

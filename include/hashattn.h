@@ -359,6 +359,7 @@ int ha_tree_mask(const int32_t* parents, const int32_t* tree_lens, int32_t batch
 /* out[b][i][h] = softmax(sm_scale * q[b][i][h] . K) V over the prefix and the nodes that node i sees, fp32 sums, bf16 output;
  * lse (optional) [batch][max_nodes][num_q_heads] f32: the natural log of the sum of e^(scaled scores). Rows of nodes behind
  * a tree's own are left as they were. A row that sees nothing (or only scores of -inf) gives zeros and an lse of -inf.
+ * An infinity in a V row that a row sees makes that channel infinite, and NaN where it meets the other one or a NaN.
  * Scaled scores of magnitudes up to 2^29 (beyond, half an ulp of one is more than fp32 has exponents for).
  * q [batch][max_nodes][num_q_heads][128] bf16 with strides q_strides[3] = {batch, node, head} in elements (HOST array;
  * multiples of 8, the 128 elements of a row contiguous), or contiguous if NULL: a view of a fused projection will do.

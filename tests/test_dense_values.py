@@ -17,6 +17,82 @@ def plant(x, b, spots):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 4, 6, 30, 50, 100])
+@pytest.mark.parametrize("prefix", [40, 700, 9000])
+def test_infinities_in_the_prefix(device, n, prefix):
+    """The output is an average with weights above zero: infinite where V is, NaN where V is or where both infinities meet, and
+    finite in all other channels. Units of one CTA, and units that many CTAs share."""
+    x = Problem(device, [prefix + n, 300 + n], [n, n], 2, n, "tree", seed=n + prefix)
+    last = prefix - 1
+    plant(x, 0, [(0, 3, 0, math.inf), (0, last, 5, -math.inf), (0, 0, 31, math.inf), (0, last, 31, math.inf),   # one sign
+                 (0, 7, 64, math.inf), (0, last - 5, 64, -math.inf),                                              # both
+                 (0, 20, 127, math.nan), (0, 21, 90, math.inf), (0, 30, 90, math.nan),
+                 (1, prefix // 2, 17, -math.inf)])
+    out, lse = x.ctx.tree_attention(x.q, x.mask, x.tree_lens)
+    x.check(out, lse)
+    assert bool((out[0, :, :GROUP, 0] == math.inf).all()) and bool((out[0, :, :GROUP, 5] == -math.inf).all())
+    assert bool((out[0, :, :GROUP, 31] == math.inf).all()) and bool(out[0, :, :GROUP, [64, 90, 127]].isnan().all())
+    assert bool((out[0, :, GROUP:, 17] == -math.inf).all())
+    assert int((~torch.isfinite(out[0, :, :GROUP])).sum()) == 6 * GROUP * n and bool(torch.isfinite(out[1]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [4, 6, 40])
+def test_infinities_in_the_prefix_and_in_drafts(device, n):
+    """An infinity of the prefix meets those of drafts in the rows that see them only."""
+    prefix, leaf = 500, n - 1
+    x = Problem(device, [prefix + n], [n], 1, n, "tree", seed=7)
+    plant(x, 0, [(0, 9, 1, math.inf), (0, prefix + leaf, 1, -math.inf),   # opposite signs
+                 (0, 9, 2, math.inf), (0, prefix + leaf, 2, math.inf),    # the same one
+                 (0, 9, 3, -math.inf), (0, prefix + leaf, 3, math.nan),
+                 (0, prefix + leaf, 4, -math.inf)])
+    out, lse = x.ctx.tree_attention(x.q, x.mask, x.tree_lens)
+    x.check(out, lse)
+    sees = x.visible[0][:, leaf].to(device)
+    assert bool(out[0, sees][:, :, [1, 3]].isnan().all()) and bool((out[0, ~sees][:, :, [1, 2]] == math.inf).all())
+    assert bool((out[0, sees][:, :, 4] == -math.inf).all()) and bool(torch.isfinite(out[0, ~sees][:, :, 4]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 4, 6, 40])
+@pytest.mark.parametrize("prefix", [300, 9000])
+def test_infinities_whose_weight_fp32_holds_as_zero(device, n, prefix):
+    """Scores thousands apart: every weight but one is zero in fp32 (and in 64 bits), but none is by its definition."""
+    x = Problem(device, [prefix + n, 200 + n], [n, n], 2, n, "tree", seed=n + prefix)
+    x.ctx, leaf = ha.DenseDecodeContext(x.cache, n, sm_scale=300.0), n - 1
+    spots = [(0, 3, 0, math.inf), (0, prefix - 1, 5, -math.inf), (0, prefix // 2, 77, math.inf), (0, prefix // 3, 100, math.inf),
+             (0, 9, 100, -math.inf), (0, 40, 101, math.nan)]
+    if n > 1:
+        spots += [(0, prefix + leaf, 20, math.inf), (0, prefix + leaf, 77, -math.inf)]
+    plant(x, 0, spots)
+    out, lse = x.ctx.tree_attention(x.q, x.mask, x.tree_lens)
+    sees = x.visible[0][:, leaf].to(device) if n > 1 else torch.zeros(n, dtype=torch.bool, device=device)
+    want = torch.zeros(n, GROUP, D, device=device)
+    want[:, :, 0], want[:, :, 5], want[:, :, 77], want[:, :, [100, 101]] = math.inf, -math.inf, math.inf, math.nan
+    want[sees, :, 20] = math.inf
+    want[sees, :, 77] = math.nan
+    got = out[0, :, :GROUP].float()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isfinite(got), torch.isfinite(want))
+    assert torch.equal(got == math.inf, want == math.inf)
+    assert bool(torch.isfinite(out[0, :, GROUP:]).all()) and bool(torch.isfinite(out[1]).all()) and bool(torch.isfinite(lse).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["k", "q"])
+@pytest.mark.parametrize("n", [1, 30, 50])
+def test_scores_that_are_not_finite_stay_nan_beside_infinite_values(device, what, n):
+    """NaN scores make their whole row NaN, infinite V or not."""
+    x = Problem(device, [600 + n], [n], 1, n, "chain", seed=n)
+    if what == "k":
+        x.k[0][0, 11, 3] = math.nan
+    else:
+        x.q[0, n - 1, 2, 8] = math.nan
+    plant(x, 0, [(0, 50, 9, math.inf)])
+    out, lse = x.ctx.tree_attention(x.q, x.mask, x.tree_lens)
+    x.check(out, lse)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n,prefix,kv_heads", [(1, 700, 2), (1, 20000, 2), (4, 3000, 4), (5, 700, 2), (9, 9000, 8), (32, 20000, 4), (40, 700, 2), (60, 9000, 2), (128, 2000, 1)])
 @pytest.mark.parametrize("power", [0, 8, 15, 17, 19, 22])
 def test_one_clear_winner_per_row(device, n, prefix, kv_heads, power):
