@@ -88,9 +88,9 @@ int launch_tree(void (*kernel)(TreeAttentionParams, CUtensorMap, CUtensorMap), i
     if (launch_smem(kernel, dim3(ctas), dim3(threads), smem_bytes, st, 1, p, k_map, v_map) != cudaSuccess) return HA_ERR_LAUNCH;
     const int rows_max = std::min(kRows, p.seqs.T * kGroup);
     cudaError_t e;
-    if constexpr (kRows <= 32) {
-        const dim3 grid(shape->num_kv_heads * groups, shape->batch, (rows_max + kTreeMergeWarps - 1) / kTreeMergeWarps);
-        e = launch(tree_merge_kernel<kTile, kRows>, grid, dim3(kTreeMergeWarps * 32), st, 1, p, ctas);
+    if constexpr (kRows == RowsLayout::kRows) {
+        const dim3 grid(shape->num_kv_heads, shape->batch, (rows_max + kTreeMergeWarps - 1) / kTreeMergeWarps);
+        e = launch(tree_merge_rows_kernel, grid, dim3(kTreeMergeWarps * 32), st, 1, p, ctas);
     } else {
         const bool few = 4ll * shape->batch * shape->num_kv_heads * groups < ctas;  // units: many partial results of each
         const int parts = shape->num_kv_heads * groups * (few ? kTaMergeParts : kTaMergeParts / 4);
@@ -173,7 +173,7 @@ int ha_tree_attention(const ha_shape_t* shape, const ha_tree_t* tree, const void
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     p.k_pages = static_cast<const __nv_bfloat16*>(k_pages);
     p.v_pages = static_cast<const __nv_bfloat16*>(v_pages);
-    if (rows == 16) return launch_tree<kRowsTile, 16, 0>(tree_attention_rows_kernel<1>, kRowsThreads, RowsLayout<1>::kSmemBytes, shape, p, st);
+    if (rows == RowsLayout::kRows) return launch_tree<kRowsTile, RowsLayout::kRows, 0>(tree_attention_rows_kernel, kRowsThreads, RowsLayout::kSmemBytes, shape, p, st);
     if (rows == 128) return launch_tree<kTaTile, 128, TaLayout<false>::kCross>(tree_attention_tc_kernel<false>, kTaThreads, TaLayout<false>::kSmemBytes, shape, p, st);
     return launch_tree<kTaTile, 256, TaLayout<true>::kCross>(tree_attention_tc_kernel<true>, kTaThreads, TaLayout<true>::kSmemBytes, shape, p, st);
 }

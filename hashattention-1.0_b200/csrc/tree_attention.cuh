@@ -47,9 +47,8 @@ constexpr uint32_t kRowsHalf = kRowsTile * 128;      // 64 rows x 64 elements
 constexpr uint32_t kRowsStage = 4 * kRowsHalf;       // K and V of a tile: 32 KB
 constexpr float kRescaleAt = 8.0f;       // a row's weights may grow to 2^8 before its sums are rescaled
 
-template <int MT>  // 16-row tiles of query rows (1 is used)
 struct RowsLayout {
-    static constexpr int kRows = 16 * MT;
+    static constexpr int kRows = 16;  // 4 query heads x up to 4 nodes
     static constexpr int kStages = 5;
     static constexpr int kAccPitch = kHeadDim + 4;
     static constexpr uint32_t kOffAcc = kStages * kRowsStage;                               // [4 warps][kRows][kAccPitch] floats
@@ -125,10 +124,9 @@ __device__ __forceinline__ void store_row(const TreeAttentionParams& p, int b, i
     if (lane == 0 && p.lse != nullptr) p.lse[row] = natural_lse(M, L);
 }
 
-template <int MT>
 __global__ void __launch_bounds__(kRowsThreads, 1)
 tree_attention_rows_kernel(const TreeAttentionParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
-    using L = RowsLayout<MT>;
+    using L = RowsLayout;
     using Cursor = DenseCursor<kRowsTile, L::kRows, 0>;
     extern __shared__ unsigned char rows_smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(rows_smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -199,43 +197,36 @@ tree_attention_rows_kernel(const TreeAttentionParams p, const __grid_constant__ 
     const uint32_t k_row = (uint32_t)(warp * 16 + ((lane >> 4) << 3) + (lane & 7)), k_chunk = (uint32_t)((lane >> 3) & 1);
     const uint32_t v_row = (uint32_t)(warp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7)), v_chunk = (uint32_t)(lane >> 4);
     while (cur.next(seg)) {
-        const int P = seg.S - seg.n, row0 = seg.group * L::kRows;
-        uint32_t qa[MT][8][4];  // the query rows as the A operand: rows lane / 4 and + 8, elements 2 (lane % 4) and + 8
+        const int P = seg.S - seg.n;  // (a sequence's rows are one group)
+        uint32_t qa[8][4];  // the query rows as the A operand: rows lane / 4 and + 8, elements 2 (lane % 4) and + 8
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int h = 0; h < 2; ++h) {
+            const int r = h * 8 + (lane >> 2);
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + seg.b * p.q_batch + (r >> 2) * p.q_node +
+                                                                    (seg.kvh * kGroup + (r & 3)) * p.q_head) + (lane & 3);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int r = row0 + mt * 16 + h * 8 + (lane >> 2);
-                const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + seg.b * p.q_batch + (r >> 2) * p.q_node +
-                                                                        (seg.kvh * kGroup + (r & 3)) * p.q_head) + (lane & 3);
-#pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {
-                    qa[mt][ks][h] = r < seg.n * kGroup ? __ldg(src + ks * 8) : 0u;
-                    qa[mt][ks][h + 2] = r < seg.n * kGroup ? __ldg(src + ks * 8 + 4) : 0u;
-                }
+            for (int ks = 0; ks < 8; ++ks) {
+                qa[ks][h] = r < seg.n * kGroup ? __ldg(src + ks * 8) : 0u;
+                qa[ks][h + 2] = r < seg.n * kGroup ? __ldg(src + ks * 8 + 4) : 0u;
             }
-        float o[MT][16][4] = {};
-        float m[MT][2], l[MT][2];
+        }
+        float o[16][4] = {};
+        float m[2], l[2];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) m[mt][h] = -INFINITY, l[mt][h] = 0.0f;
+        for (int h = 0; h < 2; ++h) m[h] = -INFINITY, l[h] = 0.0f;
 
         for (int t = seg.tile0; t < seg.tile1; ++t, ++it) {
             const uint32_t s = it % L::kStages, kb = sbase + s * kRowsStage, vb = kb + 2 * kRowsHalf;
             if (ok) ok = __all_sync(0xffffffffu, tc_wait(full(s), (it / L::kStages) & 1, s_abort, p.seqs.status)) != 0;
             if (!ok) continue;
             const int tok0 = t * kRowsTile + warp * 16;
-            float c[MT][2][4] = {};
+            float c[2][4] = {};
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) {
                 uint32_t kf[4];
                 ldmatrix4(kb + rows_at(k_row, 2 * ks + k_chunk), kf);
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    mma16816(c[mt][0], qa[mt][ks], kf[0], kf[1]);
-                    mma16816(c[mt][1], qa[mt][ks], kf[2], kf[3]);
-                }
+                mma16816(c[0], qa[ks], kf[0], kf[1]);
+                mma16816(c[1], qa[ks], kf[2], kf[3]);
             }
             uint32_t vkeep[2] = {0xffffffffu, 0xffffffffu}, bad = 0;  // V values to use; tokens of the tree with an infinity or NaN in V
             if (tok0 + 16 > P) {
@@ -258,60 +249,55 @@ tree_attention_rows_kernel(const TreeAttentionParams p, const __grid_constant__ 
                         if (tok0 + tk >= seg.S || ((bad >> tk) & 1u)) vkeep[nt] &= e ? 0x0000ffffu : 0xffff0000u;
                     }
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                for (int h = 0; h < 2; ++h) {
+                    const int node = 2 * h + (lane >> 4);
+                    const uint4 words = node < seg.n ? dense_mask(p.seqs, seg.b, node) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int node = (row0 + mt * 16 + h * 8 + (lane >> 2)) >> 2;
-                        const uint4 words = node < seg.n ? dense_mask(p.seqs, seg.b, node) : make_uint4(0, 0, 0, 0);
+                    for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-                        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int j = tok0 + nt * 8 + (lane & 3) * 2 + e;
-                                if (j >= seg.S || (j >= P && !dense_bit(words, j - P))) c[mt][nt][2 * h + e] = -INFINITY;
-                            }
-                    }
+                        for (int e = 0; e < 2; ++e) {
+                            const int j = tok0 + nt * 8 + (lane & 3) * 2 + e;
+                            if (j >= seg.S || (j >= P && !dense_bit(words, j - P))) c[nt][2 * h + e] = -INFINITY;
+                        }
+                }
             }
-            uint32_t ph[MT][4], pl[MT][4];
+            uint32_t ph[4], pl[4];
+            bool grow = false;
+            float alpha[2];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                bool grow = false;
-                float alpha[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float x = fmaxf(fmaxf(c[mt][0][2 * h], c[mt][0][2 * h + 1]), fmaxf(c[mt][1][2 * h], c[mt][1][2 * h + 1]));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2)) * p.scale_log2;
-                    alpha[h] = 1.0f;
-                    if (x > m[mt][h] + kRescaleAt) {  // (from -inf: any score at all)
-                        alpha[h] = exp2_approx(m[mt][h] - x);
-                        m[mt][h] = x;
-                        grow = true;
-                    }
+            for (int h = 0; h < 2; ++h) {
+                float x = fmaxf(fmaxf(c[0][2 * h], c[0][2 * h + 1]), fmaxf(c[1][2 * h], c[1][2 * h + 1]));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2)) * p.scale_log2;
+                alpha[h] = 1.0f;
+                if (x > m[h] + kRescaleAt) {  // (from -inf: any score at all)
+                    alpha[h] = exp2_approx(m[h] - x);
+                    m[h] = x;
+                    grow = true;
                 }
-                if (__any_sync(0xffffffffu, grow)) {
+            }
+            if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-                    for (int dt = 0; dt < 16; ++dt) {
-                        o[mt][dt][0] *= alpha[0]; o[mt][dt][1] *= alpha[0];
-                        o[mt][dt][2] *= alpha[1]; o[mt][dt][3] *= alpha[1];
-                    }
-                    l[mt][0] *= alpha[0];
-                    l[mt][1] *= alpha[1];
+                for (int dt = 0; dt < 16; ++dt) {
+                    o[dt][0] *= alpha[0]; o[dt][1] *= alpha[0];
+                    o[dt][2] *= alpha[1]; o[dt][3] *= alpha[1];
                 }
+                l[0] *= alpha[0];
+                l[1] *= alpha[1];
+            }
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float ref = m[mt][h] == -INFINITY ? 0.0f : m[mt][h];
+            for (int h = 0; h < 2; ++h) {
+                const float ref = m[h] == -INFINITY ? 0.0f : m[h];
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) {
-                        const float p0 = exp2_approx(fmaf(c[mt][nt][2 * h], p.scale_log2, -ref));
-                        const float p1 = exp2_approx(fmaf(c[mt][nt][2 * h + 1], p.scale_log2, -ref));
-                        l[mt][h] += p0 + p1;
-                        const uint32_t hi = tc_pack_bf16(p0, p1);
-                        ph[mt][2 * nt + h] = hi;
-                        pl[mt][2 * nt + h] = tc_pack_bf16(p0 - bf16_lo(hi), p1 - bf16_hi(hi));
-                        c[mt][nt][2 * h] = p0;
-                        c[mt][nt][2 * h + 1] = p1;
-                    }
+                for (int nt = 0; nt < 2; ++nt) {
+                    const float p0 = exp2_approx(fmaf(c[nt][2 * h], p.scale_log2, -ref));
+                    const float p1 = exp2_approx(fmaf(c[nt][2 * h + 1], p.scale_log2, -ref));
+                    l[h] += p0 + p1;
+                    const uint32_t hi = tc_pack_bf16(p0, p1);
+                    ph[2 * nt + h] = hi;
+                    pl[2 * nt + h] = tc_pack_bf16(p0 - bf16_lo(hi), p1 - bf16_hi(hi));
+                    c[nt][2 * h] = p0;
+                    c[nt][2 * h + 1] = p1;
                 }
             }
 #pragma unroll
@@ -319,13 +305,10 @@ tree_attention_rows_kernel(const TreeAttentionParams p, const __grid_constant__ 
                 uint32_t vf[4];
                 ldmatrix4_trans(vb + rows_at(v_row, dt + v_chunk), vf);
                 vf[0] &= vkeep[0]; vf[1] &= vkeep[1]; vf[2] &= vkeep[0]; vf[3] &= vkeep[1];
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    mma16816(o[mt][dt], ph[mt], vf[0], vf[1]);
-                    mma16816(o[mt][dt + 1], ph[mt], vf[2], vf[3]);
-                    mma16816(o[mt][dt], pl[mt], vf[0], vf[1]);
-                    mma16816(o[mt][dt + 1], pl[mt], vf[2], vf[3]);
-                }
+                mma16816(o[dt], ph, vf[0], vf[1]);
+                mma16816(o[dt + 1], ph, vf[2], vf[3]);
+                mma16816(o[dt], pl, vf[0], vf[1]);
+                mma16816(o[dt + 1], pl, vf[2], vf[3]);
             }
             if (bad != 0) {
                 // V rows with an infinity or NaN, one by one, for the rows that see them
@@ -337,19 +320,17 @@ tree_attention_rows_kernel(const TreeAttentionParams p, const __grid_constant__ 
                             const int tk = nt * 8 + 2 * w + e;
                             if (((bad >> tk) & 1u) == 0) continue;
 #pragma unroll
-                            for (int mt = 0; mt < MT; ++mt)
+                            for (int h = 0; h < 2; ++h) {
+                                const float pv = __shfl_sync(0xffffffffu, c[nt][2 * h + e], (lane & ~3) | w);
+                                const int node = 2 * h + (lane >> 4);
+                                if (node >= seg.n || !dense_bit(dense_mask(p.seqs, seg.b, node), tok0 + tk - P)) continue;
 #pragma unroll
-                                for (int h = 0; h < 2; ++h) {
-                                    const float pv = __shfl_sync(0xffffffffu, c[mt][nt][2 * h + e], (lane & ~3) | w);
-                                    const int node = (row0 + mt * 16 + h * 8 + (lane >> 2)) >> 2;
-                                    if (node >= seg.n || !dense_bit(dense_mask(p.seqs, seg.b, node), tok0 + tk - P)) continue;
-#pragma unroll
-                                    for (int dt = 0; dt < 16; ++dt) {
-                                        const uint32_t w2 = *reinterpret_cast<const uint32_t*>(smem + (vb - sbase) + rows_at(warp * 16 + tk, dt) + (lane & 3) * 4);
-                                        o[mt][dt][2 * h] = fmaf(pv, bf16_lo(w2), o[mt][dt][2 * h]);
-                                        o[mt][dt][2 * h + 1] = fmaf(pv, bf16_hi(w2), o[mt][dt][2 * h + 1]);
-                                    }
+                                for (int dt = 0; dt < 16; ++dt) {
+                                    const uint32_t w2 = *reinterpret_cast<const uint32_t*>(smem + (vb - sbase) + rows_at(warp * 16 + tk, dt) + (lane & 3) * 4);
+                                    o[dt][2 * h] = fmaf(pv, bf16_lo(w2), o[dt][2 * h]);
+                                    o[dt][2 * h + 1] = fmaf(pv, bf16_hi(w2), o[dt][2 * h + 1]);
                                 }
+                            }
                             __syncwarp();
                         }
             }
@@ -359,20 +340,18 @@ tree_attention_rows_kernel(const TreeAttentionParams p, const __grid_constant__ 
 
         // ---- the four warps' results: one row at a time per warp ------------------------------------------------------
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int h = 0; h < 2; ++h) {
+            const int r = h * 8 + (lane >> 2);
+            float sum = l[h];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if ((lane & 3) == 0) s_ml[warp * L::kRows + r] = make_float2(m[h], sum);
+            float* dst = s_acc + (size_t)(warp * L::kRows + r) * L::kAccPitch + (lane & 3) * 2;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int r = mt * 16 + h * 8 + (lane >> 2);
-                float sum = l[mt][h];
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                if ((lane & 3) == 0) s_ml[warp * L::kRows + r] = make_float2(m[mt][h], sum);
-                float* dst = s_acc + (size_t)(warp * L::kRows + r) * L::kAccPitch + (lane & 3) * 2;
-#pragma unroll
-                for (int dt = 0; dt < 16; ++dt) *reinterpret_cast<float2*>(dst + dt * 8) = make_float2(o[mt][dt][2 * h], o[mt][dt][2 * h + 1]);
-            }
+            for (int dt = 0; dt < 16; ++dt) *reinterpret_cast<float2*>(dst + dt * 8) = make_float2(o[dt][2 * h], o[dt][2 * h + 1]);
+        }
         asm volatile("bar.sync 1, %0;" ::"n"(kRowsWarps * 32) : "memory");
-        const int rows = min(L::kRows, seg.n * kGroup - row0);
+        const int rows = seg.n * kGroup;
         bool looked_up = false;  // what the prefix's V rows hold beside numbers, for a row that comes out NaN
         uint32_t prefix_classes = 0;
         for (int r = warp; r < rows; r += kRowsWarps) {
@@ -407,7 +386,7 @@ tree_attention_rows_kernel(const TreeAttentionParams p, const __grid_constant__ 
                 if (!looked_up) prefix_classes = classes(t0, min(P, t1));
                 looked_up = true;
                 uint32_t c = prefix_classes;
-                const uint4 words = dense_mask(p.seqs, seg.b, (row0 + r) >> 2);
+                const uint4 words = dense_mask(p.seqs, seg.b, r >> 2);
                 for (int t = max(P, t0); t < t1; ++t)
                     if (dense_bit(words, t - P)) c |= classes(t, t + 1);
                 if (sum == 0.0f) acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -415,7 +394,7 @@ tree_attention_rows_kernel(const TreeAttentionParams p, const __grid_constant__ 
                                        class_value(class_of(c, 2), acc.z), class_value(class_of(c, 3), acc.w));
             }
             if (seg.whole()) {
-                if (ok) store_row(p, seg.b, (row0 + r) >> 2, seg.kvh * kGroup + ((row0 + r) & 3), lane, acc, M, sum);
+                if (ok) store_row(p, seg.b, r >> 2, seg.kvh * kGroup + (r & 3), lane, acc, M, sum);
             } else {
                 const size_t at = (size_t)(2 * blockIdx.x + seg.slot) * L::kRows + r;
                 if (lane == 0) p.part_ml[at] = make_float2(M, sum);
@@ -426,27 +405,24 @@ tree_attention_rows_kernel(const TreeAttentionParams p, const __grid_constant__ 
     }
 }
 
-// The partial results of the units that several CTAs share, a warp per query row; grid (Hkv * groups of T, B, rows / 4).
+// The partial results of the units that several CTAs share, a warp per query row; grid (Hkv, B, rows / 4).
 constexpr int kTreeMergeWarps = 4;
-template <int kTile, int kRows>
-__global__ void __launch_bounds__(kTreeMergeWarps * 32) tree_merge_kernel(const TreeAttentionParams p, int ctas) {
-    using Cut = DenseCut<kTile, kRows, 0>;
+__global__ void __launch_bounds__(kTreeMergeWarps * 32) tree_merge_rows_kernel(const TreeAttentionParams p, int ctas) {
+    constexpr int kRows = RowsLayout::kRows;
+    using Cut = DenseCut<kRowsTile, kRows, 0>;
     // The lengths are read before the wait: the attention kernel in front does not write them, and what did has completed.
-    const int lane = threadIdx.x & 31, r = blockIdx.z * kTreeMergeWarps + (threadIdx.x >> 5), b = blockIdx.y;
-    const int max_groups = Cut::groups(p.seqs.T);
-    const int kvh = blockIdx.x / max_groups, group = blockIdx.x - kvh * max_groups;
+    const int lane = threadIdx.x & 31, r = blockIdx.z * kTreeMergeWarps + (threadIdx.x >> 5), b = blockIdx.y, kvh = blockIdx.x;
     int S, n;
     dense_seq(p.seqs, b, false, S, n);
-    const int row = group * kRows + r;
     int quota, before, span;
     Cut::count(p.seqs, ctas, lane, b, quota, before, span);
     const int tiles = Cut::tiles_of(S);
-    const int start = before + (kvh * Cut::groups(n) + group) * span;
+    const int start = before + kvh * span;
     const int c0 = dense_div(start, quota), c1 = dense_div(start + tiles - 1, quota);
     auto at = [&](int c) { return (size_t)(2 * c + (c == c0 && c0 * quota != start ? 1 : 0)) * kRows + r; };
     pdl_wait();
     pdl_launch_dependents();
-    if (row >= n * kGroup || c0 == c1) return;  // (one CTA had the whole unit)
+    if (r >= n * kGroup || c0 == c1) return;  // (one CTA had the whole unit)
 
     // 16 partial results at a time, all of their loads in flight together, in an order that is always the same
     constexpr int kBatch = 16;
@@ -486,7 +462,7 @@ __global__ void __launch_bounds__(kTreeMergeWarps * 32) tree_merge_kernel(const 
         }
         acc = make_float4(class_value(c[0], acc.x), class_value(c[1], acc.y), class_value(c[2], acc.z), class_value(c[3], acc.w));
     }
-    store_row(p, b, row >> 2, kvh * kGroup + (row & 3), lane, acc, M, sum);
+    store_row(p, b, r >> 2, kvh * kGroup + (r & 3), lane, acc, M, sum);
 }
 
 }  // namespace ha
