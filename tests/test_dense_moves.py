@@ -112,3 +112,71 @@ def test_eviction_keeps_the_weights_of_a_sequence_whose_length_is_out_of_range(d
         own = x.cache.page_table[1].tolist()
         for was, now in zip(before, pools(x.cache)):
             assert torch.equal(now[own], was[own])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [-1, 2 ** 31 - 1])
+def test_eviction_moves_no_row_from_or_to_a_page_out_of_range(device, bad):
+    """Page ids out of range as source and as destination: what lies there stays, all other kept rows move, and other
+    sequences' pages (physical page 0 among them) are as if nothing had been wrong."""
+    lens, keep = [900, 800], 300
+    x = Problem(device, lens, [0, 0], 2, 1, seed=9)
+    y = Problem(device, lens, [0, 0], 2, 1, seed=9)  # the same without bad ids
+    mass = torch.rand(x.ctx.mass_shape, device=device)
+    table = x.cache.page_table.clone()
+    for page in (0, 2):  # (tokens 0 .. 255: destinations, 512 .. 767: sources)
+        x.cache.page_table.copy_(table)
+        for b in range(2):
+            x.write(b)
+            y.write(b)
+        x.cache.hash_pages.copy_(y.cache.hash_pages)
+        x.cache.page_table[0, page] = bad
+        before = pools(x.cache)
+        kept, _, _ = x.ctx.cache_evict(mass, keep, 8, 8)
+        with pytest.raises(RuntimeError, match=rf"status {_lib.HA_ERR_BAD_PAGE}\)"):
+            x.ctx.check_status()
+        y.ctx.cache_evict(mass, keep, 8, 8)
+        y.ctx.check_status()
+        other = table[1].tolist()
+        for was, now, good in zip(before, pools(x.cache), pools(y.cache)):
+            assert torch.equal(now[other], good[other])
+            rest = [i for i in range(x.cache.num_pages) if i not in table.flatten().tolist()]
+            assert torch.equal(now[rest], was[rest]) and torch.equal(now[int(table[0, page])], was[int(table[0, page])])
+            for h in range(2):
+                rows_was = was[table[0].long(), h].flatten(0, 1)
+                want = rows_was.clone()
+                for i, t in enumerate(kept[0, h].tolist()):
+                    if t != i and t // 256 != page and i // 256 != page:
+                        want[i] = rows_was[t]
+                assert torch.equal(now[table[0].long(), h].flatten(0, 1), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,keep", [([4000], 1000), ([700, 300, 20], 256), ([9000, 8192, 100], 8000)])
+def test_eviction_of_sequences_far_below_the_capacity(device, lens, keep):
+    """Pages for 131072 tokens a sequence: the cluster's form of the selection on rows that fill a part of it, or one CTA of it only."""
+    cache = ha.PagedHashKVCache(len(lens), 2, 131072, device, shuffle_seed=4)
+    g = torch.Generator(device=device).manual_seed(1)
+    for pool in (cache.k_pages, cache.v_pages):
+        pool.view(torch.int16).random_(-2 ** 15, 2 ** 15, generator=g)
+    cache.hash_pages.random_(-2 ** 31, 2 ** 31 - 1, generator=g)
+    cache.seq_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+    ctx = ha.DenseDecodeContext(cache)
+    mass = torch.rand(ctx.mass_shape, generator=g, device=device)
+    before = [[r.clone() for r in flat_rows(cache, b)] for b in range(len(lens))]
+    kept, mass_out, lens_out = ctx.cache_evict(mass, keep, 16, 16)
+    ctx.check_status()
+    assert lens_out.tolist() == [min(s, keep) for s in lens]
+    for b, s in enumerate(lens):
+        now = flat_rows(cache, b)
+        for h in range(2):
+            index = evict64(mass[b, h].cpu(), s, keep, 16, 16)
+            n = len(index)
+            assert kept[b, h, :n].tolist() == index and bool((kept[b, h, n:] == -1).all())
+            at = torch.tensor(index, device=device)
+            assert torch.equal(mass_out[b, h, :n], mass[b, h][at]) and bool((mass_out[b, h, n:] == 0).all())
+            for was, is_ in zip(before[b], now):
+                want = was[h].clone()
+                want[:n] = was[h][at]
+                kind = torch.int16 if is_.dtype == torch.bfloat16 else torch.int32
+                assert torch.equal(is_[h].view(kind), want.view(kind))
