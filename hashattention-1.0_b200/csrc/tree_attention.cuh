@@ -9,9 +9,9 @@
 //
 // The products run on the warps' matrix instructions (m16n8k16, bf16 with fp32 sums): with 4 to 16 query rows, of which a tcgen05
 // tile of 128 would be mostly padding, the bytes of K and V bound the kernel and not the products (from 5 nodes on the
-// tensor-core kernel of tree_attention_tc.cuh is faster). 32 sequences of 16K to 64K tokens x 8 kv-heads take 790 to 840 us, 780 of
-// which are the bytes at the copy rate; 16 x 16384 x 8 164 us (floor 164), 131072 x 8 89 (82); 8192 x 8 13 to 17 and 701 x 8
-// 6.7 in a graph, of which the start and the second kernel are the most. The weights e^{s - m} are
+// tensor-core kernel of tree_attention_tc.cuh is faster). 32 sequences of 16K to 64K tokens x 8 kv-heads take 775 to 840 us, 780 of
+// which are the bytes at the copy rate; in a graph 16 x 16384 x 8 take 161 to 167 us (floor 164), 131072 x 8 87 (82), 8192 x 8
+// 14 (15.5 with 4 nodes) and 701 x 8 6.4, of which the start and the second kernel are the most. The weights e^{s - m} are
 // handed to the second product as two bf16 (hi + lo, 16 bits of mantissa), so that their rounding does not show beside
 // the one of the bf16 output. The maximum a row's weights refer to moves only when a score passes it by more than 2^8: the
 // sums are fp32 and do not mind, and rescaling 16 x 128 of them at every new maximum would.

@@ -24,9 +24,10 @@
 // What bounds it. A stream's turn is 24 products of 64 clocks (1536; the lo halves are 512 of them); the streams take turns every
 // 2300 to 2450 clocks, the rest being the issuing warp's waits and the way from scores to weights (1400 clocks to the first half
 // of P, 700 more to the second). Up to 128 rows: K and V of a tile take 2760 clocks at the copy rate, so a long cache is read at
-// 5.5 to 5.7 TB/s (131072 tokens x 8 kv-heads with 8 drafts: 97 us, floor 82). 256 rows: 790 TFLOP/s (1190 with the lo halves)
-// at 4 x 131072 x 8 with 64 drafts, 694 us, where the power limit has brought the clock to 1.36 GHz; in long runs 820.
-// Short calls: 5 us until the first scores, 3 for the end of a unit, 4 for the second kernel (20011 x 8 with 32 drafts: 29.6 us).
+// 4.8 to 5.7 TB/s (131072 tokens x 8 kv-heads with 8 drafts: 94 us in a burst, 111 after a second, floor 82). 256 rows: 4 x 131072
+// x 8 with 64 drafts take 680 us in a burst (810 TFLOP/s, 1210 with the lo halves), where the power limit brings the clock to
+// 1.36 GHz, and 775 to 830 in runs of a second. Short calls: 5 us until the first scores, 3 for the end of a unit, 4 for the second
+// kernel (20011 x 8 with 32 drafts: 28 us with K and V in L2, 31 to 32 from memory).
 // Loops are kept rolled where a CTA does only a few tiles: the instructions of its first tile come from memory, and took 9000 clocks
 // where a tile takes 2500.
 //
