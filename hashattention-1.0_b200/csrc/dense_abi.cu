@@ -25,8 +25,12 @@ int check_tree(const ha_tree_t* t) {
     return t->max_nodes > kMaxNodes ? HA_ERR_UNSUPPORTED_DIM : HA_OK;
 }
 
-// The kernels count the tiles of 64 tokens of all sequences, heads and groups of 16 rows in 32 bits.
+// Rows of a pool (page, kv-head, token of the page) are numbered in 32 bits.
+bool too_many_rows(const ha_shape_t* s) { return (long long)s->num_pages * s->num_kv_heads * kPage > 0x7fffffffll; }
+
+// The kernels count the tiles of 64 tokens of all sequences, heads and groups of 16 rows in 32 bits, and copy tiles by row number.
 int check_tiles(const ha_shape_t* s, const ha_tree_t* t) {
+    if (too_many_rows(s)) return HA_ERR_UNSUPPORTED_DIM;
     const double groups = (double)((t->max_nodes * kGroup + 15) / 16), tiles = (double)s->max_pages * (kPage / kRowsTile);
     return tiles > kMaxTiles / kRowsTile || tiles * groups * s->batch * s->num_kv_heads > kMaxTiles ? HA_ERR_UNSUPPORTED_DIM : HA_OK;
 }
@@ -246,7 +250,7 @@ int ha_cache_evict(const ha_shape_t* shape, int32_t keep_tokens, int32_t init_bu
         recent_budget < 0 || (long long)init_budget + recent_budget > keep_tokens)
         return HA_ERR_BAD_ARG;
     if (workspace == nullptr || workspace_bytes < evict_workspace(shape)) return HA_ERR_WORKSPACE;
-    if ((long long)shape->num_pages * shape->num_kv_heads * kPage > 0x7fffffffll) return HA_ERR_UNSUPPORTED_DIM;  // (row numbers are 32 bits)
+    if (too_many_rows(shape)) return HA_ERR_UNSUPPORTED_DIM;
     const long long capacity = (long long)shape->max_pages * kPage;
     EvictParams p;
     p.mass = mass;

@@ -333,7 +333,8 @@ int ha_rope_split(const void* qkv, const int64_t* positions, int32_t batch, int3
  * Sequences with n == 0 are left out: nothing of theirs is read or written. Lengths out of range (n < 0 or > max_nodes,
  * seq_len < n or beyond max_pages * page_size) are reported as HA_ERR_BAD_SEQ_LEN and left out too.
  * ha_tree_attention and ha_attention_mass count tiles of 64 tokens in 32 bits: shapes with more than 2^30 of them (over all sequences,
- * kv-heads and groups of 16 query rows, at max_pages each) are refused as HA_ERR_UNSUPPORTED_DIM.
+ * kv-heads and groups of 16 query rows, at max_pages each) are refused as HA_ERR_UNSUPPORTED_DIM. So are, by them and by
+ * ha_cache_evict, pools of 2^31 rows (num_pages * num_kv_heads * page_size) and more.
  * ha_tree_commit and ha_cache_evict move rows in place: the pages they write to must not be shared between sequences.
  * Cache codes of the LSH baseline depend on every key a cache has seen: after a commit or an eviction, ha_hash_prefill anew.
  * sel_stride of the shape is not used by these entry points (any value >= 1). ha_tree_mask and ha_tree_accept, which have no

@@ -1,5 +1,7 @@
 """What commit and eviction move, and what they leave alone: page ids and lengths that are out of range, rounds narrower than the
 context, capacities far above the lengths. Rows are compared bit by bit."""
+import ctypes
+
 import pytest
 import torch
 
@@ -180,3 +182,16 @@ def test_eviction_of_sequences_far_below_the_capacity(device, lens, keep):
                 want[:n] = was[h][at]
                 kind = torch.int16 if is_.dtype == torch.bfloat16 else torch.int32
                 assert torch.equal(is_[h].view(kind), want.view(kind))
+
+
+def test_pools_with_more_rows_than_are_numbered_are_refused():
+    """2^31 rows of K (512 GB): row numbers are 32 bits."""
+    lib, X = _lib.load(), ctypes.c_void_p(256)  # (never dereferenced: the checks come first)
+    tree = _lib.HaTree(8, None, None)
+    for pages, want in ((2 ** 20, _lib.HA_ERR_UNSUPPORTED_DIM), (2 ** 20 - 1, _lib.HA_ERR_WORKSPACE)):
+        shape = _lib.HaShape(1, 8, 4, 128, 256, 4, pages, 1)
+        # (a workspace that is too small is the next thing looked at, by those that take one)
+        assert lib.ha_tree_attention(shape, tree, X, None, X, X, X, X, 0.1, X, None, X, 8, X, None) == want
+        if want == _lib.HA_ERR_UNSUPPORTED_DIM:
+            assert lib.ha_attention_mass(shape, tree, X, None, X, None, X, X, X, 0.1, X, X, None) == want
+            assert lib.ha_cache_evict(shape, 10, 1, 1, X, X, X, None, X, X, X, None, ctypes.c_void_p(512), X, 1 << 40, X, None) == want
