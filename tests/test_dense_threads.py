@@ -1,14 +1,17 @@
 """Python threads that enqueue through one context, or through contexts that share workspaces, take turns: the arrays that a call is
-given reach the library together, and no other call's launches come between those of one call."""
+given reach the library together, and no other call's launches come between those of one call. And a call may be the first thing
+that a thread does with the GPU."""
 import contextlib
 import ctypes
 import threading
 import time
 
+import pytest
 import torch
 
 import hashattention_b200 as ha
-from hashattention_b200 import _lib, dense
+from hashattention_b200 import _lib, dense, synthetic
+from test_dense import D, Problem
 
 T = 4
 
@@ -111,3 +114,32 @@ def test_threads_on_contexts_that_share_a_workspace_take_turns(monkeypatch):
     run_threads(jobs + more)
     assert sorted(map(str, lib.seen)) == sorted(map(str, want + want_first))
     assert lib.together == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("call", ["attention of 1 node", "attention of 6 nodes", "received weights", "key hashes", "eviction", "commit"])
+def test_the_first_cuda_call_of_a_thread(device, call):
+    """A new thread has no CUDA context of its own until the runtime gives it one: the library's entry points must not need it before."""
+    n = 1 if call == "attention of 1 node" else 6
+    x = Problem(device, [700, 300], [n, n], 2, n, "chain", seed=1)
+    out, lse = x.ctx.tree_attention(x.q)
+    mass, want = x.ctx.new_mass(), x.ctx.attention_mass(x.q, lse, x.ctx.new_mass())
+    sparse = ha.SparseDecodeContext(x.cache, ha.Budget(8, 0.25, 8), synthetic.make_usa(8, D, seed=0, bf16=True).packed(device))
+    sparse.hash_prefill()
+    codes = x.cache.hash_pages.clone()
+    o2, l2 = torch.zeros_like(out), torch.zeros_like(lse)
+    words, rest = torch.zeros(2, 4, dtype=torch.int32, device=device), x.ctx.cache_evict(mass, 1000, 4, 4)
+    kept = rest[0].clone()
+    torch.cuda.synchronize()
+    run_threads([{"attention of 1 node": lambda: x.ctx.tree_attention(x.q, out=o2, lse=l2),
+                  "attention of 6 nodes": lambda: x.ctx.tree_attention(x.q, out=o2, lse=l2),
+                  "received weights": lambda: x.ctx.attention_mass(x.q, lse, mass),
+                  "key hashes": sparse.hash_prefill,
+                  "eviction": lambda: x.ctx.cache_evict(mass, 1000, 4, 4, kept=rest[0], mass_out=rest[1], lens_out=rest[2]),
+                  "commit": lambda: x.ctx.tree_commit(words, max_nodes=n)}[call]])
+    x.ctx.check_status()
+    if call.startswith("attention"):
+        assert torch.equal(o2, out) and torch.equal(l2, lse)
+    if call == "received weights":
+        assert torch.equal(mass, want)
+    assert torch.equal(x.cache.hash_pages, codes) and torch.equal(rest[0], kept)
