@@ -259,6 +259,8 @@ class DenseDecodeContext:
                 out = make(*size, HEAD_DIM, dtype=torch.bfloat16, device=self.device)
             else:
                 _check(out, "out", torch.bfloat16, (*size, HEAD_DIM), self.device)
+                if out.data_ptr() == q.data_ptr():
+                    raise ValueError("out must be another tensor than q, which is read until the last row is written")
             if lse is None:
                 lse = make(*size, dtype=torch.float32, device=self.device)
             else:

@@ -365,7 +365,7 @@ int ha_tree_mask(const int32_t* parents, const int32_t* tree_lens, int32_t batch
  * 2^88 (the weighted sums of up to 2^31 tokens, by weights of up to 2^8, are divided at the end).
  * q [batch][max_nodes][num_q_heads][128] bf16 with strides q_strides[3] = {batch, node, head} in elements (HOST array;
  * multiples of 8, the 128 elements of a row contiguous), or contiguous if NULL: a view of a fused projection will do.
- * out is contiguous. sm_scale > 0.                                                                                  */
+ * out is contiguous and does not overlap q. sm_scale > 0.                                                             */
 int ha_tree_attention(const ha_shape_t* shape, const ha_tree_t* tree, const void* q, const int64_t* q_strides,
                       const void* k_pages, const void* v_pages, const int32_t* page_table, const int32_t* seq_lens,
                       float sm_scale, void* out, float* lse, void* workspace, size_t workspace_bytes,

@@ -140,3 +140,12 @@ def test_one_clear_winner_per_row(device, n, prefix, kv_heads, power):
         want = x.v[b][:, winner[b]].transpose(0, 1).repeat_interleave(GROUP, 1)  # [n, Hq, D]
         assert torch.equal(out[b], want)
         assert bool(((lse[b].double() / (126 * 2.0 ** power) - 1).abs() <= 5 * 2.0 ** -24 + 2.0 ** -23).all())
+
+
+@pytest.mark.gpu
+def test_the_output_in_the_place_of_the_queries_is_refused(device):
+    """Queries are read again behind the first written rows where a draft's V has an infinity."""
+    x = Problem(device, [300], [6], 1, 6, seed=1)
+    q = x.q.contiguous()
+    with pytest.raises(ValueError, match="another tensor"):
+        x.ctx.tree_attention(q, x.mask, x.tree_lens, out=q)
