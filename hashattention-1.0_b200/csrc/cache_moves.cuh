@@ -277,14 +277,9 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
     for (int i = at_all; i < p.read_words; i += kAll) p.read[unit * p.read_words + i] = 0;
     if (unit == 0 && at_all == 0) *p.ticket = 0;
     const int S = evict_len(p.seq_lens, b, p.max_pages, at_all == 0 && kvh == 0, p.status);
-    if (S < 0) {  // (the same for the whole cluster) reported, and left as it is: its weights pass on
-        if (at_all == 0 && kvh == 0) p.lens_out[b] = __ldg(p.seq_lens + b);
-        if (mass_out != nullptr)
-            for (size_t i = at_all; i < pitch / 4; i += kAll) reinterpret_cast<float4*>(mass_out)[i] = __ldg(reinterpret_cast<const float4*>(mass) + i);
-        return;
-    }
-    const int stay = min(S, p.keep);
-    if (at_all == 0 && kvh == 0) p.lens_out[b] = stay;
+    // (a refused length is reported and passed on, with the whole row of weights)
+    const int stay = S < 0 ? (int)pitch : min(S, p.keep);
+    if (at_all == 0 && kvh == 0) p.lens_out[b] = S < 0 ? __ldg(p.seq_lens + b) : stay;
     if (mass_out != nullptr) {
         const int first4 = (stay + 3) & ~3;
         if (at_all < first4 - stay) mass_out[stay + at_all] = 0.0f;
@@ -292,7 +287,7 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
     }
     if (S <= p.keep) {  // (the same for the whole cluster)
         for (int i = at_all; i < stay; i += kAll) {
-            kept[i] = i;
+            if (S >= 0) kept[i] = i;
             if (mass_out != nullptr) mass_out[i] = __ldg(mass + i);
         }
         return;
