@@ -20,7 +20,8 @@
 // token that only other branches of the tree see stays with those. An infinity in a V row that a row does see is NaN in the products
 // (the lo half of its weight is negative or zero as often as not), where the average, whose weights are above zero, is
 // infinite. So a channel that came out NaN is looked up at the end, in the V rows themselves (v_classes): its average is
-// NaN if one of them is or if both infinities are among them. That reads V again, but only then.
+// NaN if one of them is, if both infinities are among them, or if one meets a weight that is zero by its score of -inf. That reads V
+// again, but only then.
 #pragma once
 
 #include "dense_common.cuh"
@@ -86,22 +87,30 @@ __device__ __forceinline__ float class_value(uint32_t c, float finite) {
     return c == 0 ? finite : (c == 1 ? INFINITY : (c == 2 ? -INFINITY : __uint_as_float(0x7fffffffu)));
 }
 // The classes of the channels 16 q .. 16 q + 15 of V over the tokens [t0, t1) of a sequence (table: its row of the page table), by a
-// whole warp, a token per lane: bit k of the lower half and bit k of the upper half.
-__device__ __noinline__ uint32_t v_classes(const __nv_bfloat16* v_pages, const int32_t* table, int num_pages, int Hkv, int kvh, int t0, int t1, int q) {
+// whole warp, a token per lane: bit k of the lower half and bit k of the upper half. For rows whose sum of weights is a number: where K is not
+// finite, their score then is -inf, and zero times an infinity is NaN.
+__device__ __noinline__ uint32_t v_classes(const __nv_bfloat16* k_pages, const __nv_bfloat16* v_pages, const int32_t* table, int num_pages, int Hkv, int kvh,
+                                           int t0, int t1, int q) {
     uint32_t found = 0;
 #pragma unroll 4
     for (int t = t0 + (int)(threadIdx.x & 31); t < t1; t += 32) {
         int page = __ldg(table + t / kPage);
         if (page < 0 || page >= num_pages) page = 0;  // (reported by the loading warp, which took the same)
-        const uint4* row = reinterpret_cast<const uint4*>(v_pages + (((size_t)page * Hkv + kvh) * kPage + t % kPage) * kHeadDim) + 2 * q;
+        const size_t at = (((size_t)page * Hkv + kvh) * kPage + t % kPage) * kHeadDim;
+        const uint4* row = reinterpret_cast<const uint4*>(v_pages + at) + 2 * q;
         const uint4 a = __ldg(row), b = __ldg(row + 1);
         if (any_nonfinite(a) || any_nonfinite(b)) {
             const uint32_t words[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            uint32_t of_token = 0;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const uint32_t lo = value_class(bf16_lo(words[k])), hi = value_class(bf16_hi(words[k]));
-                found |= ((lo & 1u) | (hi & 1u) << 1) << (2 * k) | ((lo >> 1) | (hi >> 1) << 1) << (2 * k + 16);
+                of_token |= ((lo & 1u) | (hi & 1u) << 1) << (2 * k) | ((lo >> 1) | (hi >> 1) << 1) << (2 * k + 16);
             }
+            bool weightless = false;
+#pragma unroll 1
+            for (int c = 0; c < 16; ++c) weightless |= any_nonfinite(__ldg(reinterpret_cast<const uint4*>(k_pages + at) + c));
+            found |= weightless ? of_token | __funnelshift_l(of_token, of_token, 16) : of_token;
         }
     }
     return __reduce_or_sync(0xffffffffu, found);
@@ -116,10 +125,12 @@ __device__ __forceinline__ float natural_lse(float M, float sum) {
 // The output row and log-sum-exp of (sequence, node, query head): 4 dimensions per lane.
 __device__ __forceinline__ void store_row(const TreeAttentionParams& p, int b, int node, int qh, int lane, float4 acc, float M, float L) {
     const size_t row = ((size_t)b * p.seqs.T + node) * ((size_t)p.seqs.Hkv * kGroup) + qh;
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // a row that sees nothing: zeros
-    uint2 w;
-    w.x = tc_pack_bf16(acc.x * inv, acc.y * inv);
-    w.y = tc_pack_bf16(acc.z * inv, acc.w * inv);
+    const float inv = 1.0f / L;
+    uint2 w = make_uint2(0, 0);  // a row that sees nothing, or scores of -inf only: zeros
+    if (L != 0.0f) {
+        w.x = tc_pack_bf16(acc.x * inv, acc.y * inv);
+        w.y = tc_pack_bf16(acc.z * inv, acc.w * inv);
+    }
     reinterpret_cast<uint2*>(p.out + row * kHeadDim)[lane] = w;
     if (lane == 0 && p.lse != nullptr) p.lse[row] = natural_lse(M, L);
 }
@@ -373,11 +384,11 @@ tree_attention_rows_kernel(const TreeAttentionParams p, const __grid_constant__ 
                 acc.z = fmaf(a.z, f, acc.z); acc.w = fmaf(a.w, f, acc.w);
             }
             if (__any_sync(0xffffffffu, !(acc.x == acc.x && acc.y == acc.y && acc.z == acc.z && acc.w == acc.w)) && sum >= 0.0f) {
-                // (with a sum of NaN the row is NaN; a sum of 0: scores of -inf only)
+                // (with a sum of NaN the row is NaN)
                 auto classes = [&](int t0, int t1) {  // of the lane's four channels
                     uint32_t mine = 0;
                     for (int q = 0; q < 8; ++q) {
-                        const uint32_t c = v_classes(p.v_pages, p.seqs.page_table + (size_t)seg.b * p.seqs.max_pages, p.seqs.num_pages, p.seqs.Hkv, seg.kvh, t0, t1, q);
+                        const uint32_t c = v_classes(p.k_pages, p.v_pages, p.seqs.page_table + (size_t)seg.b * p.seqs.max_pages, p.seqs.num_pages, p.seqs.Hkv, seg.kvh, t0, t1, q);
                         if (q == lane >> 2) mine = c >> (4 * (lane & 3));
                     }
                     return mine;
@@ -389,9 +400,8 @@ tree_attention_rows_kernel(const TreeAttentionParams p, const __grid_constant__ 
                 const uint4 words = dense_mask(p.seqs, seg.b, r >> 2);
                 for (int t = max(P, t0); t < t1; ++t)
                     if (dense_bit(words, t - P)) c |= classes(t, t + 1);
-                if (sum == 0.0f) acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                else acc = make_float4(class_value(class_of(c, 0), acc.x), class_value(class_of(c, 1), acc.y),
-                                       class_value(class_of(c, 2), acc.z), class_value(class_of(c, 3), acc.w));
+                acc = make_float4(class_value(class_of(c, 0), acc.x), class_value(class_of(c, 1), acc.y),
+                                  class_value(class_of(c, 2), acc.z), class_value(class_of(c, 3), acc.w));
             }
             if (seg.whole()) {
                 if (ok) store_row(p, seg.b, r >> 2, seg.kvh * kGroup + (r & 3), lane, acc, M, sum);

@@ -438,7 +438,7 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
                 const bool second = !kWide && stream_tiles(seg, 1) > 0;  // (otherwise that stream's columns hold something else)
                 const size_t out_row = ((size_t)seg.b * p.seqs.T + node) * ((size_t)p.seqs.Hkv * kGroup) + seg.kvh * kGroup + (r & 3);
                 const int row_in = (kWide ? 128 * w : 0) + r;  // of the unit
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const float inv = 1.0f / sum;
                 const uint32_t bad = s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3];
                 const int q0 = kWide ? 4 * half : 2 * group, q1 = q0 + (kWide ? 4 : 2);
 #pragma unroll 1
@@ -458,11 +458,11 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
                     }
                     nan = nan && mine && sum >= 0.0f;  // (with a sum of NaN the row is NaN)
                     if (__any_sync(0xffffffffu, nan)) {
-                        const uint32_t classes = v_classes(p.v_pages, p.seqs.page_table + (size_t)seg.b * p.seqs.max_pages, p.seqs.num_pages, p.seqs.Hkv,
+                        const uint32_t classes = v_classes(p.k_pages, p.v_pages, p.seqs.page_table + (size_t)seg.b * p.seqs.max_pages, p.seqs.num_pages, p.seqs.Hkv,
                                                            seg.kvh, seg.tile0 * kTaTile, min(P, seg.tile1 * kTaTile), q);
 #pragma unroll
                         for (int k = 0; k < 16; ++k)
-                            if (nan) acc[k] = sum == 0.0f ? 0.0f : class_value(class_of(classes, k), acc[k]);  // (0: scores of -inf only)
+                            if (nan) acc[k] = class_value(class_of(classes, k), acc[k]);
                     }
                     if (mine) {
                         if (bad != 0) {
@@ -477,14 +477,14 @@ tree_attention_tc_kernel(const TreeAttentionParams p, const __grid_constant__ CU
 #pragma unroll
                                 for (int k = 0; k < 16; ++k) {
                                     const float v = __bfloat162float(p.v_pages[at + 16 * q + k]);
-                                    acc[k] = fmaf(value_class(v) == 0 ? e : 1.0f, v, acc[k]);  // (any weight above zero: e may be one that fp32 holds as 0)
+                                    acc[k] = fmaf(value_class(v) == 0 || dot == -INFINITY ? e : 1.0f, v, acc[k]);  // (a weight that fp32 holds as 0 is not one)
                                 }
                             }
                         }
                         if (seg.whole()) {
                             uint32_t words[8];
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) words[k] = tc_pack_bf16(acc[2 * k] * inv, acc[2 * k + 1] * inv);
+                            for (int k = 0; k < 8; ++k) words[k] = sum == 0.0f ? 0u : tc_pack_bf16(acc[2 * k] * inv, acc[2 * k + 1] * inv);
                             uint4* dst = reinterpret_cast<uint4*>(p.out + out_row * kHeadDim + 16 * q);
                             dst[0] = make_uint4(words[0], words[1], words[2], words[3]);
                             dst[1] = make_uint4(words[4], words[5], words[6], words[7]);
@@ -643,8 +643,8 @@ __global__ void __launch_bounds__(kTaMergeThreads) tree_merge_tc_kernel(const Tr
                 }
                 acc = make_float4(class_value(c[0], acc.x), class_value(c[1], acc.y), class_value(c[2], acc.z), class_value(c[3], acc.w));
             }
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            s_out[lane][warp] = make_uint2(tc_pack_bf16(acc.x * inv, acc.y * inv), tc_pack_bf16(acc.z * inv, acc.w * inv));
+            const float inv = 1.0f / sum;
+            s_out[lane][warp] = sum == 0.0f ? make_uint2(0, 0) : make_uint2(tc_pack_bf16(acc.x * inv, acc.y * inv), tc_pack_bf16(acc.z * inv, acc.w * inv));
             if (d4 == 0 && row0 + lane < rows && p.lse != nullptr) p.lse[out_row(row0 + lane)] = natural_lse(M, sum);
         }
         __syncthreads();  // (and the other half's results have been read)

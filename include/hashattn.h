@@ -360,7 +360,7 @@ int ha_tree_mask(const int32_t* parents, const int32_t* tree_lens, int32_t batch
 /* out[b][i][h] = softmax(sm_scale * q[b][i][h] . K) V over the prefix and the nodes that node i sees, fp32 sums, bf16 output;
  * lse (optional) [batch][max_nodes][num_q_heads] f32: the natural log of the sum of e^(scaled scores). Rows of nodes behind
  * a tree's own are left as they were. A row that sees nothing (or only scores of -inf) gives zeros and an lse of -inf.
- * An infinity in a V row that a row sees makes that channel infinite, and NaN where it meets the other one or a NaN.
+ * An infinity in a V row that a row sees makes that channel infinite, and NaN where it meets the other one, a NaN or a score of -inf.
  * Scaled scores of magnitudes up to 2^29 (beyond, half an ulp of one is more than fp32 has exponents for), and V values of up to
  * 2^88 (the weighted sums of up to 2^31 tokens, by weights of up to 2^8, are divided at the end).
  * q [batch][max_nodes][num_q_heads][128] bf16 with strides q_strides[3] = {batch, node, head} in elements (HOST array;

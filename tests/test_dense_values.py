@@ -149,3 +149,28 @@ def test_the_output_in_the_place_of_the_queries_is_refused(device):
     q = x.q.contiguous()
     with pytest.raises(ValueError, match="another tensor"):
         x.ctx.tree_attention(q, x.mask, x.tree_lens, out=q)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 3, 6, 40])
+@pytest.mark.parametrize("prefix", [0, 500, 9000])
+def test_infinite_values_under_scores_of_minus_infinity(device, n, prefix):
+    """K of -inf against q above zero: a weight of zero, and zero times an infinity is NaN. A row whose scores are all -inf is zeros."""
+    x = Problem(device, [prefix + n, 200 + n], [n, n], 2, n, "chain", seed=n + prefix)
+    x.q[..., 7] = x.q[..., 7].abs() + 0.5
+    S, leaf = prefix + n, prefix + n - 1
+    if prefix:
+        x.k[0][0, 30, 7], x.v[0][0, 30, 3] = -math.inf, math.inf           # weightless: NaN
+        x.k[0][0, prefix - 1, 7] = -math.inf                                # weightless beside finite values: nothing
+        x.v[0][0, 60, 9] = math.inf                                         # infinite
+        x.v[0][0, 61, 3] = math.inf
+    x.k[0][0, leaf, 7], x.v[0][0, leaf, 11] = -math.inf, -math.inf
+    x.k[1][1, :, 7], x.v[1][1, ::3, 20] = -math.inf, math.inf               # every score of a kv-head
+    x.write(0)
+    x.write(1)
+    out, lse = x.ctx.tree_attention(x.q, x.mask, x.tree_lens)
+    assert bool((out[1, :, GROUP:] == 0).all()) and bool((lse[1, :, GROUP:] == -math.inf).all())
+    x.lens, x.nodes = [S, 0], [n, 0]  # (the definition's 0 / 0 of the second one has been looked at)
+    out[1] = lse[1] = 0
+    if S > 1:
+        x.check(out, lse)
