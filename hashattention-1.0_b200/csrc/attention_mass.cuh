@@ -60,14 +60,15 @@ constexpr int kMassBarRead = kMassBarS + 4;                   // [2 groups][2 bu
 constexpr int kMassBarQ = kMassBarRead + 4;                   // 16 warps: the unit's queries are in place
 constexpr int kMassBarFinal = kMassBarQ + 1;
 constexpr int kMassBars = kMassBarFinal + 1;
-constexpr uint32_t kMassOffLse = 0;                                    // [512] -lse in powers of two, rounded; -inf where there is no row
+constexpr uint32_t kMassOffLse = 0;                                    // [512] -lse in powers of two, rounded; -inf where there is no row or it is NaN
 constexpr uint32_t kMassOffNode = kMassOffLse + kMassMaxRows * 4;      // [128] the counted nodes
 constexpr uint32_t kMassOffVis = kMassOffNode + kMaxNodes * 4;         // [128 drafts] counted nodes that see the draft, one bit each
 constexpr uint32_t kMassOffPart = kMassOffVis + kMaxNodes * 16;        // [2 groups][2 tiles][128] sums of the second half of the columns;
                                                                        // in front of a unit's tiles: [128] mask words of the counted nodes
 constexpr uint32_t kMassOffBar = kMassOffPart + 2 * 2 * 128 * 4;
 constexpr uint32_t kMassOffTmem = kMassOffBar + kMassBars * 8;
-constexpr uint32_t kMassOffRing = (kMassOffTmem + 8 + 1023) / 1024 * 1024;
+constexpr uint32_t kMassOffNan = (kMassOffTmem + 8 + 15) / 16 * 16;    // counted nodes with a row whose log-sum-exp is NaN, one bit each
+constexpr uint32_t kMassOffRing = (kMassOffNan + 16 + 1023) / 1024 * 1024;
 __host__ __device__ constexpr size_t mass_smem_bytes(int slots, int q_rows) { return kMassOffRing + (size_t)slots * kMassSlot + (size_t)q_rows * 256 + 1024; }
 inline int mass_slots(int q_rows) {
     int slots = kMassMaxSlots;
@@ -98,6 +99,7 @@ __global__ void __launch_bounds__(kMassThreads, 1) attention_mass_kernel(const A
     uint4* s_mask = reinterpret_cast<uint4*>(smem + kMassOffPart);
     uint4* s_vis = reinterpret_cast<uint4*>(smem + kMassOffVis);
     float* s_part = reinterpret_cast<float*>(smem + kMassOffPart);
+    uint32_t* s_nan = reinterpret_cast<uint32_t*>(smem + kMassOffNan);
     auto bar = [&](int i) { return bars + 8u * (uint32_t)i; };
     if (tid == 0) {
         auto init = [&](int first, int n, uint32_t count) {
@@ -247,11 +249,13 @@ __global__ void __launch_bounds__(kMassThreads, 1) attention_mass_kernel(const A
                                                                      (seg.kvh * kGroup + (row & 3)) * p.q_head) + c);
                 *reinterpret_cast<uint4*>(smem + off_q + (c >> 3) * q_half + tc_swizzled(qr, c & 7)) = v;
             }
+            bool nan_row = false;
             if (t_all < padded) {
                 float l = -INFINITY;  // (so too for a row that sees nothing)
                 if (t_all < rows) {
                     const float lse = __ldg(p.lse + ((size_t)seg.b * p.seqs.T + s_node[t_all >> 2]) * ((size_t)p.seqs.Hkv * kGroup) + seg.kvh * kGroup + (t_all & 3));
-                    if (lse != -INFINITY) l = -(float)((double)lse * p.lse_scale);
+                    nan_row = lse != lse;
+                    if (lse != -INFINITY && !nan_row) l = -(float)((double)lse * p.lse_scale);
                 }
                 s_lse[t_all] = l;
             }
@@ -337,9 +341,25 @@ __global__ void __launch_bounds__(kMassThreads, 1) attention_mass_kernel(const A
                 float* others = s_part + (2 * g + ((i >> 1) & 1)) * 128;  // (written again two tiles on, behind a barrier of the one between)
                 if (part == 1) others[r] = sum;
                 asm volatile("bar.sync %0, 64;" ::"r"(2 + 4 * g + quarter) : "memory");
-                if (part == 0 && ok && j < seg.S) atomicAdd(mass + j, sum + others[r]);  // (no other thread of the call adds to it)
+                if (part == 0 && ok && j < seg.S) atomicAdd(mass + j, sum + others[r]);  // (no other thread of the call adds a number to it)
             }
-            asm volatile("bar.sync 1, 512;" ::: "memory");
+            // A row whose log-sum-exp is NaN makes NaN of the tokens that it sees. (In the exponent, where tokens that a row does not
+            // see are taken out by -inf, it would make NaN of those too.) The barrier at the end of a unit tells whether there is one.
+            uint32_t any_nan;
+            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 512, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                         : "=r"(any_nan) : "r"(nan_row ? 1u : 0u) : "memory");
+            if (any_nan != 0) {
+                if (t_all < kMaskWords) s_nan[t_all] = 0;
+                asm volatile("bar.sync 1, 512;" ::: "memory");
+                if (nan_row) atomicOr(&s_nan[t_all >> 7], 1u << ((t_all >> 2) & 31));
+                asm volatile("bar.sync 1, 512;" ::: "memory");
+                const uint4 nan = *reinterpret_cast<const uint4*>(s_nan);
+                for (int j = seg.tile0 * kMassTile + t_all; j < min(seg.S, seg.tile1 * kMassTile); j += kMassWarps * 32) {
+                    const uint4 v = j < P ? nan : s_vis[j - P];
+                    if (((v.x & nan.x) | (v.y & nan.y) | (v.z & nan.z) | (v.w & nan.w)) != 0) atomicAdd(mass + j, __uint_as_float(0x7fffffffu));
+                }
+                asm volatile("bar.sync 1, 512;" ::: "memory");
+            }
         }
     }
 

@@ -374,8 +374,9 @@ int ha_tree_attention(const ha_shape_t* shape, const ha_tree_t* tree, const void
 /* mass[b][j][t] += sum over the counted nodes i and the query heads h of kv-head j of the weight e^(score - lse[b][i][h])
  * that cached token t has in row (i, h); mass [batch][num_kv_heads][max_pages * page_size] f32. rows (optional) [batch][4]:
  * the nodes whose weights count, one bit each (an accepted path); NULL: all of the tree. q, q_strides, sm_scale, the tree
- * and lse as ha_tree_attention took and left them. Rows with an lse of -inf count for nothing. A weight is off by what the
- * rounding of score and lse to fp32 makes of it: about 2^-23 of their magnitude, relative to the weight.                */
+ * and lse as ha_tree_attention took and left them. Rows with an lse of -inf count for nothing, rows with one of NaN make NaN
+ * of what they see. A weight is off by what the rounding of score and lse to fp32 makes of it: about 2^-23 of their magnitude,
+ * relative to the weight.                                                                                            */
 int ha_attention_mass(const ha_shape_t* shape, const ha_tree_t* tree, const void* q, const int64_t* q_strides,
                       const float* lse, const uint32_t* rows, const void* k_pages, const int32_t* page_table,
                       const int32_t* seq_lens, float sm_scale, float* mass, int32_t* status, void* stream);

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import hashattention_b200 as ha
-from test_dense import D, GROUP, Problem
+from test_dense import D, GROUP, Problem, score_error, weights64
 
 
 def plant(x, b, spots):
@@ -174,3 +174,30 @@ def test_infinite_values_under_scores_of_minus_infinity(device, n, prefix):
     out[1] = lse[1] = 0
     if S > 1:
         x.check(out, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 5, 20, 64, 128])
+@pytest.mark.parametrize("prefix", [0, 300, 3000])
+def test_received_weights_of_rows_that_are_nan(device, n, prefix):
+    """A row whose log-sum-exp is NaN gives NaN to the tokens it sees and nothing to the others."""
+    x = Problem(device, [prefix + n, 100 + n], [n, n], 2, n, "tree", seed=n + prefix)
+    leaf, mid = n - 1, n // 2
+    x.k[0][0, prefix + leaf, 5] = math.nan   # kv-head 0: the rows that see the leaf (itself)
+    x.q[0, mid, GROUP + 1, 3] = math.nan     # kv-head 1: one row of one node
+    x.write(0)
+    _, lse = x.ctx.tree_attention(x.q, x.mask, x.tree_lens)
+    mass = x.ctx.attention_mass(x.q, lse, x.ctx.new_mass(), x.mask, x.tree_lens)
+    x.ctx.check_status()
+    sees, S = x.sees(0), prefix + n
+    p, _ = weights64(x.q[0], x.k[0], sees, x.scale)           # [n, Hq, S], NaN in the rows that are
+    nan_rows = torch.isnan(lse[0])                             # [n, Hq]
+    assert nan_rows.nonzero().tolist() == sorted([[leaf, h] for h in range(GROUP)] + [[mid, GROUP + 1]])
+    p = torch.where(nan_rows[..., None], torch.where(sees[:, None], math.nan, 0.0).double(), p)
+    want = p.view(n, 2, GROUP, S).sum((0, 2))
+    got = mass[0, :, :S].double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    d = score_error(x.q[0].nan_to_num(), x.k[0].nan_to_num(), x.scale)
+    fine = ~torch.isnan(want)
+    assert bool(((got - want).abs()[fine] <= (want * (2 * d + 2.0 ** -18 + 513 * 2.0 ** -24))[fine]).all())
+    assert bool(torch.isfinite(mass[1]).all()) and bool((mass[0, :, S:] == 0).all())
