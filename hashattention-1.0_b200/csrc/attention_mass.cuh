@@ -85,6 +85,22 @@ __device__ __forceinline__ uint4 counted_nodes(const uint32_t* rows, int b, int 
     return set;
 }
 
+// A row whose log-sum-exp is NaN makes NaN of the tokens [j0, j1) that it sees. (In the exponent, where tokens that a row does not
+// see are taken out by -inf, it would make NaN of those too.) By the threads that form weights; out of line, so that the kernel's end, whose
+// instructions come from memory, stays short.
+__device__ __noinline__ void mass_of_nan_rows(uint32_t* s_nan, const uint4* s_vis, bool nan_row, int t_all, float* mass, int j0, int j1, int P) {
+    if (t_all < kMaskWords) s_nan[t_all] = 0;
+    asm volatile("bar.sync 1, 512;" ::: "memory");
+    if (nan_row) atomicOr(&s_nan[t_all >> 7], 1u << ((t_all >> 2) & 31));
+    asm volatile("bar.sync 1, 512;" ::: "memory");
+    const uint4 nan = *reinterpret_cast<const uint4*>(s_nan);
+    for (int j = j0 + t_all; j < j1; j += kMassWarps * 32) {
+        const uint4 v = j < P ? nan : s_vis[j - P];
+        if (((v.x & nan.x) | (v.y & nan.y) | (v.z & nan.z) | (v.w & nan.w)) != 0) atomicAdd(mass + j, __uint_as_float(0x7fffffffu));
+    }
+    asm volatile("bar.sync 1, 512;" ::: "memory");
+}
+
 __global__ void __launch_bounds__(kMassThreads, 1) attention_mass_kernel(const AttentionMassParams p, const __grid_constant__ CUtensorMap k_map) {
     using Cursor = DenseCursor<kMassTile, kMassMaxRows, 0>;
     extern __shared__ unsigned char mass_smem_raw[];
@@ -343,23 +359,11 @@ __global__ void __launch_bounds__(kMassThreads, 1) attention_mass_kernel(const A
                 asm volatile("bar.sync %0, 64;" ::"r"(2 + 4 * g + quarter) : "memory");
                 if (part == 0 && ok && j < seg.S) atomicAdd(mass + j, sum + others[r]);  // (no other thread of the call adds a number to it)
             }
-            // A row whose log-sum-exp is NaN makes NaN of the tokens that it sees. (In the exponent, where tokens that a row does not
-            // see are taken out by -inf, it would make NaN of those too.) The barrier at the end of a unit tells whether there is one.
+            // (the barrier at the end of a unit tells whether it has a row that is NaN)
             uint32_t any_nan;
             asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 512, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
                          : "=r"(any_nan) : "r"(nan_row ? 1u : 0u) : "memory");
-            if (any_nan != 0) {
-                if (t_all < kMaskWords) s_nan[t_all] = 0;
-                asm volatile("bar.sync 1, 512;" ::: "memory");
-                if (nan_row) atomicOr(&s_nan[t_all >> 7], 1u << ((t_all >> 2) & 31));
-                asm volatile("bar.sync 1, 512;" ::: "memory");
-                const uint4 nan = *reinterpret_cast<const uint4*>(s_nan);
-                for (int j = seg.tile0 * kMassTile + t_all; j < min(seg.S, seg.tile1 * kMassTile); j += kMassWarps * 32) {
-                    const uint4 v = j < P ? nan : s_vis[j - P];
-                    if (((v.x & nan.x) | (v.y & nan.y) | (v.z & nan.z) | (v.w & nan.w)) != 0) atomicAdd(mass + j, __uint_as_float(0x7fffffffu));
-                }
-                asm volatile("bar.sync 1, 512;" ::: "memory");
-            }
+            if (any_nan != 0) mass_of_nan_rows(s_nan, s_vis, nan_row, t_all, mass, seg.tile0 * kMassTile, min(seg.S, seg.tile1 * kMassTile), P);
         }
     }
 

@@ -259,8 +259,9 @@ class DenseDecodeContext:
                 out = make(*size, HEAD_DIM, dtype=torch.bfloat16, device=self.device)
             else:
                 _check(out, "out", torch.bfloat16, (*size, HEAD_DIM), self.device)
-                if out.data_ptr() == q.data_ptr():
-                    raise ValueError("out must be another tensor than q, which is read until the last row is written")
+            q_ptr, out_ptr = q.data_ptr(), out.data_ptr()
+            if q_ptr == out_ptr:
+                raise ValueError("out must be another tensor than q, which is read until the last row is written")
             if lse is None:
                 lse = make(*size, dtype=torch.float32, device=self.device)
             else:
@@ -268,8 +269,8 @@ class DenseDecodeContext:
             c = self.cache
             with library_call(self.device, "ha_tree_attention"):
                 rc = self.lib.ha_tree_attention(
-                    self._shape_ref, tree, q.data_ptr(), strides, c.k_pages.data_ptr(), c.v_pages.data_ptr(), c.page_table.data_ptr(),
-                    c.seq_lens.data_ptr(), self.sm_scale, out.data_ptr(), lse.data_ptr(), self._workspace_ptr,
+                    self._shape_ref, tree, q_ptr, strides, c.k_pages.data_ptr(), c.v_pages.data_ptr(), c.page_table.data_ptr(),
+                    c.seq_lens.data_ptr(), self.sm_scale, out_ptr, lse.data_ptr(), self._workspace_ptr,
                     self.workspace_bytes, self._status_ptr, _stream_ptr(self.device))
         _raise_on(rc, "ha_tree_attention")
         return out, lse
